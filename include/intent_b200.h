@@ -45,6 +45,8 @@ extern "C" {
 #define B200_F32 0
 #define B200_F16 1
 #define B200_BF16 2
+#define B200_I8 3   /* codes of an 8-bit cache */
+#define B200_E4M3 4
 
 /* Number of int32 words every workspace view must hold (zero-initialised by
    the caller once; word 0 is a sticky device-side status, see b200_workspace_status). */
@@ -283,6 +285,131 @@ int b200_flash_attention(const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2
                          int32_t dtype, int32_t head_group, int32_t causal, void *stream);
 
 /*
+ * RMS norm of every query and key head and the rotation by the token's position, one pass over q and
+ * k (tokens, heads, D):   z = x / sqrt(mean(x^2) + epsilon) * weight,   y = R(position) z.
+ * R turns pair i < cosine_d1 by the angle whose cosine and sine stand at [position, i] of the f32
+ * tables (rows, pairs); the pairs are columns (i, i + pairs), or (2i, 2i + 1) with `interleaved`;
+ * columns from 2 * pairs on pass.  f32 arithmetic, one rounding.  No counterpart in the reference.
+ * positions: int32.  A negative one marks padding: its rows become zeros.  So do the rows of a
+ * position behind the tables, which is also recorded in the workspace (b200_workspace_status).
+ * D a multiple of 16 in [16, 256], pairs a multiple of 8; unit inner strides, 16-byte aligned bases,
+ * outer strides of whole 16-byte steps.  An output may be its own input view, and otherwise overlaps
+ * no operand.  q and k may be slices of one tensor, and so may the outputs.
+ */
+int b200_head_norm_rotary(
+    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
+    const void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
+    const void *q_weight, int64_t q_weight_d0, int64_t q_weight_s0,
+    const void *k_weight, int64_t k_weight_d0, int64_t k_weight_s0,
+    const void *cosine, int64_t cosine_d0, int64_t cosine_d1, int64_t cosine_s0, int64_t cosine_s1,
+    const void *sine, int64_t sine_d0, int64_t sine_d1, int64_t sine_s0, int64_t sine_s1,
+    const void *positions, int64_t positions_d0, int64_t positions_s0,
+    void *q_out, int64_t q_out_d0, int64_t q_out_d1, int64_t q_out_d2, int64_t q_out_s0, int64_t q_out_s1, int64_t q_out_s2,
+    void *k_out, int64_t k_out_d0, int64_t k_out_d1, int64_t k_out_d2, int64_t k_out_s0, int64_t k_out_s1, int64_t k_out_s2,
+    float epsilon, void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t interleaved, void *stream);
+
+/*
+ * Its backward pass, from the gradients of both outputs: with g = R^T dy, u = g * weight and
+ * r = 1 / sqrt(mean(x^2) + epsilon),
+ *   dx = r (u - x r mean(u x r)),   dweight = sum over tokens and heads of g x r   (f32).
+ * Rows of padding get zeros and add nothing.  partial: f32 scratch of (rows, D) contiguous,
+ * rows as b200_head_norm_rotary_scratch says for this device; the weights' sums are taken in a fixed
+ * order, so results do not vary.  Layout rules are the forward entry's; dq and dk may be the gradient
+ * or input view of the same rows.
+ */
+int b200_head_norm_rotary_scratch(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t *rows);
+int b200_head_norm_rotary_backward(
+    const void *grad_q, int64_t grad_q_d0, int64_t grad_q_d1, int64_t grad_q_d2, int64_t grad_q_s0, int64_t grad_q_s1, int64_t grad_q_s2,
+    const void *grad_k, int64_t grad_k_d0, int64_t grad_k_d1, int64_t grad_k_d2, int64_t grad_k_s0, int64_t grad_k_s1, int64_t grad_k_s2,
+    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
+    const void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
+    const void *q_weight, int64_t q_weight_d0, int64_t q_weight_s0,
+    const void *k_weight, int64_t k_weight_d0, int64_t k_weight_s0,
+    const void *cosine, int64_t cosine_d0, int64_t cosine_d1, int64_t cosine_s0, int64_t cosine_s1,
+    const void *sine, int64_t sine_d0, int64_t sine_d1, int64_t sine_s0, int64_t sine_s1,
+    const void *positions, int64_t positions_d0, int64_t positions_s0,
+    void *dq, int64_t dq_d0, int64_t dq_d1, int64_t dq_d2, int64_t dq_s0, int64_t dq_s1, int64_t dq_s2,
+    void *dk, int64_t dk_d0, int64_t dk_d1, int64_t dk_d2, int64_t dk_s0, int64_t dk_s1, int64_t dk_s2,
+    void *dq_weight, int64_t dq_weight_d0, int64_t dq_weight_s0, void *dk_weight, int64_t dk_weight_d0, int64_t dk_weight_s0,
+    void *partial, int64_t partial_d0, int64_t partial_d1, int64_t partial_s0, int64_t partial_s1,
+    float epsilon, void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t interleaved, void *stream);
+
+/*
+ * Rows of keys and values (tokens, heads, D), f16 or bf16, into the slots of a paged cache
+ * (pages, heads, page_size, D); slot = page * page_size + place, int64.  `store` is the cache's type:
+ * the rows' own (a copy; scales are ignored), or B200_I8 / B200_E4M3 with f32 scales
+ * (pages, heads, page_size), one for each row:
+ *   i8:   scale = max(f32(amax / 127), 2^-126)          e4m3: scale = 2^max(ceil(log2(amax / 448)), -126)
+ *   code = x / scale rounded to the nearest, ties to even.  A row that holds an infinity or a NaN gets the
+ *   scale NaN and codes 0.
+ * A negative slot marks padding, whose row is not written; nor is the row of a slot behind the cache,
+ * which is recorded in the workspace.  The slots of one call that are not negative must differ: what a
+ * slot holds that is named twice is unspecified.  D a multiple of 16 in [16, 256]; unit inner strides,
+ * 16-byte aligned bases, outer strides of whole 16-byte steps.  Key and value cache may be parts of
+ * one allocation.  No counterpart in the reference.
+ */
+int b200_cache_write(
+    const void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
+    const void *v, int64_t v_d0, int64_t v_d1, int64_t v_d2, int64_t v_s0, int64_t v_s1, int64_t v_s2,
+    const void *slots, int64_t slots_d0, int64_t slots_s0,
+    void *k_cache, int64_t k_cache_d0, int64_t k_cache_d1, int64_t k_cache_d2, int64_t k_cache_d3,
+    int64_t k_cache_s0, int64_t k_cache_s1, int64_t k_cache_s2, int64_t k_cache_s3,
+    void *v_cache, int64_t v_cache_d0, int64_t v_cache_d1, int64_t v_cache_d2, int64_t v_cache_d3,
+    int64_t v_cache_s0, int64_t v_cache_s1, int64_t v_cache_s2, int64_t v_cache_s3,
+    void *k_scale, int64_t k_scale_d0, int64_t k_scale_d1, int64_t k_scale_d2, int64_t k_scale_s0, int64_t k_scale_s1, int64_t k_scale_s2,
+    void *v_scale, int64_t v_scale_d0, int64_t v_scale_d1, int64_t v_scale_d2, int64_t v_scale_s0, int64_t v_scale_s1, int64_t v_scale_s2,
+    void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t store, void *stream);
+
+/*
+ * The rows of `slots` back out of the cache, as f16 or bf16 (of a 16-bit cache: its own type);
+ * code * scale in f32, rounded once.  Padding (a negative slot) and slots behind the cache, which are
+ * recorded in the workspace, give zeros.  A slot may be named any number of times.
+ */
+int b200_cache_read(
+    const void *k_cache, int64_t k_cache_d0, int64_t k_cache_d1, int64_t k_cache_d2, int64_t k_cache_d3,
+    int64_t k_cache_s0, int64_t k_cache_s1, int64_t k_cache_s2, int64_t k_cache_s3,
+    const void *v_cache, int64_t v_cache_d0, int64_t v_cache_d1, int64_t v_cache_d2, int64_t v_cache_d3,
+    int64_t v_cache_s0, int64_t v_cache_s1, int64_t v_cache_s2, int64_t v_cache_s3,
+    const void *slots, int64_t slots_d0, int64_t slots_s0,
+    const void *k_scale, int64_t k_scale_d0, int64_t k_scale_d1, int64_t k_scale_d2, int64_t k_scale_s0, int64_t k_scale_s1, int64_t k_scale_s2,
+    const void *v_scale, int64_t v_scale_d0, int64_t v_scale_d1, int64_t v_scale_d2, int64_t v_scale_s0, int64_t v_scale_s1, int64_t v_scale_s2,
+    void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
+    void *v, int64_t v_d0, int64_t v_d1, int64_t v_d2, int64_t v_s0, int64_t v_s1, int64_t v_s2,
+    void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t store, void *stream);
+
+/*
+ * Attention of one new token a sequence: q (batch, heads, D) over the first lengths[b] rows of each
+ * sequence, which lie in the pages that row b of block_table (int32) names, in the cache that
+ * b200_cache_write fills.  heads is a multiple of the cache's heads; query head h reads key head
+ * h / (heads / kv_heads).   s = scale * q . k,  out = softmax(s) . v,  lse = log(sum(e^s)) (f32, natural
+ * logarithm; lse may be null).  A sequence of length 0 (or less) gets zeros and -infinity.  Nothing
+ * past a sequence's length is read into a result, whatever it holds; entries of block_table past it may have any
+ * value.  An entry within it that is no page counts its positions as absent, a length
+ * greater than the table's columns * page_size counts as that, and both are recorded in the
+ * workspace.  D is 64 or 128; f32 arithmetic, the softmax weights enter the products with 16 bits or
+ * more (see the kernel), one rounding at the end; sums are joined in a fixed order, so results do not vary.
+ * partial: 16-byte aligned scratch, f32 words as b200_paged_attention_scratch says for this device
+ * (keys = table columns * page_size).  Calls that may overlap need scratch of their own each.
+ * No counterpart in the reference.
+ */
+int b200_paged_attention_scratch(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t keys,
+                                            int32_t store, int64_t *words);
+int b200_paged_attention(
+    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
+    const void *k_cache, int64_t k_cache_d0, int64_t k_cache_d1, int64_t k_cache_d2, int64_t k_cache_d3,
+    int64_t k_cache_s0, int64_t k_cache_s1, int64_t k_cache_s2, int64_t k_cache_s3,
+    const void *v_cache, int64_t v_cache_d0, int64_t v_cache_d1, int64_t v_cache_d2, int64_t v_cache_d3,
+    int64_t v_cache_s0, int64_t v_cache_s1, int64_t v_cache_s2, int64_t v_cache_s3,
+    const void *k_scale, int64_t k_scale_d0, int64_t k_scale_d1, int64_t k_scale_d2, int64_t k_scale_s0, int64_t k_scale_s1, int64_t k_scale_s2,
+    const void *v_scale, int64_t v_scale_d0, int64_t v_scale_d1, int64_t v_scale_d2, int64_t v_scale_s0, int64_t v_scale_s1, int64_t v_scale_s2,
+    const void *block_table, int64_t table_d0, int64_t table_d1, int64_t table_s0, int64_t table_s1,
+    const void *lengths, int64_t lengths_d0, int64_t lengths_s0,
+    void *out, int64_t out_d0, int64_t out_d1, int64_t out_d2, int64_t out_s0, int64_t out_s1, int64_t out_s2,
+    void *lse, int64_t lse_d0, int64_t lse_d1, int64_t lse_s0, int64_t lse_s1,
+    float scale, void *partial, int64_t partial_d0, int64_t partial_s0, void *workspace, int64_t ws_d0, int64_t ws_s0,
+    int32_t dtype, int32_t store, void *stream);
+
+/*
  * CSR SpMM  Y = A . X, i32 indices, f32 values, strict source-order
  * accumulation per row with an unfused multiply then add, so results are
  * bit-identical to a sequential left-to-right evaluation.  Replaces csr_spmm
@@ -355,9 +482,12 @@ int b200_gather_probe(const void *table, int64_t table_rows, int64_t gathers, in
 int b200_selftest_bounded_wait(void *workspace, int64_t ws_d0, int64_t ws_s0, int64_t limit_cycles, void *stream);
 
 /*
- * Reads word 0 of a workspace after synchronising `stream`: B200_OK, or
- * B200_ERR_DEVICE_TIMEOUT when a bounded wait inside a kernel gave up.
- * `detail` (may be null) receives word 1, which names the wait that ran out.
+ * Reads word 0 of a workspace after synchronising `stream`: B200_OK,
+ * B200_ERR_DEVICE_TIMEOUT when a bounded wait inside a kernel gave up, or
+ * B200_ERR_INVALID_ARGUMENT when a kernel met a position, slot, page or length outside
+ * its table or cache and left it out.
+ * `detail` (may be null) receives word 1, which names the wait that ran out, or the
+ * token or sequence.
  */
 int b200_workspace_status(const void *workspace, int32_t *detail, void *stream);
 

@@ -1,0 +1,164 @@
+// Rows of attention heads: views, 16-column pieces of a row held by one lane, argument checks.
+// Shared by the per-head norm and rotation, the paged cache and the attention over it.
+#pragma once
+
+#include <math.h>
+
+#include "common.cuh"
+
+namespace b200 {
+namespace heads {
+
+// ---- host: views as the ABI passes them -----------------------------------
+struct View3 {
+  const void *data;
+  int64_t d0, d1, d2, s0, s1, s2;
+};
+struct View4 {
+  const void *data;
+  int64_t d0, d1, d2, d3, s0, s1, s2, s3;
+};
+
+inline int element_size(int dtype) { return dtype == B200_F32 ? 4 : dtype == B200_F16 || dtype == B200_BF16 ? 2 : 1; }
+
+// Every stride times extent stays far from the end of 64 bits, whatever the caller passes.
+inline bool sane(int64_t extent, int64_t stride) {
+  return extent >= 0 && extent < (int64_t(1) << 40) && stride > -(int64_t(1) << 40) && stride < (int64_t(1) << 40) &&
+         (extent <= 1 || llabs(stride) <= (int64_t(1) << 60) / extent);
+}
+inline bool sane(const View3 &v) { return sane(v.d0, v.s0) && sane(v.d1, v.s1) && sane(v.d2, v.s2); }
+inline bool sane(const View4 &v) { return sane(v.d0, v.s0) && sane(v.d1, v.s1) && sane(v.d2, v.s2) && sane(v.d3, v.s3); }
+
+// Rows move as 128-bit vectors: unit innermost stride, 16-byte aligned base and outer strides.
+inline bool vector_rows(const View3 &v, int size) {
+  const int64_t step = 16 / size;
+  return v.s2 == 1 && aligned16(v.data) && (v.d0 <= 1 || v.s0 % step == 0) && (v.d1 <= 1 || v.s1 % step == 0);
+}
+inline bool vector_rows(const View4 &v, int size) {
+  const int64_t step = 16 / size;
+  return v.s3 == 1 && aligned16(v.data) && (v.d0 <= 1 || v.s0 % step == 0) && (v.d1 <= 1 || v.s1 % step == 0) &&
+         (v.d2 <= 1 || v.s2 % step == 0);
+}
+
+struct Span {
+  uintptr_t begin, end;
+};
+inline Span span(const void *data, int size, int count, const int64_t *extents, const int64_t *strides) {
+  int64_t low = 0, high = 0;
+  for (int i = 0; i < count; ++i) {
+    if (extents[i] == 0) return {0, 0};
+    const int64_t reach = (extents[i] - 1) * strides[i];
+    (reach < 0 ? low : high) += reach;
+  }
+  const uintptr_t base = reinterpret_cast<uintptr_t>(data);
+  return {base + low * size, base + (high + 1) * size};
+}
+inline Span span(const View3 &v, int size) {
+  const int64_t extents[] = {v.d0, v.d1, v.d2}, strides[] = {v.s0, v.s1, v.s2};
+  return span(v.data, size, 3, extents, strides);
+}
+inline Span span(const View4 &v, int size) {
+  const int64_t extents[] = {v.d0, v.d1, v.d2, v.d3}, strides[] = {v.s0, v.s1, v.s2, v.s3};
+  return span(v.data, size, 4, extents, strides);
+}
+inline bool overlap(const Span &a, const Span &b) { return a.begin < b.end && b.begin < a.end; }
+
+// Whether two elements of a view that is written share an address: a sufficient test that every
+// layout made by permuting and slicing a dense tensor passes.  Axes in the order of their strides;
+// each must step over all that the smaller ones reach.
+inline bool distinct(int count, const int64_t *extents, const int64_t *strides) {
+  int order[5];
+  for (int i = 0; i < count; ++i) {
+    if (extents[i] == 0) return true;
+    order[i] = i;
+  }
+  for (int i = 1; i < count; ++i)
+    for (int j = i; j > 0 && llabs(strides[order[j]]) < llabs(strides[order[j - 1]]); --j) {
+      const int other = order[j];
+      order[j] = order[j - 1];
+      order[j - 1] = other;
+    }
+  int64_t reach = 0;
+  for (int i = 0; i < count; ++i) {
+    const int axis = order[i];
+    if (extents[axis] == 1) continue;
+    if (llabs(strides[axis]) <= reach) return false;
+    reach += (extents[axis] - 1) * llabs(strides[axis]);
+  }
+  return true;
+}
+inline bool distinct(const View3 &v) {
+  const int64_t extents[] = {v.d0, v.d1, v.d2}, strides[] = {v.s0, v.s1, v.s2};
+  return distinct(3, extents, strides);
+}
+inline bool distinct(const View4 &v) {
+  const int64_t extents[] = {v.d0, v.d1, v.d2, v.d3}, strides[] = {v.s0, v.s1, v.s2, v.s3};
+  return distinct(4, extents, strides);
+}
+
+// Whether two views that are written share no element, by a sufficient test: they lie apart, or they
+// have one shape and one layout and interleave (keys and values of one allocation).
+inline bool apart(const View4 &a, const View4 &b, int size) {
+  if (!overlap(span(a, size), span(b, size))) return true;
+  const int64_t extents[] = {a.d0, a.d1, a.d2, a.d3, 2};
+  const int64_t strides[] = {a.s0, a.s1, a.s2, a.s3, ((const char *)b.data - (const char *)a.data) / size};
+  if (a.d0 != b.d0 || a.d1 != b.d1 || a.d2 != b.d2 || a.d3 != b.d3 || (a.d0 > 1 && a.s0 != b.s0) || (a.d1 > 1 && a.s1 != b.s1) ||
+      (a.d2 > 1 && a.s2 != b.s2) || (a.d3 > 1 && a.s3 != b.s3))
+    return false;
+  return distinct(5, extents, strides);
+}
+inline bool apart(const View3 &a, const View3 &b, int size) {
+  return apart(View4{a.data, a.d0, a.d1, a.d2, 1, a.s0, a.s1, a.s2, 1}, View4{b.data, b.d0, b.d1, b.d2, 1, b.s0, b.s1, b.s2, 1}, size);
+}
+
+// Lanes that share a row when each holds 16 of its columns: a power of two, so that a warp holds
+// whole rows and the sum over a row is a butterfly of shuffles.
+inline int row_lanes(int64_t columns) {
+  int lanes = 1;
+  while (lanes * 16 < columns) lanes *= 2;
+  return lanes;
+}
+
+// ---- device ------------------------------------------------------------------
+// Word 0 of the workspace becomes 3 and word 1 the position of a bad index (b200_workspace_status
+// reports it); the first one found stays.
+__device__ __forceinline__ void report_index(int *status, int position) {
+  if (atomicCAS(status, 0, 3) == 0) status[1] = position;
+}
+
+// Eight consecutive columns, as raw 128-bit vectors and as f32.
+template <typename T> struct Eight {
+  static constexpr int kVectors = 8 * sizeof(T) / 16;
+  uint4 raw[kVectors];
+  __device__ __forceinline__ void load(const T *pointer) {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) raw[i] = reinterpret_cast<const uint4 *>(pointer)[i];
+  }
+  __device__ __forceinline__ void store(T *pointer) const {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) reinterpret_cast<uint4 *>(pointer)[i] = raw[i];
+  }
+  __device__ __forceinline__ void clear() {
+#pragma unroll
+    for (int i = 0; i < kVectors; ++i) raw[i] = make_uint4(0, 0, 0, 0);
+  }
+  __device__ __forceinline__ void widen(float *out) const {
+    const T *lanes = reinterpret_cast<const T *>(raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = Element<T>::widen(lanes[i]);
+  }
+  __device__ __forceinline__ void narrow(const float *in) {
+    T *lanes = reinterpret_cast<T *>(raw);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) lanes[i] = Element<T>::narrow(in[i]);
+  }
+};
+
+template <int LANES> __device__ __forceinline__ float row_sum(float v) {
+#pragma unroll
+  for (int offset = LANES / 2; offset > 0; offset >>= 1) v += __shfl_xor_sync(0xffffffffu, v, offset);
+  return v;
+}
+
+}  // namespace heads
+}  // namespace b200

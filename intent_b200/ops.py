@@ -18,7 +18,7 @@ import torch
 
 from . import _native
 
-_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+_CODES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2, torch.int8: 3, torch.float8_e4m3fn: 4}
 
 
 def _slots(tensor: torch.Tensor) -> list:
@@ -283,6 +283,197 @@ def attention_backward_dq(q, k, v, grad_output, lse, delta, scale: float, *, hea
           *_slots(lse), *_slots(delta), *_slots(grad_q), float(scale), *_slots(space), _CODES[q.dtype],
           int(head_group), int(causal), _stream(q))
     return grad_q
+
+
+def _status_workspace(device: torch.device) -> torch.Tensor:
+    """``workspace(device)`` for entries that record a bad index there.  It is made once per device and
+    shared by all streams, so the first call may not fall into a graph capture, whose replays would
+    clear it, and its zeros have to be there before any other stream writes to it."""
+    if device not in _workspaces:
+        with torch.cuda.device(device):
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("call intent_b200.ops.workspace(device) once before capturing this operator into a graph")
+            workspace(device)
+            torch.cuda.current_stream(device).synchronize()
+    return _workspaces[device]
+
+
+def _scratch_size(name: str, device: torch.device, *arguments) -> int:
+    size = ctypes.c_int64(0)
+    _call(name, device, *arguments, ctypes.byref(size))
+    return size.value
+
+
+def _rotary_operands(q, k, q_weight, k_weight, cos, sin, positions) -> None:
+    _float_type("q", q)
+    if q.dim() != 3 or k.dim() != 3 or cos.dim() != 2:
+        raise ValueError("q and k are (tokens, heads, head_dim) tensors, cos and sin (rows, pairs)")
+    _expect("k", k, q.dtype, (q.shape[0], k.shape[1], q.shape[2]))
+    _expect("q_weight", q_weight, q.dtype, (q.shape[2],))
+    _expect("k_weight", k_weight, q.dtype, (q.shape[2],))
+    _expect("cos", cos, torch.float32)
+    _expect("sin", sin, torch.float32, cos.shape)
+    _expect("positions", positions, torch.int32, (q.shape[0],))
+
+
+def head_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, epsilon: float = 1e-6, *, interleaved: bool = False,
+                     q_out=None, k_out=None):
+    """RMS norm of every head of ``q`` and ``k`` (tokens, heads, head_dim), times its weight, and the
+    rotation by the token's position, in one launch.  ``cos`` and ``sin`` (rows, pairs) are f32 tables
+    over positions; pair ``i`` is columns ``(i, i + pairs)``, or ``(2i, 2i + 1)`` with ``interleaved``, and
+    columns from ``2 * pairs`` on are not turned.  ``positions`` (tokens,) int32: a negative one marks
+    padding, whose rows become zeros; one behind the tables gives zeros too and is reported by
+    ``workspace_status``.  Returns ``(q_out, k_out)``; an output may be its input."""
+    device = _require_cuda(q, k, q_weight, k_weight, cos, sin, positions, *(t for t in (q_out, k_out) if t is not None))
+    _rotary_operands(q, k, q_weight, k_weight, cos, sin, positions)
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    if k_out is None:
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=device)
+    _expect("q_out", q_out, q.dtype, q.shape)
+    _expect("k_out", k_out, k.dtype, k.shape)
+    _call("b200_head_norm_rotary", device, *_slots(q), *_slots(k), *_slots(q_weight), *_slots(k_weight), *_slots(cos),
+          *_slots(sin), *_slots(positions), *_slots(q_out), *_slots(k_out), float(epsilon),
+          *_slots(_status_workspace(device)), _CODES[q.dtype], int(bool(interleaved)), _stream(q))
+    return q_out, k_out
+
+
+def head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions, epsilon: float = 1e-6, *,
+                              interleaved: bool = False, dq=None, dk=None):
+    """The gradients of ``head_norm_rotary``'s inputs from those of its outputs: ``(dq, dk, dq_weight,
+    dk_weight)``, the weights' in f32.  Rows of padding get zeros and add nothing.  ``dq`` may be
+    ``grad_q`` or ``q``, and ``dk`` likewise."""
+    device = _require_cuda(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions,
+                           *(t for t in (dq, dk) if t is not None))
+    _rotary_operands(q, k, q_weight, k_weight, cos, sin, positions)
+    _expect("grad_q", grad_q, q.dtype, q.shape)
+    _expect("grad_k", grad_k, k.dtype, k.shape)
+    if dq is None:
+        dq = torch.empty(q.shape, dtype=q.dtype, device=device)
+    if dk is None:
+        dk = torch.empty(k.shape, dtype=k.dtype, device=device)
+    _expect("dq", dq, q.dtype, q.shape)
+    _expect("dk", dk, k.dtype, k.shape)
+    space = _status_workspace(device)
+    rows = _scratch_size("b200_head_norm_rotary_scratch", device, q.shape[0], q.shape[1], k.shape[1], q.shape[2])
+    partial = torch.empty((rows, q.shape[2]), dtype=torch.float32, device=device)
+    weights = torch.empty((2, q.shape[2]), dtype=torch.float32, device=device)
+    dq_weight, dk_weight = weights[0], weights[1]
+    _call("b200_head_norm_rotary_backward", device, *_slots(grad_q), *_slots(grad_k), *_slots(q), *_slots(k),
+          *_slots(q_weight), *_slots(k_weight), *_slots(cos), *_slots(sin), *_slots(positions), *_slots(dq), *_slots(dk),
+          *_slots(dq_weight), *_slots(dk_weight), *_slots(partial), float(epsilon), *_slots(space), _CODES[q.dtype],
+          int(bool(interleaved)), _stream(q))
+    return dq, dk, dq_weight, dk_weight
+
+
+_NO_SCALE = [None] + [0] * 6
+
+
+def _cache_operands(k_cache, v_cache, k_scale, v_scale) -> list:
+    """Checks a paged cache (pages, heads, page_size, head_dim) and returns its scales' slots."""
+    if k_cache.dtype not in (torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn):
+        raise TypeError(f"k_cache must be float16, bfloat16, int8 or float8_e4m3fn, got {k_cache.dtype}")
+    if k_cache.dim() != 4:
+        raise ValueError("a cache is a (pages, heads, page_size, head_dim) tensor")
+    _expect("v_cache", v_cache, k_cache.dtype, k_cache.shape)
+    if k_cache.element_size() == 2:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("a 16-bit cache has no scales")
+        return _NO_SCALE + _NO_SCALE
+    if k_scale is None or v_scale is None:
+        raise ValueError("an 8-bit cache needs k_scale and v_scale")
+    _expect("k_scale", k_scale, torch.float32, k_cache.shape[:3])
+    _expect("v_scale", v_scale, torch.float32, k_cache.shape[:3])
+    return _slots(k_scale) + _slots(v_scale)
+
+
+def cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
+    """Puts rows of keys and values (tokens, heads, head_dim), f16 or bf16, into the slots of a paged
+    cache (pages, heads, page_size, head_dim) of any memory order with a unit inner stride, in one launch;
+    slot = page * page_size + place, int64.  A cache of the rows' type gets them as they are.  One of int8 or float8_e4m3fn gets codes, and
+    ``k_scale`` / ``v_scale`` (pages, heads, page_size) f32 a scale for each row: the largest magnitude / 127, or
+    the power of two that brings it to at most 448; code * scale is the value.  A row with an infinity or a NaN reads
+    back as NaN throughout.  Negative slots mark padding and are skipped; so are slots behind the cache, which
+    ``workspace_status`` reports.  Slots of one call must differ.  Returns ``(k_cache, v_cache)``."""
+    scales = tuple(t for t in (k_scale, v_scale) if t is not None)
+    device = _require_cuda(k, v, slots, k_cache, v_cache, *scales)
+    _float_type("k", k, (torch.float16, torch.bfloat16))
+    scale_slots = _cache_operands(k_cache, v_cache, k_scale, v_scale)
+    if k_cache.element_size() == 2:
+        _expect("k_cache", k_cache, k.dtype)
+    if k.dim() != 3:
+        raise ValueError("k and v are (tokens, heads, head_dim) tensors")
+    _expect("k", k, k.dtype, (k.shape[0], k_cache.shape[1], k_cache.shape[3]))
+    _expect("v", v, k.dtype, k.shape)
+    _expect("slots", slots, torch.int64, (k.shape[0],))
+    _call("b200_cache_write", device, *_slots(k), *_slots(v), *_slots(slots), *_slots(k_cache), *_slots(v_cache), *scale_slots,
+          *_slots(_status_workspace(device)), _CODES[k.dtype], _CODES[k_cache.dtype], _stream(k))
+    return k_cache, v_cache
+
+
+def cache_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, *, dtype=None, k_out=None, v_out=None):
+    """The rows of ``slots`` out of a cache that ``cache_write`` filled, ``(k, v)`` of shape (tokens, heads, head_dim):
+    of a 16-bit cache as they are, of an 8-bit one as code * scale in ``dtype`` (f16 or bf16, the default).
+    Negative slots give zeros, and so do slots behind the cache, which ``workspace_status`` reports."""
+    given = tuple(t for t in (k_scale, v_scale, k_out, v_out) if t is not None)
+    device = _require_cuda(k_cache, v_cache, slots, *given)
+    scale_slots = _cache_operands(k_cache, v_cache, k_scale, v_scale)
+    if slots.dim() != 1:
+        raise ValueError("slots has one axis")
+    _expect("slots", slots, torch.int64)
+    if dtype is None:
+        dtype = k_cache.dtype if k_cache.element_size() == 2 else k_out.dtype if k_out is not None else torch.bfloat16
+    if dtype not in (torch.float16, torch.bfloat16):
+        raise TypeError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
+    if k_cache.element_size() == 2 and dtype != k_cache.dtype:
+        raise TypeError(f"a {k_cache.dtype} cache gives its rows as they are, not as {dtype}")
+    shape = (slots.shape[0], k_cache.shape[1], k_cache.shape[3])
+    if k_out is None:
+        k_out = torch.empty(shape, dtype=dtype, device=device)
+    if v_out is None:
+        v_out = torch.empty(shape, dtype=dtype, device=device)
+    _expect("k_out", k_out, dtype, shape)
+    _expect("v_out", v_out, dtype, shape)
+    _call("b200_cache_read", device, *_slots(k_cache), *_slots(v_cache), *_slots(slots), *scale_slots, *_slots(k_out),
+          *_slots(v_out), *_slots(_status_workspace(device)), _CODES[dtype], _CODES[k_cache.dtype], _stream(k_cache))
+    return k_out, v_out
+
+
+def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, k_scale=None, v_scale=None, out=None,
+                    return_lse: bool = False):
+    """Attention of one new token a sequence: ``q`` (batch, heads, head_dim) over the first ``lengths[b]`` rows of each
+    sequence in a paged cache (``cache_write``), whose pages row ``b`` of ``block_table`` (batch, columns) names in
+    order; both int32.  heads is a multiple of the cache's heads, neighbouring query heads share a key head;
+    head_dim is 64 or 128.  A sequence of length 0 gets zeros (and lse -infinity).  What lies behind a sequence, in its last page or in
+    the table, is never used.  A page outside the cache is left out, a length past the table is cut there, and
+    ``workspace_status`` reports both.  Returns ``out``, or ``(out, lse)`` with the natural logarithm of the sums (f32)."""
+    given = tuple(t for t in (k_scale, v_scale, out) if t is not None)
+    device = _require_cuda(q, k_cache, v_cache, block_table, lengths, *given)
+    _float_type("q", q, (torch.float16, torch.bfloat16))
+    scale_slots = _cache_operands(k_cache, v_cache, k_scale, v_scale)
+    if k_cache.element_size() == 2:
+        _expect("k_cache", k_cache, q.dtype)
+    if q.dim() != 3 or block_table.dim() != 2:
+        raise ValueError("q is a (batch, heads, head_dim) tensor and block_table a (batch, columns) one")
+    if q.shape[2] != k_cache.shape[3]:
+        raise ValueError(f"q has head_dim {q.shape[2]}, the cache {k_cache.shape[3]}")
+    if k_cache.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k_cache.shape[1]:
+        raise ValueError(f"{q.shape[1]} query heads are not a multiple of the cache's {k_cache.shape[1]}")
+    _expect("block_table", block_table, torch.int32, (q.shape[0], block_table.shape[1]))
+    _expect("lengths", lengths, torch.int32, (q.shape[0],))
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=device)
+    _expect("out", out, q.dtype, q.shape)
+    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if return_lse else None
+    space = _status_workspace(device)
+    store = _CODES[k_cache.dtype]
+    words = _scratch_size("b200_paged_attention_scratch", device, q.shape[0], q.shape[1], k_cache.shape[1], q.shape[2],
+                          block_table.shape[1] * k_cache.shape[2], store)
+    partial = torch.empty((words,), dtype=torch.float32, device=device)   # the call's own: calls may overlap
+    _call("b200_paged_attention", device, *_slots(q), *_slots(k_cache), *_slots(v_cache), *scale_slots, *_slots(block_table),
+          *_slots(lengths), *_slots(out), *(_slots(lse) if return_lse else [None] + [0] * 4), float(scale), *_slots(partial),
+          *_slots(space), _CODES[q.dtype], store, _stream(q))
+    return (out, lse) if return_lse else out
 
 
 def gather_probe(table: torch.Tensor, gathers: int, *, variant: int = 1, hints: bool = True) -> None:

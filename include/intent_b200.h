@@ -285,6 +285,12 @@ int b200_flash_attention(const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2
                          int32_t dtype, int32_t head_group, int32_t causal, void *stream);
 
 /*
+ * The operators around a key-value cache take their views as one host array of `count` int64 words:
+ * the slots of the convention above (pointer, extents, element strides), view after view, in the order
+ * that each entry names with the views' ranks.  The array is read during the call only.
+ */
+
+/*
  * RMS norm of every query and key head and the rotation by the token's position, one pass over q and
  * k (tokens, heads, D):   z = x / sqrt(mean(x^2) + epsilon) * weight,   y = R(position) z.
  * R turns pair i < cosine_d1 by the angle whose cosine and sine stand at [position, i] of the f32
@@ -295,18 +301,9 @@ int b200_flash_attention(const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2
  * D a multiple of 16 in [16, 256], pairs a multiple of 8; unit inner strides, 16-byte aligned bases,
  * outer strides of whole 16-byte steps.  An output may be its own input view, and otherwise overlaps
  * no operand.  q and k may be slices of one tensor, and so may the outputs.
+ * slots: q 3, k 3, q_weight 1, k_weight 1, cosine 2, sine 2, positions 1, q_out 3, k_out 3, workspace 1.
  */
-int b200_head_norm_rotary(
-    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
-    const void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
-    const void *q_weight, int64_t q_weight_d0, int64_t q_weight_s0,
-    const void *k_weight, int64_t k_weight_d0, int64_t k_weight_s0,
-    const void *cosine, int64_t cosine_d0, int64_t cosine_d1, int64_t cosine_s0, int64_t cosine_s1,
-    const void *sine, int64_t sine_d0, int64_t sine_d1, int64_t sine_s0, int64_t sine_s1,
-    const void *positions, int64_t positions_d0, int64_t positions_s0,
-    void *q_out, int64_t q_out_d0, int64_t q_out_d1, int64_t q_out_d2, int64_t q_out_s0, int64_t q_out_s1, int64_t q_out_s2,
-    void *k_out, int64_t k_out_d0, int64_t k_out_d1, int64_t k_out_d2, int64_t k_out_s0, int64_t k_out_s1, int64_t k_out_s2,
-    float epsilon, void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t interleaved, void *stream);
+int b200_head_norm_rotary(const int64_t *slots, int64_t count, float epsilon, int32_t dtype, int32_t interleaved, void *stream);
 
 /*
  * Its backward pass, from the gradients of both outputs: with g = R^T dy, u = g * weight and
@@ -316,23 +313,12 @@ int b200_head_norm_rotary(
  * rows as b200_head_norm_rotary_scratch says for this device; the weights' sums are taken in a fixed
  * order, so results do not vary.  Layout rules are the forward entry's; dq and dk may be the gradient
  * or input view of the same rows.
+ * slots: grad_q 3, grad_k 3, q 3, k 3, q_weight 1, k_weight 1, cosine 2, sine 2, positions 1, dq 3, dk 3,
+ * dq_weight 1, dk_weight 1, partial 2, workspace 1.
  */
 int b200_head_norm_rotary_scratch(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t head_dim, int64_t *rows);
-int b200_head_norm_rotary_backward(
-    const void *grad_q, int64_t grad_q_d0, int64_t grad_q_d1, int64_t grad_q_d2, int64_t grad_q_s0, int64_t grad_q_s1, int64_t grad_q_s2,
-    const void *grad_k, int64_t grad_k_d0, int64_t grad_k_d1, int64_t grad_k_d2, int64_t grad_k_s0, int64_t grad_k_s1, int64_t grad_k_s2,
-    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
-    const void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
-    const void *q_weight, int64_t q_weight_d0, int64_t q_weight_s0,
-    const void *k_weight, int64_t k_weight_d0, int64_t k_weight_s0,
-    const void *cosine, int64_t cosine_d0, int64_t cosine_d1, int64_t cosine_s0, int64_t cosine_s1,
-    const void *sine, int64_t sine_d0, int64_t sine_d1, int64_t sine_s0, int64_t sine_s1,
-    const void *positions, int64_t positions_d0, int64_t positions_s0,
-    void *dq, int64_t dq_d0, int64_t dq_d1, int64_t dq_d2, int64_t dq_s0, int64_t dq_s1, int64_t dq_s2,
-    void *dk, int64_t dk_d0, int64_t dk_d1, int64_t dk_d2, int64_t dk_s0, int64_t dk_s1, int64_t dk_s2,
-    void *dq_weight, int64_t dq_weight_d0, int64_t dq_weight_s0, void *dk_weight, int64_t dk_weight_d0, int64_t dk_weight_s0,
-    void *partial, int64_t partial_d0, int64_t partial_d1, int64_t partial_s0, int64_t partial_s1,
-    float epsilon, void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t interleaved, void *stream);
+int b200_head_norm_rotary_backward(const int64_t *slots, int64_t count, float epsilon, int32_t dtype, int32_t interleaved,
+                                   void *stream);
 
 /*
  * Rows of keys and values (tokens, heads, D), f16 or bf16, into the slots of a paged cache
@@ -347,35 +333,17 @@ int b200_head_norm_rotary_backward(
  * slot holds that is named twice is unspecified.  D a multiple of 16 in [16, 256]; unit inner strides,
  * 16-byte aligned bases, outer strides of whole 16-byte steps.  Key and value cache may be parts of
  * one allocation.  No counterpart in the reference.
+ * slots: k 3, v 3, slots 1, k_cache 4, v_cache 4, k_scale 3, v_scale 3, workspace 1.
  */
-int b200_cache_write(
-    const void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
-    const void *v, int64_t v_d0, int64_t v_d1, int64_t v_d2, int64_t v_s0, int64_t v_s1, int64_t v_s2,
-    const void *slots, int64_t slots_d0, int64_t slots_s0,
-    void *k_cache, int64_t k_cache_d0, int64_t k_cache_d1, int64_t k_cache_d2, int64_t k_cache_d3,
-    int64_t k_cache_s0, int64_t k_cache_s1, int64_t k_cache_s2, int64_t k_cache_s3,
-    void *v_cache, int64_t v_cache_d0, int64_t v_cache_d1, int64_t v_cache_d2, int64_t v_cache_d3,
-    int64_t v_cache_s0, int64_t v_cache_s1, int64_t v_cache_s2, int64_t v_cache_s3,
-    void *k_scale, int64_t k_scale_d0, int64_t k_scale_d1, int64_t k_scale_d2, int64_t k_scale_s0, int64_t k_scale_s1, int64_t k_scale_s2,
-    void *v_scale, int64_t v_scale_d0, int64_t v_scale_d1, int64_t v_scale_d2, int64_t v_scale_s0, int64_t v_scale_s1, int64_t v_scale_s2,
-    void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t store, void *stream);
+int b200_cache_write(const int64_t *slots, int64_t count, int32_t dtype, int32_t store, void *stream);
 
 /*
  * The rows of `slots` back out of the cache, as f16 or bf16 (of a 16-bit cache: its own type);
  * code * scale in f32, rounded once.  Padding (a negative slot) and slots behind the cache, which are
  * recorded in the workspace, give zeros.  A slot may be named any number of times.
+ * slots: k_cache 4, v_cache 4, slots 1, k_scale 3, v_scale 3, k 3, v 3, workspace 1.
  */
-int b200_cache_read(
-    const void *k_cache, int64_t k_cache_d0, int64_t k_cache_d1, int64_t k_cache_d2, int64_t k_cache_d3,
-    int64_t k_cache_s0, int64_t k_cache_s1, int64_t k_cache_s2, int64_t k_cache_s3,
-    const void *v_cache, int64_t v_cache_d0, int64_t v_cache_d1, int64_t v_cache_d2, int64_t v_cache_d3,
-    int64_t v_cache_s0, int64_t v_cache_s1, int64_t v_cache_s2, int64_t v_cache_s3,
-    const void *slots, int64_t slots_d0, int64_t slots_s0,
-    const void *k_scale, int64_t k_scale_d0, int64_t k_scale_d1, int64_t k_scale_d2, int64_t k_scale_s0, int64_t k_scale_s1, int64_t k_scale_s2,
-    const void *v_scale, int64_t v_scale_d0, int64_t v_scale_d1, int64_t v_scale_d2, int64_t v_scale_s0, int64_t v_scale_s1, int64_t v_scale_s2,
-    void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
-    void *v, int64_t v_d0, int64_t v_d1, int64_t v_d2, int64_t v_s0, int64_t v_s1, int64_t v_s2,
-    void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t store, void *stream);
+int b200_cache_read(const int64_t *slots, int64_t count, int32_t dtype, int32_t store, void *stream);
 
 /*
  * Attention of one new token a sequence: q (batch, heads, D) over the first lengths[b] rows of each
@@ -391,23 +359,11 @@ int b200_cache_read(
  * partial: 16-byte aligned scratch, f32 words as b200_paged_attention_scratch says for this device
  * (keys = table columns * page_size).  Calls that may overlap need scratch of their own each.
  * No counterpart in the reference.
+ * slots: q 3, k_cache 4, v_cache 4, k_scale 3, v_scale 3, block_table 2, lengths 1, out 3, lse 2, partial 1, workspace 1.
  */
 int b200_paged_attention_scratch(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t keys,
                                             int32_t store, int64_t *words);
-int b200_paged_attention(
-    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
-    const void *k_cache, int64_t k_cache_d0, int64_t k_cache_d1, int64_t k_cache_d2, int64_t k_cache_d3,
-    int64_t k_cache_s0, int64_t k_cache_s1, int64_t k_cache_s2, int64_t k_cache_s3,
-    const void *v_cache, int64_t v_cache_d0, int64_t v_cache_d1, int64_t v_cache_d2, int64_t v_cache_d3,
-    int64_t v_cache_s0, int64_t v_cache_s1, int64_t v_cache_s2, int64_t v_cache_s3,
-    const void *k_scale, int64_t k_scale_d0, int64_t k_scale_d1, int64_t k_scale_d2, int64_t k_scale_s0, int64_t k_scale_s1, int64_t k_scale_s2,
-    const void *v_scale, int64_t v_scale_d0, int64_t v_scale_d1, int64_t v_scale_d2, int64_t v_scale_s0, int64_t v_scale_s1, int64_t v_scale_s2,
-    const void *block_table, int64_t table_d0, int64_t table_d1, int64_t table_s0, int64_t table_s1,
-    const void *lengths, int64_t lengths_d0, int64_t lengths_s0,
-    void *out, int64_t out_d0, int64_t out_d1, int64_t out_d2, int64_t out_s0, int64_t out_s1, int64_t out_s2,
-    void *lse, int64_t lse_d0, int64_t lse_d1, int64_t lse_s0, int64_t lse_s1,
-    float scale, void *partial, int64_t partial_d0, int64_t partial_s0, void *workspace, int64_t ws_d0, int64_t ws_s0,
-    int32_t dtype, int32_t store, void *stream);
+int b200_paged_attention(const int64_t *slots, int64_t count, float scale, int32_t dtype, int32_t store, void *stream);
 
 /*
  * CSR SpMM  Y = A . X, i32 indices, f32 values, strict source-order

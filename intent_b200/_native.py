@@ -41,16 +41,13 @@ SIGNATURES = {
     "b200_gemm": _view(2) + _view(2) + _view(2) + _view(1) + [_I32, _I32, _P],
     "b200_gemm_static_scratch": _view(2) + _view(2) + _view(2) + [_I32, _I32, _I32, _P],
     "b200_flash_attention": _view(4) * 4 + [_F32] + _view(1) + [_I32, _I32, _I32, _P],
-    "b200_head_norm_rotary": (_view(3) * 2 + _view(1) * 2 + _view(2) * 2 + _view(1) + _view(3) * 2 + [_F32] + _view(1)
-                              + [_I32, _I32, _P]),
+    "b200_head_norm_rotary": [_P, _I64, _F32, _I32, _I32, _P],
     "b200_head_norm_rotary_scratch": [_I64] * 4 + [ctypes.POINTER(_I64)],
-    "b200_head_norm_rotary_backward": (_view(3) * 4 + _view(1) * 2 + _view(2) * 2 + _view(1) + _view(3) * 2 + _view(1) * 2
-                                       + _view(2) + [_F32] + _view(1) + [_I32, _I32, _P]),
-    "b200_cache_write": _view(3) * 2 + _view(1) + _view(4) * 2 + _view(3) * 2 + _view(1) + [_I32, _I32, _P],
-    "b200_cache_read": _view(4) * 2 + _view(1) + _view(3) * 4 + _view(1) + [_I32, _I32, _P],
+    "b200_head_norm_rotary_backward": [_P, _I64, _F32, _I32, _I32, _P],
+    "b200_cache_write": [_P, _I64, _I32, _I32, _P],
+    "b200_cache_read": [_P, _I64, _I32, _I32, _P],
     "b200_paged_attention_scratch": [_I64] * 5 + [_I32, ctypes.POINTER(_I64)],
-    "b200_paged_attention": (_view(3) + _view(4) * 2 + _view(3) * 2 + _view(2) + _view(1) + _view(3) + _view(2) + [_F32]
-                             + _view(1) + _view(1) + [_I32, _I32, _P]),
+    "b200_paged_attention": [_P, _I64, _F32, _I32, _I32, _P],
     "b200_csr_spmm": _view(1) * 3 + _view(2) * 2 + _view(1) + [_P],
     "b200_csr_spmv": _view(1) * 5 + [_P],
     "b200_softmax_backward": _view(2) * 3 + [_I32, _P],

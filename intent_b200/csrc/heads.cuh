@@ -19,6 +19,32 @@ struct View4 {
   int64_t d0, d1, d2, d3, s0, s1, s2, s3;
 };
 
+struct View2 {
+  const void *data;
+  int64_t d0, d1, s0, s1;
+};
+struct View1 {
+  const void *data;
+  int64_t d0, s0;
+};
+
+// Takes views off an array of slots: pointer, extents, strides of each, as the ABI orders them.
+class Slots {
+ public:
+  Slots(const int64_t *words, int64_t count) : words_(words), count_(words ? count : 0) {}
+  View1 view1() { return {pointer(), next(), next()}; }
+  View2 view2() { return {pointer(), next(), next(), next(), next()}; }
+  View3 view3() { return {pointer(), next(), next(), next(), next(), next(), next()}; }
+  View4 view4() { return {pointer(), next(), next(), next(), next(), next(), next(), next(), next()}; }
+  bool exact() const { return taken_ == count_; }   // neither more nor fewer than there are
+
+ private:
+  int64_t next() { return taken_++ < count_ ? words_[taken_ - 1] : 0; }
+  const void *pointer() { return reinterpret_cast<const void *>(next()); }
+  const int64_t *words_;
+  int64_t count_, taken_ = 0;
+};
+
 inline int element_size(int dtype) { return dtype == B200_F32 ? 4 : dtype == B200_F16 || dtype == B200_BF16 ? 2 : 1; }
 
 // Every stride times extent stays far from the end of 64 bits, whatever the caller passes.
@@ -119,11 +145,51 @@ inline int row_lanes(int64_t columns) {
   return lanes;
 }
 
+// Threads of a block of the kernels that move rows.
+constexpr int kThreads = 256;
+
+inline int check_units(const char *what, int64_t tokens, int64_t slices) {
+  if (tokens * slices >= (int64_t(1) << 32) - (1 << 21))   // counted in 32 bits: a 64-bit division costs as much as a row's arithmetic
+    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: 2^32 rows or more in one call", what);
+  return B200_OK;
+}
+
 // ---- device ------------------------------------------------------------------
 // Word 0 of the workspace becomes 3 and word 1 the position of a bad index (b200_workspace_status
 // reports it); the first one found stays.
 __device__ __forceinline__ void report_index(int *status, int position) {
   if (atomicCAS(status, 0, 3) == 0) status[1] = position;
+}
+
+// Two f32 at a time (one instruction each on this part).
+struct Two {
+  float a, b;
+};
+__device__ __forceinline__ uint64_t bits(Two v) {
+  uint64_t r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(v.a), "f"(v.b));
+  return r;
+}
+__device__ __forceinline__ Two two(uint64_t v) {
+  Two r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.a), "=f"(r.b) : "l"(v));
+  return r;
+}
+__device__ __forceinline__ Two mul(Two x, Two y) {
+  uint64_t r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(x)), "l"(bits(y)));
+  return two(r);
+}
+__device__ __forceinline__ Two fma(Two x, Two y, Two z) {
+  uint64_t r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r) : "l"(bits(x)), "l"(bits(y)), "l"(bits(z)));
+  return two(r);
+}
+__device__ __forceinline__ Two swap(Two x) { return {x.b, x.a}; }
+__device__ __forceinline__ Two add(Two x, Two y) {
+  uint64_t r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(x)), "l"(bits(y)));
+  return two(r);
 }
 
 // Eight consecutive columns, as raw 128-bit vectors and as f32.

@@ -38,6 +38,8 @@
 namespace b200 {
 namespace {
 
+using heads::View1;
+using heads::View2;
 using heads::View3;
 using heads::View4;
 
@@ -772,85 +774,79 @@ extern "C" int b200_paged_attention_scratch(int64_t batch, int64_t heads, int64_
   return B200_OK;
 }
 
-#define VIEW3(name) \
-  View3 { name, name##_d0, name##_d1, name##_d2, name##_s0, name##_s1, name##_s2 }
-#define VIEW4(name) \
-  View4 { name, name##_d0, name##_d1, name##_d2, name##_d3, name##_s0, name##_s1, name##_s2, name##_s3 }
-
-extern "C" int b200_paged_attention(
-    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
-    const void *k_cache, int64_t k_cache_d0, int64_t k_cache_d1, int64_t k_cache_d2, int64_t k_cache_d3,
-    int64_t k_cache_s0, int64_t k_cache_s1, int64_t k_cache_s2, int64_t k_cache_s3,
-    const void *v_cache, int64_t v_cache_d0, int64_t v_cache_d1, int64_t v_cache_d2, int64_t v_cache_d3,
-    int64_t v_cache_s0, int64_t v_cache_s1, int64_t v_cache_s2, int64_t v_cache_s3,
-    const void *k_scale, int64_t k_scale_d0, int64_t k_scale_d1, int64_t k_scale_d2, int64_t k_scale_s0, int64_t k_scale_s1, int64_t k_scale_s2,
-    const void *v_scale, int64_t v_scale_d0, int64_t v_scale_d1, int64_t v_scale_d2, int64_t v_scale_s0, int64_t v_scale_s1, int64_t v_scale_s2,
-    const void *block_table, int64_t table_d0, int64_t table_d1, int64_t table_s0, int64_t table_s1,
-    const void *lengths, int64_t lengths_d0, int64_t lengths_s0,
-    void *out, int64_t out_d0, int64_t out_d1, int64_t out_d2, int64_t out_s0, int64_t out_s1, int64_t out_s2,
-    void *lse, int64_t lse_d0, int64_t lse_d1, int64_t lse_s0, int64_t lse_s1,
-    float scale, void *partial, int64_t partial_d0, int64_t partial_s0, void *workspace, int64_t ws_d0, int64_t ws_s0,
-    int32_t dtype, int32_t store, void *stream) {
+extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float scale, int32_t dtype, int32_t store, void *stream) {
   const char *what = "paged_attention";
+  heads::Slots from(slots, count);
+  const View3 q = from.view3();
+  cache::Cache held{};
+  held.k = from.view4();
+  held.v = from.view4();
+  held.k_scale = from.view3();
+  held.v_scale = from.view3();
+  const View2 table = from.view2();
+  const View1 lengths = from.view1();
+  const View3 out = from.view3();
+  const View2 lse = from.view2();
+  const View1 partial = from.view1(), workspace = from.view1();
+  if (!from.exact()) return fail(B200_ERR_INVALID_ARGUMENT, "%s: %lld slots do not describe its views", what, (long long)count);
   if (dtype != B200_F16 && dtype != B200_BF16) return fail(B200_ERR_INVALID_ARGUMENT, "%s: queries are f16 or bf16", what);
-  const View3 query = VIEW3(q), result = VIEW3(out);
-  const cache::Cache held{VIEW4(k_cache), VIEW4(v_cache), VIEW3(k_scale), VIEW3(v_scale)};
   const int status = cache::check(what, held, dtype, store, 256);
   if (status != B200_OK) return status;
-  if (!heads::sane(query) || !heads::sane(result) || !heads::sane(table_d0, table_s0) || !heads::sane(table_d1, table_s1) ||
-      !heads::sane(lengths_d0, lengths_s0) || !heads::sane(lse_d0, lse_s0) || !heads::sane(lse_d1, lse_s1))
+  const View4 &k = held.k, &v = held.v;
+  if (!heads::sane(q) || !heads::sane(out) || !heads::sane(table.d0, table.s0) || !heads::sane(table.d1, table.s1) ||
+      !heads::sane(lengths.d0, lengths.s0) || !heads::sane(lse.d0, lse.s0) || !heads::sane(lse.d1, lse.s1))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: negative or huge extent or stride", what);
-  if (k_cache_d3 != 64 && k_cache_d3 != 128)
-    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: head_dim %lld is not 64 or 128", what, (long long)k_cache_d3);
-  if (q_d2 != k_cache_d3 || out_d0 != q_d0 || out_d1 != q_d1 || out_d2 != q_d2)
+  if (k.d3 != 64 && k.d3 != 128)
+    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: head_dim %lld is not 64 or 128", what, (long long)k.d3);
+  if (q.d2 != k.d3 || out.d0 != q.d0 || out.d1 != q.d1 || out.d2 != q.d2)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: queries, output and cache differ in shape", what);
-  if (k_cache_d1 < 1 || q_d1 < 1 || q_d1 % k_cache_d1)
+  if (k.d1 < 1 || q.d1 < 1 || q.d1 % k.d1)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the query heads are not a multiple of the cache's heads", what);
-  if (q_d0 > 65535 || q_d1 > 65536)
+  if (q.d0 > 65535 || q.d1 > 65536)
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: more than 65535 sequences or 65536 heads", what);
-  if (table_d0 != q_d0 || lengths_d0 != q_d0)
+  if (table.d0 != q.d0 || lengths.d0 != q.d0)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: block table, lengths and queries differ in sequences", what);
-  if (lse && (lse_d0 != q_d0 || lse_d1 != q_d1)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: lse is (sequences, heads)", what);
+  if (lse.data && (lse.d0 != q.d0 || lse.d1 != q.d1)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: lse is (sequences, heads)", what);
   if (!isfinite(scale)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: scale is not a finite number", what);
-  if (!workspace || ws_d0 < B200_WORKSPACE_WORDS || ws_s0 != 1)
+  if (!workspace.data || workspace.d0 < B200_WORKSPACE_WORDS || workspace.s0 != 1)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the workspace needs %d contiguous int32 words", what, B200_WORKSPACE_WORDS);
-  if (q_d0 == 0) return B200_OK;
-  if (k_cache_d2 && table_d1 > (INT32_MAX - 4096) / k_cache_d2)   // key positions and steps are counted in int32
+  if (q.d0 == 0) return B200_OK;
+  if (k.d2 && table.d1 > (INT32_MAX - 4096) / k.d2)   // key positions and steps are counted in int32
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: a row of the block table names 2^31 positions or more", what);
-  const int64_t most_keys = table_d1 * k_cache_d2;
-  const int64_t group = q_d1 / k_cache_d1, runs = runs_of(q_d0, k_cache_d1, group, most_keys, store);
-  if (!q || !out || !lengths || (table_d1 && !block_table) || !partial)
+  const int64_t most_keys = table.d1 * k.d2;
+  const int64_t group = q.d1 / k.d1, runs = runs_of(q.d0, k.d1, group, most_keys, store);
+  if (!q.data || !out.data || !lengths.data || (table.d1 && !table.data) || !partial.data)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  if (partial_d0 < runs * 2 * rows_of(group) * partial_floats((int)q_d2) || partial_s0 != 1 || !aligned16(partial))
+  if (partial.d0 < runs * 2 * rows_of(group) * partial_floats((int)q.d2) || partial.s0 != 1 || !aligned16(partial.data))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the scratch is too short, not contiguous or not 16-byte aligned", what);
-  if (!heads::vector_rows(query, 2) || !heads::vector_rows(result, 2))
+  if (!heads::vector_rows(q, 2) || !heads::vector_rows(out, 2))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT,
                 "%s: rows need a unit inner stride, a 16-byte aligned base and outer strides of whole 16-byte steps", what);
   const int size = heads::element_size(store);
-  const heads::Span to = heads::span(result, 2);
-  if (!heads::distinct(result) || heads::overlap(to, heads::span(query, 2)) || heads::overlap(to, heads::span(held.k, size)) ||
-      heads::overlap(to, heads::span(held.v, size)))
+  const heads::Span to = heads::span(out, 2);
+  if (!heads::distinct(out) || heads::overlap(to, heads::span(q, 2)) || heads::overlap(to, heads::span(k, size)) ||
+      heads::overlap(to, heads::span(v, size)))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the output overlaps itself or an input", what);
 
   Problem p{};
-  p.q = q; p.q_batch = q_s0; p.q_head = q_s1;
-  p.k = static_cast<const uint8_t *>(k_cache); p.v = static_cast<const uint8_t *>(v_cache);
-  p.k_page = k_cache_s0 * size; p.k_head = k_cache_s1 * size; p.k_slot = k_cache_s2 * size;
-  p.v_page = v_cache_s0 * size; p.v_head = v_cache_s1 * size; p.v_slot = v_cache_s2 * size;
-  p.k_scale = static_cast<const float *>(k_scale); p.v_scale = static_cast<const float *>(v_scale);
-  p.ks_page = k_scale_s0; p.ks_head = k_scale_s1; p.ks_slot = k_scale_s2;
-  p.vs_page = v_scale_s0; p.vs_head = v_scale_s1; p.vs_slot = v_scale_s2;
-  p.table = static_cast<const int *>(block_table); p.table_row = table_s0; p.table_column = table_s1;
-  p.lengths = static_cast<const int *>(lengths); p.lengths_step = lengths_s0;
-  p.out = out; p.out_batch = out_s0; p.out_head = out_s1;
-  p.lse = static_cast<float *>(lse); p.lse_batch = lse_s0; p.lse_head = lse_s1;
-  p.partial = static_cast<float *>(partial);
-  p.batch = (int)q_d0; p.kv_heads = (int)k_cache_d1; p.group = (int)group;
+  p.q = q.data; p.q_batch = q.s0; p.q_head = q.s1;
+  p.k = static_cast<const uint8_t *>(k.data); p.v = static_cast<const uint8_t *>(v.data);
+  p.k_page = k.s0 * size; p.k_head = k.s1 * size; p.k_slot = k.s2 * size;
+  p.v_page = v.s0 * size; p.v_head = v.s1 * size; p.v_slot = v.s2 * size;
+  p.k_scale = static_cast<const float *>(held.k_scale.data); p.v_scale = static_cast<const float *>(held.v_scale.data);
+  p.ks_page = held.k_scale.s0; p.ks_head = held.k_scale.s1; p.ks_slot = held.k_scale.s2;
+  p.vs_page = held.v_scale.s0; p.vs_head = held.v_scale.s1; p.vs_slot = held.v_scale.s2;
+  p.table = static_cast<const int *>(table.data); p.table_row = table.s0; p.table_column = table.s1;
+  p.lengths = static_cast<const int *>(lengths.data); p.lengths_step = lengths.s0;
+  p.out = const_cast<void *>(out.data); p.out_batch = out.s0; p.out_head = out.s1;
+  p.lse = static_cast<float *>(const_cast<void *>(lse.data)); p.lse_batch = lse.s0; p.lse_head = lse.s1;
+  p.partial = static_cast<float *>(const_cast<void *>(partial.data));
+  p.batch = (int)q.d0; p.kv_heads = (int)k.d1; p.group = (int)group;
   p.row_tiles = (int)((group + rows_of(group) - 1) / rows_of(group));
-  p.page_size = (int)k_cache_d2; p.pages = (int)k_cache_d0; p.runs = (int)runs;
+  p.page_size = (int)k.d2; p.pages = (int)k.d0; p.runs = (int)runs;
   p.most_keys = most_keys;
   p.scale_log2e = scale * kLog2e;
-  p.status = static_cast<int *>(workspace);
+  p.status = static_cast<int *>(const_cast<void *>(workspace.data));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  return dtype == B200_F16 ? by_store<__half>(p, store, (int)q_d2, s) : by_store<__nv_bfloat16>(p, store, (int)q_d2, s);
+  return dtype == B200_F16 ? by_store<__half>(p, store, (int)q.d2, s) : by_store<__nv_bfloat16>(p, store, (int)q.d2, s);
 }

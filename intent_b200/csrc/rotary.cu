@@ -13,15 +13,29 @@
 // 16 columns as two 128-bit vectors (16-bit types) chosen so that BOTH ends of its pairs are its own:
 // the rotation needs no exchange, the mean is a butterfly over those lanes.  The 8 cosines and 8
 // sines that a lane needs are loaded once for all the heads that it takes of a token.
+//
+// Rows arrive by cp.async in places of shared memory that are each thread's own, several rows ahead: what is
+// in flight takes no registers, and 16 warps of an SM keep 64 KB and more on their way.  Arithmetic is on
+// pairs of f32.  Measured for 16384 tokens of 32 and 8 heads of 128 columns in bf16: 58 us forward, 5.8 TB/s
+// (337 MB; 52 us at the 6447 GB/s of a copy), 86 us backward, 5.8 TB/s (504 MB; 78 us).  Without the
+// ring and the pairs, one row a thread at a time: 77 and 138 us.
 #include "heads.cuh"
 
 namespace b200 {
 namespace {
 
 using heads::Eight;
+using heads::fma;
+using heads::mul;
+using heads::swap;
+using heads::Two;
+using heads::View1;
+using heads::View2;
 using heads::View3;
 
-constexpr int kThreads = 256;
+using heads::kThreads;
+
+constexpr int kBlocksPerSm = 2;
 
 struct Operand {        // one of q, k (and, for the backward pass, its gradients)
   const void *x;
@@ -30,7 +44,7 @@ struct Operand {        // one of q, k (and, for the backward pass, its gradient
   void *out;
   int64_t x_token, x_head, grad_token, grad_head, out_token, out_head;
   int heads;
-  int slices;           // units per token: ceil(heads / rows of a unit)
+  uint32_t slices;      // units per token: ceil(heads / rows of a unit)
 };
 
 struct Rotation {
@@ -54,22 +68,68 @@ __device__ __forceinline__ void pieces(const Rotation &r, int e, int &first, int
   second = split ? r.half + 8 * e : 16 * e + 8;
 }
 
-// x[0..8) and x[8..16) are the pieces; BACK turns by the opposite angle.
+// 16 columns of a row, neighbours in pairs: own[0..4) is the first piece and own[4..8) the second.
+struct Row {
+  Two own[8];
+  template <typename T> __device__ __forceinline__ void widen(const Eight<T> &a, const Eight<T> &b) {
+    float x[16];
+    a.widen(x);
+    b.widen(x + 8);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) own[i] = {x[2 * i], x[2 * i + 1]};
+  }
+  template <typename T> __device__ __forceinline__ void narrow(Eight<T> &a, Eight<T> &b) const {
+    float x[16];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { x[2 * i] = own[i].a; x[2 * i + 1] = own[i].b; }
+    a.narrow(x);
+    b.narrow(x + 8);
+  }
+  __device__ __forceinline__ float dot(const Row &other) const {
+    Two sum = mul(own[0], other.own[0]);
+#pragma unroll
+    for (int i = 1; i < 8; ++i) sum = fma(own[i], other.own[i], sum);
+    return sum.a + sum.b;
+  }
+};
+
+// A turn as y = x * straight + partner(x) * crossed, where a column's partner is the other member of
+// its pair.  Lanes whose columns pass never look at partners: an infinity there times 0 would be NaN.
+__device__ __forceinline__ Row turned_row(const Row &x, const Row &straight, const Row &crossed, bool turned, bool interleaved) {
+  Row y;
+  if (!turned) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.own[i] = mul(x.own[i], straight.own[i]);
+  } else if (interleaved) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.own[i] = fma(x.own[i], straight.own[i], mul(swap(x.own[i]), crossed.own[i]));
+  } else {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y.own[i] = fma(x.own[i], straight.own[i], mul(x.own[(i + 4) & 7], crossed.own[i]));
+  }
+  return y;
+}
+
+// straight and crossed of R (BACK: of its transpose) for lane `e` at a position.
 template <bool BACK>
-__device__ __forceinline__ void turn(float (&x)[16], const float (&c)[8], const float (&s)[8], bool interleaved) {
-  if (interleaved) {
+__device__ __forceinline__ void angles(const Rotation &r, int e, int position, Row &straight, Row &crossed) {
+  const float4 *c4 = reinterpret_cast<const float4 *>(r.cosine + position * r.cosine_row + 8 * e);
+  const float4 *s4 = reinterpret_cast<const float4 *>(r.sine + position * r.sine_row + 8 * e);
+  const float4 c0 = __ldg(c4), c1 = __ldg(c4 + 1), s0 = __ldg(s4), s1 = __ldg(s4 + 1);
+  const float c[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, s[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
+  if (r.interleaved) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      const float a = x[2 * i], b = x[2 * i + 1], t = BACK ? -s[i] : s[i];
-      x[2 * i] = a * c[i] - b * t;
-      x[2 * i + 1] = b * c[i] + a * t;
+      straight.own[i] = {c[i], c[i]};
+      crossed.own[i] = BACK ? Two{s[i], -s[i]} : Two{-s[i], s[i]};
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const float a = x[i], b = x[i + 8], t = BACK ? -s[i] : s[i];
-      x[i] = a * c[i] - b * t;
-      x[i + 8] = b * c[i] + a * t;
+    for (int i = 0; i < 4; ++i) {
+      straight.own[i] = straight.own[i + 4] = {c[2 * i], c[2 * i + 1]};
+      const Two positive = {s[2 * i], s[2 * i + 1]}, negative = {-s[2 * i], -s[2 * i + 1]};
+      crossed.own[i] = BACK ? positive : negative;
+      crossed.own[i + 4] = BACK ? negative : positive;
     }
   }
 }
@@ -82,81 +142,148 @@ __device__ __forceinline__ int place(const Rotation &r, int token, bool first_la
   return -1;
 }
 
+// A group's place in the grid of units: a division at the start, additions from then on.
+struct Cursor {
+  uint32_t base, token, slice;      // base: the block's first unit of the round
+  __device__ __forceinline__ Cursor(uint32_t first, uint32_t group, uint32_t slices)
+      : base(first), token((first + group) / slices), slice((first + group) % slices) {}
+  __device__ __forceinline__ void advance(uint32_t step, uint32_t step_token, uint32_t step_slice, uint32_t slices) {
+    base += step;
+    token += step_token;
+    slice += step_slice;
+    if (slice >= slices) {
+      slice -= slices;
+      ++token;
+    }
+  }
+};
+
+// Rows on their way to a thread: each copies its own pieces of the rows it will take into its own
+// places of shared memory (16 bytes a thread, neighbours side by side) STAGES - 1 rows ahead, so that
+// what is in flight does not take registers and nobody waits for anybody else.
+template <int VECTORS, int STAGES> struct Ring {
+  static constexpr int kBytes = VECTORS * STAGES * kThreads * 16;
+  uint4 *mine;
+  uint32_t address;
+  __device__ __forceinline__ explicit Ring(unsigned char *smem) {
+    mine = reinterpret_cast<uint4 *>(smem) + threadIdx.x;
+    address = (uint32_t)__cvta_generic_to_shared(mine);
+  }
+  template <typename T> __device__ __forceinline__ void copy(int stage, int vector, const T *from, bool live) const {
+#pragma unroll
+    for (int i = 0; i < Eight<T>::kVectors; ++i)
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(
+                       address + ((stage * VECTORS + vector * Eight<T>::kVectors + i) * kThreads) * 16),
+                   "l"(reinterpret_cast<const uint4 *>(from) + i), "r"(live ? 16 : 0) : "memory");
+  }
+  template <typename T> __device__ __forceinline__ Eight<T> take(int stage, int vector) const {
+    Eight<T> v;
+#pragma unroll
+    for (int i = 0; i < Eight<T>::kVectors; ++i)
+      v.raw[i] = mine[(stage * VECTORS + vector * Eight<T>::kVectors + i) * kThreads];
+    return v;
+  }
+  static __device__ __forceinline__ void commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+  static __device__ __forceinline__ void wait() { asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory"); }
+};
+
 // ------------------------------------------------------------------ forward
-// A unit is ROWS heads of one token, all of q or all of k: ROWS x 2 vectors in flight in a lane.
-template <typename T, int LANES, int ROWS>
-__global__ void __launch_bounds__(kThreads)
-head_norm_rotary_kernel(Operand q, Operand k, Rotation r) {
-  const int e = threadIdx.x % LANES;
-  const int64_t unit = (int64_t)blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
-  const int slices = q.slices + k.slices;
-  const int token = (int)(unit / slices);
-  const bool unit_live = token < r.tokens;
-  int slice = (int)(unit - (int64_t)token * slices);
-  const bool is_key = slice >= q.slices;
-  if (is_key) slice -= q.slices;
-  const int head_count = is_key ? k.heads : q.heads;
-  const int head0 = slice * ROWS;
-  const bool lane_live = unit_live && e * 16 < r.columns;
+// A unit is `unit_rows` heads of one token, all of q or all of k; they share one load of the cosines,
+// sines and weights, whose products (32 registers) are all that a row's turn needs.
+template <typename T> constexpr int kForwardStages = sizeof(T) == 2 ? 6 : 4;
+
+template <typename T, int LANES>
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+head_norm_rotary_kernel(Operand q, Operand k, Rotation r, int unit_rows, uint32_t units) {
+  constexpr int kGroups = kThreads / LANES, kStages = kForwardStages<T>;
+  using Copies = Ring<2 * Eight<T>::kVectors, kStages>;
+  extern __shared__ __align__(16) unsigned char dynamic_smem[];
+  const Copies ring(dynamic_smem);
+  const int e = threadIdx.x % LANES, group = threadIdx.x / LANES;
+  const uint32_t slices = q.slices + k.slices, step = gridDim.x * kGroups;
+  const bool inside = e * 16 < r.columns, interleaved = r.interleaved;
   int first, second;
   pieces(r, e, first, second);
 
-  Eight<T> a[ROWS], b[ROWS];
-  const T *source = static_cast<const T *>(is_key ? k.x : q.x) +
-                    (unit_live ? token * (is_key ? k.x_token : q.x_token) : 0);
-  const int64_t source_head = is_key ? k.x_head : q.x_head;
-#pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    a[i].clear();
-    b[i].clear();
-    if (lane_live && head0 + i < head_count) {
-      a[i].load(source + (head0 + i) * source_head + first);
-      b[i].load(source + (head0 + i) * source_head + second);
+  // every group of the block runs the same number of rounds: the shuffles below are whole-warp
+  const uint32_t step_token = step / slices, step_slice = step % slices;
+  Cursor load(blockIdx.x * kGroups, group, slices);
+  Cursor use = load;
+  int load_row = 0, load_rows = 0;
+  const T *source = nullptr;
+  int64_t source_head = 0;
+  auto produce = [&](int stage) {
+    if (load.base < units) {
+      if (load_row == 0) {
+        const bool is_key = load.slice >= q.slices;
+        const Operand &o = is_key ? k : q;
+        const int head0 = (int)(is_key ? load.slice - q.slices : load.slice) * unit_rows;
+        load_rows = load.base + group < units && inside ? min(unit_rows, o.heads - head0) : 0;
+        source_head = o.x_head;
+        source = static_cast<const T *>(o.x) + (load_rows ? load.token * o.x_token + head0 * o.x_head : 0);
+      }
+      const T *from = load_row < load_rows ? source + load_row * source_head : source;
+      ring.template copy<T>(stage, 0, from + first, load_row < load_rows);
+      ring.template copy<T>(stage, 1, from + second, load_row < load_rows);
+      if (++load_row == unit_rows) {
+        load_row = 0;
+        load.advance(step, step_token, step_slice, slices);
+      }
     }
-  }
-  const int position = unit_live ? place(r, token, e == 0) : -1;
-  const bool turned = lane_live && e * 8 < r.half && position >= 0;
-  float cosine[8], sine[8];
-  if (turned) {
-    const float4 *c4 = reinterpret_cast<const float4 *>(r.cosine + position * r.cosine_row + 8 * e);
-    const float4 *s4 = reinterpret_cast<const float4 *>(r.sine + position * r.sine_row + 8 * e);
-    const float4 c0 = __ldg(c4), c1 = __ldg(c4 + 1), s0 = __ldg(s4), s1 = __ldg(s4 + 1);
-    cosine[0] = c0.x; cosine[1] = c0.y; cosine[2] = c0.z; cosine[3] = c0.w;
-    cosine[4] = c1.x; cosine[5] = c1.y; cosine[6] = c1.z; cosine[7] = c1.w;
-    sine[0] = s0.x; sine[1] = s0.y; sine[2] = s0.z; sine[3] = s0.w;
-    sine[4] = s1.x; sine[5] = s1.y; sine[6] = s1.z; sine[7] = s1.w;
-  }
-  float w[16];
+    ring.commit();
+  };
 #pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = 0.0f;
-  if (lane_live) {
-    const T *weight = static_cast<const T *>(is_key ? k.weight : q.weight);
-    Eight<T> w0, w1;
-    w0.load(weight + first);
-    w1.load(weight + second);
-    w0.widen(w);
-    w1.widen(w + 8);
-  }
-  T *target = static_cast<T *>(is_key ? k.out : q.out) + (unit_live ? token * (is_key ? k.out_token : q.out_token) : 0);
-  const int64_t target_head = is_key ? k.out_head : q.out_head;
+  for (int i = 0; i < kStages - 1; ++i) produce(i);
+  int stage = 0;
+  for (; use.base < units; use.advance(step, step_token, step_slice, slices)) {
+    const uint32_t unit = use.base + group, token = use.token;
+    const bool is_key = use.slice >= q.slices, live = unit < units && inside;
+    const Operand &o = is_key ? k : q;
+    const int head0 = (int)(is_key ? use.slice - q.slices : use.slice) * unit_rows, rows = live ? min(unit_rows, o.heads - head0) : 0;
+    const int position = unit < units ? place(r, token, e == 0) : -1;
+    const bool turned = live && e * 8 < r.half && position >= 0;
+    Row straight, crossed, w;
+    if (live) {
+      const T *weight = static_cast<const T *>(o.weight);
+      Eight<T> w0, w1;
+      w0.load(weight + first);
+      w1.load(weight + second);
+      w.widen(w0, w1);
+    }
+    if (turned) {
+      angles<false>(r, e, position, straight, crossed);
 #pragma unroll
-  for (int i = 0; i < ROWS; ++i) {
-    float x[16];
-    a[i].widen(x);
-    b[i].widen(x + 8);
-    float squares = 0.0f;
+      for (int i = 0; i < 8; ++i) {   // the partner's weight goes with the partner
+        crossed.own[i] = mul(crossed.own[i], interleaved ? swap(w.own[i]) : w.own[(i + 4) & 7]);
+        straight.own[i] = mul(straight.own[i], w.own[i]);
+      }
+    } else {
 #pragma unroll
-    for (int j = 0; j < 16; ++j) squares += x[j] * x[j];
-    squares = heads::row_sum<LANES>(squares);
-    const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(squares * r.inverse_columns + r.epsilon));
+      for (int i = 0; i < 8; ++i) straight.own[i] = w.own[i];
+    }
+    T *target = static_cast<T *>(o.out) + (live ? token * o.out_token + head0 * o.out_head : 0);
+#pragma unroll 1
+    for (int row = 0; row < unit_rows; ++row) {
+      produce(stage == 0 ? kStages - 1 : stage - 1);
+      ring.wait();
+      Row x;
+      x.widen(ring.template take<T>(stage, 0), ring.template take<T>(stage, 1));
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      const float squares = heads::row_sum<LANES>(x.dot(x));
+      const float rstd = rsqrtf(squares * r.inverse_columns + r.epsilon);
 #pragma unroll
-    for (int j = 0; j < 16; ++j) x[j] = position < 0 ? 0.0f : x[j] * rstd * w[j];
-    if (turned) turn<false>(x, cosine, sine, r.interleaved);   // other columns pass as they are, infinities too
-    if (lane_live && head0 + i < head_count) {
-      a[i].narrow(x);
-      b[i].narrow(x + 8);
-      a[i].store(target + (head0 + i) * target_head + first);
-      b[i].store(target + (head0 + i) * target_head + second);
+      for (int i = 0; i < 8; ++i) x.own[i] = mul(x.own[i], Two{rstd, rstd});
+      if (row < rows) {
+        Eight<T> a, b;
+        if (position < 0) {
+          a.clear();
+          b.clear();
+        } else {
+          turned_row(x, straight, crossed, turned, interleaved).narrow(a, b);
+        }
+        a.store(target + row * o.out_head + first);
+        b.store(target + row * o.out_head + second);
+      }
     }
   }
 }
@@ -166,92 +293,120 @@ head_norm_rotary_kernel(Operand q, Operand k, Rotation r) {
 // weight only: 16 columns in f32, over all the rows it meets.  A block adds its lanes' sums in a
 // fixed order and writes one row of `partial`; the second kernel adds those rows, again in a fixed
 // order, so that dw does not vary from run to run.
-constexpr int kUnitRows = 8;   // heads of a token that share one load of its cosines and sines
+template <typename T> constexpr int kBackwardStages = sizeof(T) == 2 ? 5 : 3;
 
 template <typename T, int LANES>
-__global__ void __launch_bounds__(kThreads)
-head_norm_rotary_backward_kernel(Operand q, Operand k, Rotation r, int q_blocks, float *__restrict__ partial) {
-  constexpr int kGroups = kThreads / LANES;
-  __shared__ float sums[kGroups][LANES * 16 + 1];
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm)
+head_norm_rotary_backward_kernel(Operand q, Operand k, Rotation r, int unit_rows, int q_blocks, float *__restrict__ partial) {
+  constexpr int kGroups = kThreads / LANES, kStages = kBackwardStages<T>;
+  using Copies = Ring<4 * Eight<T>::kVectors, kStages>;
+  static_assert(Copies::kBytes >= kGroups * (LANES * 16 + 1) * 4, "the ring holds the block's sums in the end");
+  extern __shared__ __align__(16) unsigned char dynamic_smem[];
+  const Copies ring(dynamic_smem);
   const int e = threadIdx.x % LANES, group = threadIdx.x / LANES;
-  const bool is_key = (int)blockIdx.x >= q_blocks;
-  const Operand &o = is_key ? k : q;
-  const int block = is_key ? blockIdx.x - q_blocks : blockIdx.x;
-  const int blocks = is_key ? gridDim.x - q_blocks : q_blocks;
-  const bool lane_live = e * 16 < r.columns;
+  const bool is_key = (int)blockIdx.x >= q_blocks, interleaved = r.interleaved;
+  const Operand o = is_key ? k : q;
+  const uint32_t block = is_key ? blockIdx.x - q_blocks : blockIdx.x;
+  const uint32_t step = (is_key ? gridDim.x - q_blocks : q_blocks) * kGroups, units = r.tokens * o.slices;
+  const bool inside = e * 16 < r.columns;
   int first, second;
   pieces(r, e, first, second);
-  float w[16], dw[16];
+  Row w, dw;
 #pragma unroll
-  for (int i = 0; i < 16; ++i) w[i] = dw[i] = 0.0f;
-  if (lane_live) {
+  for (int i = 0; i < 8; ++i) w.own[i] = dw.own[i] = {0.0f, 0.0f};
+  if (inside) {
     const T *weight = static_cast<const T *>(o.weight);
     Eight<T> w0, w1;
     w0.load(weight + first);
     w1.load(weight + second);
-    w0.widen(w);
-    w1.widen(w + 8);
+    w.widen(w0, w1);
   }
-  const int64_t units = (int64_t)r.tokens * o.slices;
+  const uint32_t step_token = step / o.slices, step_slice = step % o.slices;
+  Cursor load(block * kGroups, group, o.slices);
+  Cursor use = load;
+  int load_row = 0, load_rows = 0;
+  const T *x_source = nullptr, *grad_source = nullptr;
+  auto produce = [&](int stage) {
+    if (load.base < units) {
+      if (load_row == 0) {
+        const int head0 = (int)load.slice * unit_rows;
+        load_rows = load.base + group < units && inside ? min(unit_rows, o.heads - head0) : 0;
+        x_source = static_cast<const T *>(o.x) + (load_rows ? load.token * o.x_token + head0 * o.x_head : 0);
+        grad_source = static_cast<const T *>(o.grad) + (load_rows ? load.token * o.grad_token + head0 * o.grad_head : 0);
+      }
+      const bool live = load_row < load_rows;
+      const T *x = live ? x_source + load_row * o.x_head : x_source, *g = live ? grad_source + load_row * o.grad_head : grad_source;
+      ring.template copy<T>(stage, 0, x + first, live);
+      ring.template copy<T>(stage, 1, x + second, live);
+      ring.template copy<T>(stage, 2, g + first, live);
+      ring.template copy<T>(stage, 3, g + second, live);
+      if (++load_row == unit_rows) {
+        load_row = 0;
+        load.advance(step, step_token, step_slice, o.slices);
+      }
+    }
+    ring.commit();
+  };
+#pragma unroll
+  for (int i = 0; i < kStages - 1; ++i) produce(i);
+  int stage = 0;
   // every group of the block runs the same number of rounds: the shuffles below are whole-warp
-  for (int64_t base = (int64_t)block * kGroups; base < units; base += (int64_t)blocks * kGroups) {
-    const int64_t unit = base + group;
-    const bool unit_live = unit < units;
-    const int token = unit_live ? (int)(unit / o.slices) : 0;
-    const int head0 = unit_live ? (int)(unit - (int64_t)token * o.slices) * kUnitRows : 0;
-    const int rows = unit_live ? min(kUnitRows, o.heads - head0) : 0;
-    const int position = unit_live ? place(r, token, e == 0) : -1;
-    const bool turned = lane_live && e * 8 < r.half && position >= 0;
-    float cosine[8], sine[8];
+  for (; use.base < units; use.advance(step, step_token, step_slice, o.slices)) {
+    const uint32_t unit = use.base + group, token = use.token;
+    const int head0 = (int)use.slice * unit_rows;
+    const int rows = unit < units && inside ? min(unit_rows, o.heads - head0) : 0;
+    const int position = unit < units ? place(r, token, e == 0) : -1;
+    const bool turned = inside && e * 8 < r.half && position >= 0;
+    Row straight, crossed;
     if (turned) {
-      const float *c = r.cosine + position * r.cosine_row + 8 * e, *s = r.sine + position * r.sine_row + 8 * e;
+      angles<true>(r, e, position, straight, crossed);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) { cosine[i] = __ldg(c + i); sine[i] = __ldg(s + i); }
+      for (int i = 0; i < 8; ++i) straight.own[i] = {1.0f, 1.0f};
     }
-    const T *x_row = static_cast<const T *>(o.x) + token * o.x_token + head0 * o.x_head;
-    const T *grad_row = static_cast<const T *>(o.grad) + token * o.grad_token + head0 * o.grad_head;
-    T *out_row = static_cast<T *>(o.out) + token * o.out_token + head0 * o.out_head;
-#pragma unroll 2
-    for (int row = 0; row < kUnitRows; ++row) {
-      const bool live = lane_live && row < rows;
-      Eight<T> xa, xb, ga, gb;
-      xa.clear(); xb.clear(); ga.clear(); gb.clear();
-      if (live && position >= 0) {
-        xa.load(x_row + row * o.x_head + first);
-        xb.load(x_row + row * o.x_head + second);
-        ga.load(grad_row + row * o.grad_head + first);
-        gb.load(grad_row + row * o.grad_head + second);
+    T *target = static_cast<T *>(o.out) + (rows ? token * o.out_token + head0 * o.out_head : 0);
+#pragma unroll 1
+    for (int row = 0; row < unit_rows; ++row) {
+      produce(stage == 0 ? kStages - 1 : stage - 1);
+      ring.wait();
+      Row x, g;
+      x.widen(ring.template take<T>(stage, 0), ring.template take<T>(stage, 1));
+      g.widen(ring.template take<T>(stage, 2), ring.template take<T>(stage, 3));
+      stage = stage == kStages - 1 ? 0 : stage + 1;
+      if (position < 0) {   // padding may hold anything, and adds nothing
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x.own[i] = g.own[i] = {0.0f, 0.0f};
       }
-      float x[16], g[16];
-      xa.widen(x); xb.widen(x + 8);
-      ga.widen(g); gb.widen(g + 8);
-      float squares = 0.0f;
+      const float squares = heads::row_sum<LANES>(x.dot(x));
+      // 0 where nothing counts: with epsilon 0 a row of zeros has no finite one
+      const float rstd = row < rows && position >= 0 ? rsqrtf(squares * r.inverse_columns + r.epsilon) : 0.0f;
+      g = turned_row(g, straight, crossed, turned, interleaved);
 #pragma unroll
-      for (int j = 0; j < 16; ++j) squares += x[j] * x[j];
-      squares = heads::row_sum<LANES>(squares);
-      const float rstd = __fdiv_rn(1.0f, __fsqrt_rn(squares * r.inverse_columns + r.epsilon));
-      if (turned) turn<true>(g, cosine, sine, r.interleaved);
-      float projection = 0.0f;
-#pragma unroll
-      for (int j = 0; j < 16; ++j) {
-        x[j] *= rstd;
-        dw[j] += g[j] * x[j];
-        g[j] *= w[j];
-        projection += g[j] * x[j];
+      for (int i = 0; i < 8; ++i) {
+        x.own[i] = mul(x.own[i], Two{rstd, rstd});
+        dw.own[i] = fma(g.own[i], x.own[i], dw.own[i]);
+        g.own[i] = mul(g.own[i], w.own[i]);
       }
-      projection = heads::row_sum<LANES>(projection) * r.inverse_columns;
-      if (live) {
+      const float projection = -heads::row_sum<LANES>(g.dot(x)) * r.inverse_columns;
+      if (row < rows) {
 #pragma unroll
-        for (int j = 0; j < 16; ++j) g[j] = position < 0 ? 0.0f : rstd * (g[j] - x[j] * projection);
-        xa.narrow(g);
-        xb.narrow(g + 8);
-        xa.store(out_row + row * o.out_head + first);
-        xb.store(out_row + row * o.out_head + second);
+        for (int i = 0; i < 8; ++i)
+          g.own[i] = mul(fma(x.own[i], Two{projection, projection}, g.own[i]), Two{rstd, rstd});
+        Eight<T> a, b;
+        g.narrow(a, b);
+        a.store(target + row * o.out_head + first);
+        b.store(target + row * o.out_head + second);
       }
     }
   }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncthreads();
+  float(*sums)[LANES * 16 + 1] = reinterpret_cast<float(*)[LANES * 16 + 1]>(dynamic_smem);
 #pragma unroll
-  for (int i = 0; i < 16; ++i) sums[group][i * LANES + e] = dw[i];
+  for (int i = 0; i < 8; ++i) {
+    sums[group][2 * i * LANES + e] = dw.own[i].a;
+    sums[group][(2 * i + 1) * LANES + e] = dw.own[i].b;
+  }
   __syncthreads();
   for (int slot = threadIdx.x; slot < LANES * 16; slot += kThreads) {
     const int owner = slot % LANES, i = slot / LANES;
@@ -288,15 +443,10 @@ head_norm_rotary_reduce_kernel(const float *__restrict__ partial, int q_blocks, 
 // --------------------------------------------------------------------- host
 struct Arguments {
   View3 q, k;
-  const void *q_weight, *k_weight;
-  int64_t q_weight_d0, q_weight_s0, k_weight_d0, k_weight_s0;
-  const void *cosine, *sine;
-  int64_t cos_d0, cos_d1, cos_s0, cos_s1, sin_d0, sin_d1, sin_s0, sin_s1;
-  const void *positions;
-  int64_t positions_d0, positions_s0;
+  View1 q_weight, k_weight;
+  View2 cosine, sine;
+  View1 positions, workspace;
   float epsilon;
-  void *workspace;
-  int64_t ws_d0, ws_s0;
   int32_t dtype, interleaved;
 };
 
@@ -317,19 +467,19 @@ int check(const char *what, const Arguments &a, const View3 *const *rows, int ro
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: head_dim %lld is not a multiple of 16 in [16, 256]", what, (long long)columns);
   if (tokens >= (int64_t(1) << 31) || a.q.d1 > 65536 || a.k.d1 > 65536)
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: 2^31 tokens or more, or more than 65536 heads", what);
-  if (a.q_weight_d0 != columns || a.k_weight_d0 != columns)
+  if (a.q_weight.d0 != columns || a.k_weight.d0 != columns)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: a weight does not have head_dim entries", what);
-  if (a.cos_d0 != a.sin_d0 || a.cos_d1 != a.sin_d1 || a.cos_d0 < 0 || a.cos_d1 < 0)
+  if (a.cosine.d0 != a.sine.d0 || a.cosine.d1 != a.sine.d1 || a.cosine.d0 < 0 || a.cosine.d1 < 0)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the cosine and sine tables differ in shape", what);
-  if (a.cos_d1 < 8 || a.cos_d1 % 8 || 2 * a.cos_d1 > columns)
-    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: %lld rotated pairs are not a multiple of 8 within head_dim", what, (long long)a.cos_d1);
-  if (a.cos_d0 >= (int64_t(1) << 31))
+  if (a.cosine.d1 < 8 || a.cosine.d1 % 8 || 2 * a.cosine.d1 > columns)
+    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: %lld rotated pairs are not a multiple of 8 within head_dim", what, (long long)a.cosine.d1);
+  if (a.cosine.d0 >= (int64_t(1) << 31))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the tables have 2^31 rows or more", what);
-  if (a.positions_d0 != tokens) return fail(B200_ERR_INVALID_ARGUMENT, "%s: positions does not have one entry a token", what);
-  if (!heads::sane(a.positions_d0, a.positions_s0) || !heads::sane(a.cos_d0, a.cos_s0) || !heads::sane(a.sin_d0, a.sin_s0))
+  if (a.positions.d0 != tokens) return fail(B200_ERR_INVALID_ARGUMENT, "%s: positions does not have one entry a token", what);
+  if (!heads::sane(a.positions.d0, a.positions.s0) || !heads::sane(a.cosine.d0, a.cosine.s0) || !heads::sane(a.sine.d0, a.sine.s0))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: negative or huge extent or stride", what);
   if (!(a.epsilon >= 0.0f) || isinf(a.epsilon)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: epsilon is not a number >= 0", what);
-  if (!a.workspace || a.ws_d0 < B200_WORKSPACE_WORDS || a.ws_s0 != 1)
+  if (!a.workspace.data || a.workspace.d0 < B200_WORKSPACE_WORDS || a.workspace.s0 != 1)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the workspace needs %d contiguous int32 words", what, B200_WORKSPACE_WORDS);
   for (int i = 0; i < row_views; ++i) {
     const View3 &v = *rows[i];
@@ -338,12 +488,12 @@ int check(const char *what, const Arguments &a, const View3 *const *rows, int ro
       return fail(B200_ERR_UNSUPPORTED_LAYOUT,
                   "%s: rows need a unit inner stride, a 16-byte aligned base and outer strides of whole 16-byte steps", what);
   }
-  if (tokens && (!a.q_weight || !a.k_weight || !a.positions || (a.cos_d0 && (!a.cosine || !a.sine))))
+  if (tokens && (!a.q_weight.data || !a.k_weight.data || !a.positions.data || (a.cosine.d0 && (!a.cosine.data || !a.sine.data))))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  if (a.q_weight_s0 != 1 || a.k_weight_s0 != 1 || !aligned16(a.q_weight) || !aligned16(a.k_weight))
+  if (a.q_weight.s0 != 1 || a.k_weight.s0 != 1 || !aligned16(a.q_weight.data) || !aligned16(a.k_weight.data))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: weights need a unit stride and a 16-byte aligned base", what);
-  if (a.cos_s1 != 1 || a.sin_s1 != 1 || !aligned16(a.cosine) || !aligned16(a.sine) ||
-      (a.cos_d0 > 1 && (a.cos_s0 % 4 || a.sin_s0 % 4)))
+  if (a.cosine.s1 != 1 || a.sine.s1 != 1 || !aligned16(a.cosine.data) || !aligned16(a.sine.data) ||
+      (a.cosine.d0 > 1 && (a.cosine.s0 % 4 || a.sine.s0 % 4)))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT,
                 "%s: tables need a unit inner stride, a 16-byte aligned base and a row pitch of whole 16-byte steps", what);
   return B200_OK;
@@ -390,61 +540,77 @@ Operand operand(const View3 &x, const View3 *grad, const void *weight, const Vie
   o.out_token = out.s0;
   o.out_head = out.s1;
   o.heads = (int)x.d1;
-  o.slices = (int)((x.d1 + rows - 1) / rows);
+  o.slices = (uint32_t)((x.d1 + rows - 1) / rows);
   return o;
 }
 
 Rotation rotation(const Arguments &a) {
   Rotation r{};
-  r.cosine = static_cast<const float *>(a.cosine);
-  r.sine = static_cast<const float *>(a.sine);
-  r.cosine_row = a.cos_s0;
-  r.sine_row = a.sin_s0;
-  r.table_rows = (int)a.cos_d0;
-  r.half = (int)a.cos_d1;
+  r.cosine = static_cast<const float *>(a.cosine.data);
+  r.sine = static_cast<const float *>(a.sine.data);
+  r.cosine_row = a.cosine.s0;
+  r.sine_row = a.sine.s0;
+  r.table_rows = (int)a.cosine.d0;
+  r.half = (int)a.cosine.d1;
   r.columns = (int)a.q.d2;
   r.interleaved = a.interleaved;
-  r.positions = static_cast<const int *>(a.positions);
-  r.positions_step = a.positions_s0;
+  r.positions = static_cast<const int *>(a.positions.data);
+  r.positions_step = a.positions.s0;
   r.tokens = (int)a.q.d0;
   r.inverse_columns = 1.0f / (float)a.q.d2;
   r.epsilon = a.epsilon;
-  r.status = static_cast<int *>(a.workspace);
+  r.status = static_cast<int *>(const_cast<void *>(a.workspace.data));
   return r;
 }
 
-template <typename T, int ROWS> int launch_forward(const Arguments &a, const View3 &q_out, const View3 &k_out, cudaStream_t stream) {
-  const Operand q = operand(a.q, nullptr, a.q_weight, q_out, ROWS), k = operand(a.k, nullptr, a.k_weight, k_out, ROWS);
-  const Rotation r = rotation(a);
-  const int lanes = heads::row_lanes(r.columns);
-  const int64_t units = (int64_t)r.tokens * (q.slices + k.slices), per_block = kThreads / lanes;
-  const int64_t blocks = (units + per_block - 1) / per_block;
-  if (blocks >= (int64_t(1) << 31)) return fail(B200_ERR_UNSUPPORTED_LAYOUT, "head_norm_rotary: too many rows for one launch");
-  switch (lanes) {
-  case 1: head_norm_rotary_kernel<T, 1, ROWS><<<(unsigned)blocks, kThreads, 0, stream>>>(q, k, r); break;
-  case 2: head_norm_rotary_kernel<T, 2, ROWS><<<(unsigned)blocks, kThreads, 0, stream>>>(q, k, r); break;
-  case 4: head_norm_rotary_kernel<T, 4, ROWS><<<(unsigned)blocks, kThreads, 0, stream>>>(q, k, r); break;
-  case 8: head_norm_rotary_kernel<T, 8, ROWS><<<(unsigned)blocks, kThreads, 0, stream>>>(q, k, r); break;
-  default: head_norm_rotary_kernel<T, 16, ROWS><<<(unsigned)blocks, kThreads, 0, stream>>>(q, k, r); break;
+// Heads of a token that a unit takes: as many as leave every resident group of lanes some work, at most
+// 8 (one load of the angles is then a tenth of what the rows move), and so that no more than a seventh of
+// the rounds fall on rows that are not there.
+int rows_of_unit(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t columns) {
+  const int64_t groups = (int64_t)kBlocksPerSm * sm_count() * kThreads / heads::row_lanes(columns), all = q_heads + k_heads;
+  for (int64_t rows = 8; rows > 1; --rows) {
+    const int64_t units = (q_heads + rows - 1) / rows + (k_heads + rows - 1) / rows;
+    if (tokens * units >= groups && units * rows * 7 <= all * 8) return (int)rows;
   }
+  return 1;
+}
+
+template <typename T, int LANES>
+int launch_forward(const Operand &q, const Operand &k, const Rotation &r, int unit_rows, cudaStream_t stream) {
+  constexpr int kBytes = Ring<2 * Eight<T>::kVectors, kForwardStages<T>>::kBytes, kGroups = kThreads / LANES;
+  const auto kernel = head_norm_rotary_kernel<T, LANES>;
+  B200_CUDA_TRY(opt_in_dynamic_smem(kernel, kBytes));
+  const int64_t units = (int64_t)r.tokens * (q.slices + k.slices), need = (units + kGroups - 1) / kGroups;
+  const int64_t resident = (int64_t)kBlocksPerSm * sm_count();
+  kernel<<<(unsigned)(need < resident ? need : resident), kThreads, kBytes, stream>>>(q, k, r, unit_rows, (uint32_t)units);
   B200_CUDA_TRY(cudaGetLastError());
   return B200_OK;
 }
 
 template <typename T> int forward(const Arguments &a, const View3 &q_out, const View3 &k_out, cudaStream_t stream) {
-  return launch_forward<T, 1>(a, q_out, k_out, stream);
+  const int unit_rows = rows_of_unit(a.q.d0, a.q.d1, a.k.d1, a.q.d2);
+  const Operand q = operand(a.q, nullptr, a.q_weight.data, q_out, unit_rows), k = operand(a.k, nullptr, a.k_weight.data, k_out, unit_rows);
+  const int status = heads::check_units("head_norm_rotary", a.q.d0, (int64_t)q.slices + k.slices);
+  if (status != B200_OK) return status;
+  const Rotation r = rotation(a);
+  switch (heads::row_lanes(r.columns)) {
+  case 1: return launch_forward<T, 1>(q, k, r, unit_rows, stream);
+  case 2: return launch_forward<T, 2>(q, k, r, unit_rows, stream);
+  case 4: return launch_forward<T, 4>(q, k, r, unit_rows, stream);
+  case 8: return launch_forward<T, 8>(q, k, r, unit_rows, stream);
+  default: return launch_forward<T, 16>(q, k, r, unit_rows, stream);
+  }
 }
 
 // Blocks of the backward pass: as many as are resident at once, q's and k's in proportion to their rows.
 struct BackwardShape {
-  int q_blocks, blocks;
+  int unit_rows, q_blocks, blocks;
 };
 BackwardShape backward_shape(int64_t tokens, int64_t q_heads, int64_t k_heads, int64_t columns) {
+  const int unit_rows = rows_of_unit(tokens, q_heads, k_heads, columns);
   const int64_t groups = kThreads / heads::row_lanes(columns);
-  const auto need = [&](int64_t heads) {
-    return (tokens * ((heads + kUnitRows - 1) / kUnitRows) + groups - 1) / groups;
-  };
-  const int64_t most = 3 * (int64_t)sm_count(), q_need = need(q_heads), k_need = need(k_heads);
+  const auto need = [&](int64_t heads) { return (tokens * ((heads + unit_rows - 1) / unit_rows) + groups - 1) / groups; };
+  const int64_t most = (int64_t)kBlocksPerSm * sm_count(), q_need = need(q_heads), k_need = need(k_heads);
   int64_t q_blocks = q_need, k_blocks = k_need;
   if (q_need + k_need > most) {
     q_blocks = most * q_need / (q_need + k_need);
@@ -452,23 +618,30 @@ BackwardShape backward_shape(int64_t tokens, int64_t q_heads, int64_t k_heads, i
     k_blocks = most - q_blocks;
     if (k_blocks < 1 && k_need) { k_blocks = 1; q_blocks = most - 1; }
   }
-  return {(int)q_blocks, (int)(q_blocks + k_blocks)};
+  return {unit_rows, (int)q_blocks, (int)(q_blocks + k_blocks)};
 }
 
 template <typename T, int LANES>
 cudaError_t launch_backward(const Operand &q, const Operand &k, const Rotation &r, const BackwardShape &shape, float *partial,
                             cudaStream_t stream) {
-  if (shape.blocks)
-    head_norm_rotary_backward_kernel<T, LANES><<<shape.blocks, kThreads, 0, stream>>>(q, k, r, shape.q_blocks, partial);
+  if (!shape.blocks) return cudaSuccess;
+  constexpr int kBytes = Ring<4 * Eight<T>::kVectors, kBackwardStages<T>>::kBytes;
+  const auto kernel = head_norm_rotary_backward_kernel<T, LANES>;
+  const cudaError_t error = opt_in_dynamic_smem(kernel, kBytes);
+  if (error != cudaSuccess) return error;
+  kernel<<<shape.blocks, kThreads, kBytes, stream>>>(q, k, r, shape.unit_rows, shape.q_blocks, partial);
   return cudaGetLastError();
 }
 
 template <typename T>
 int backward(const Arguments &a, const View3 &grad_q, const View3 &grad_k, const View3 &dq, const View3 &dk, float *partial,
              float *dq_weight, float *dk_weight, cudaStream_t stream) {
-  const Operand q = operand(a.q, &grad_q, a.q_weight, dq, kUnitRows), k = operand(a.k, &grad_k, a.k_weight, dk, kUnitRows);
-  const Rotation r = rotation(a);
   const BackwardShape shape = backward_shape(a.q.d0, a.q.d1, a.k.d1, a.q.d2);
+  const Operand q = operand(a.q, &grad_q, a.q_weight.data, dq, shape.unit_rows);
+  const Operand k = operand(a.k, &grad_k, a.k_weight.data, dk, shape.unit_rows);
+  const int status = heads::check_units("head_norm_rotary_backward", a.q.d0, (int64_t)q.slices + k.slices);
+  if (status != B200_OK) return status;
+  const Rotation r = rotation(a);
   cudaError_t error;
   switch (heads::row_lanes(r.columns)) {
   case 1: error = launch_backward<T, 1>(q, k, r, shape, partial, stream); break;
@@ -498,29 +671,24 @@ int backward(const Arguments &a, const View3 &grad_q, const View3 &grad_k, const
 
 using namespace b200;
 
-#define VIEW3(name) \
-  View3 { name, name##_d0, name##_d1, name##_d2, name##_s0, name##_s1, name##_s2 }
-#define ARGUMENTS                                                                                                        \
-  Arguments {                                                                                                            \
-    VIEW3(q), VIEW3(k), q_weight, k_weight, q_weight_d0, q_weight_s0, k_weight_d0, k_weight_s0, cosine, sine, cosine_d0, \
-        cosine_d1, cosine_s0, cosine_s1, sine_d0, sine_d1, sine_s0, sine_s1, positions, positions_d0, positions_s0,      \
-        epsilon, workspace, ws_d0, ws_s0, dtype, interleaved                                                             \
-  }
-
-extern "C" int b200_head_norm_rotary(
-    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
-    const void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
-    const void *q_weight, int64_t q_weight_d0, int64_t q_weight_s0,
-    const void *k_weight, int64_t k_weight_d0, int64_t k_weight_s0,
-    const void *cosine, int64_t cosine_d0, int64_t cosine_d1, int64_t cosine_s0, int64_t cosine_s1,
-    const void *sine, int64_t sine_d0, int64_t sine_d1, int64_t sine_s0, int64_t sine_s1,
-    const void *positions, int64_t positions_d0, int64_t positions_s0,
-    void *q_out, int64_t q_out_d0, int64_t q_out_d1, int64_t q_out_d2, int64_t q_out_s0, int64_t q_out_s1, int64_t q_out_s2,
-    void *k_out, int64_t k_out_d0, int64_t k_out_d1, int64_t k_out_d2, int64_t k_out_s0, int64_t k_out_s1, int64_t k_out_s2,
-    float epsilon, void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t interleaved, void *stream) {
+extern "C" int b200_head_norm_rotary(const int64_t *slots, int64_t count, float epsilon, int32_t dtype, int32_t interleaved,
+                                     void *stream) {
   const char *what = "head_norm_rotary";
-  const Arguments a = ARGUMENTS;
-  const View3 to_q = VIEW3(q_out), to_k = VIEW3(k_out);
+  heads::Slots from(slots, count);
+  Arguments a{};
+  a.q = from.view3();
+  a.k = from.view3();
+  a.q_weight = from.view1();
+  a.k_weight = from.view1();
+  a.cosine = from.view2();
+  a.sine = from.view2();
+  a.positions = from.view1();
+  const View3 to_q = from.view3(), to_k = from.view3();
+  a.workspace = from.view1();
+  if (!from.exact()) return fail(B200_ERR_INVALID_ARGUMENT, "%s: %lld slots do not describe its views", what, (long long)count);
+  a.epsilon = epsilon;
+  a.dtype = dtype;
+  a.interleaved = interleaved;
   const View3 *const rows[] = {&a.q, &a.k, &to_q, &to_k};
   int status = check(what, a, rows, 4);
   if (status != B200_OK) return status;
@@ -545,42 +713,46 @@ extern "C" int b200_head_norm_rotary_scratch(int64_t tokens, int64_t q_heads, in
   return B200_OK;
 }
 
-extern "C" int b200_head_norm_rotary_backward(
-    const void *grad_q, int64_t grad_q_d0, int64_t grad_q_d1, int64_t grad_q_d2, int64_t grad_q_s0, int64_t grad_q_s1, int64_t grad_q_s2,
-    const void *grad_k, int64_t grad_k_d0, int64_t grad_k_d1, int64_t grad_k_d2, int64_t grad_k_s0, int64_t grad_k_s1, int64_t grad_k_s2,
-    const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2, int64_t q_s0, int64_t q_s1, int64_t q_s2,
-    const void *k, int64_t k_d0, int64_t k_d1, int64_t k_d2, int64_t k_s0, int64_t k_s1, int64_t k_s2,
-    const void *q_weight, int64_t q_weight_d0, int64_t q_weight_s0,
-    const void *k_weight, int64_t k_weight_d0, int64_t k_weight_s0,
-    const void *cosine, int64_t cosine_d0, int64_t cosine_d1, int64_t cosine_s0, int64_t cosine_s1,
-    const void *sine, int64_t sine_d0, int64_t sine_d1, int64_t sine_s0, int64_t sine_s1,
-    const void *positions, int64_t positions_d0, int64_t positions_s0,
-    void *dq, int64_t dq_d0, int64_t dq_d1, int64_t dq_d2, int64_t dq_s0, int64_t dq_s1, int64_t dq_s2,
-    void *dk, int64_t dk_d0, int64_t dk_d1, int64_t dk_d2, int64_t dk_s0, int64_t dk_s1, int64_t dk_s2,
-    void *dq_weight, int64_t dq_weight_d0, int64_t dq_weight_s0, void *dk_weight, int64_t dk_weight_d0, int64_t dk_weight_s0,
-    void *partial, int64_t partial_d0, int64_t partial_d1, int64_t partial_s0, int64_t partial_s1,
-    float epsilon, void *workspace, int64_t ws_d0, int64_t ws_s0, int32_t dtype, int32_t interleaved, void *stream) {
+extern "C" int b200_head_norm_rotary_backward(const int64_t *slots, int64_t count, float epsilon, int32_t dtype,
+                                              int32_t interleaved, void *stream) {
   const char *what = "head_norm_rotary_backward";
-  const Arguments a = ARGUMENTS;
-  const View3 from_q = VIEW3(grad_q), from_k = VIEW3(grad_k), to_q = VIEW3(dq), to_k = VIEW3(dk);
+  heads::Slots from(slots, count);
+  Arguments a{};
+  const View3 from_q = from.view3(), from_k = from.view3();
+  a.q = from.view3();
+  a.k = from.view3();
+  a.q_weight = from.view1();
+  a.k_weight = from.view1();
+  a.cosine = from.view2();
+  a.sine = from.view2();
+  a.positions = from.view1();
+  const View3 to_q = from.view3(), to_k = from.view3();
+  const View1 to_q_weight = from.view1(), to_k_weight = from.view1();
+  const View2 partial = from.view2();
+  a.workspace = from.view1();
+  if (!from.exact()) return fail(B200_ERR_INVALID_ARGUMENT, "%s: %lld slots do not describe its views", what, (long long)count);
+  a.epsilon = epsilon;
+  a.dtype = dtype;
+  a.interleaved = interleaved;
   const View3 *const rows[] = {&a.q, &a.k, &from_q, &from_k, &to_q, &to_k};
   int status = check(what, a, rows, 6);
   if (status != B200_OK) return status;
-  if (!dq_weight || !dk_weight || dq_weight_d0 != a.q.d2 || dk_weight_d0 != a.q.d2)
+  if (!to_q_weight.data || !to_k_weight.data || to_q_weight.d0 != a.q.d2 || to_k_weight.d0 != a.q.d2)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: a weight's gradient does not have head_dim entries", what);
-  if (dq_weight_s0 != 1 || dk_weight_s0 != 1)
+  if (to_q_weight.s0 != 1 || to_k_weight.s0 != 1)
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the weights' gradients need a unit stride", what);
   const BackwardShape shape = backward_shape(a.q.d0, a.q.d1, a.k.d1, a.q.d2);
-  if (partial_d0 < shape.blocks || partial_d1 != a.q.d2 || (shape.blocks && !partial))
+  if (partial.d0 < shape.blocks || partial.d1 != a.q.d2 || (shape.blocks && !partial.data))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the scratch needs (%d, head_dim) f32", what, shape.blocks);
-  if (partial_s1 != 1 || (shape.blocks > 1 && partial_s0 != partial_d1))
+  if (partial.s1 != 1 || (shape.blocks > 1 && partial.s0 != partial.d1))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the scratch is contiguous", what);
   const int size = heads::element_size(dtype);
   status = check_output(what, to_q, size, rows, 4, &to_k);
   if (status == B200_OK) status = check_output(what, to_k, size, rows, 4, nullptr);
   if (status != B200_OK) return status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
-  float *scratch = static_cast<float *>(partial), *dqw = static_cast<float *>(dq_weight), *dkw = static_cast<float *>(dk_weight);
+  float *scratch = static_cast<float *>(const_cast<void *>(partial.data));
+  float *dqw = static_cast<float *>(const_cast<void *>(to_q_weight.data)), *dkw = static_cast<float *>(const_cast<void *>(to_k_weight.data));
   switch (dtype) {
   case B200_F32: return backward<float>(a, from_q, from_k, to_q, to_k, scratch, dqw, dkw, s);
   case B200_F16: return backward<__half>(a, from_q, from_k, to_q, to_k, scratch, dqw, dkw, s);

@@ -13,6 +13,8 @@ buffers: contiguous ``torch.empty`` on the argument device
 from __future__ import annotations
 
 import ctypes
+from array import array
+from functools import lru_cache
 
 import torch
 
@@ -285,35 +287,81 @@ def attention_backward_dq(q, k, v, grad_output, lse, delta, scale: float, *, hea
     return grad_q
 
 
-def _status_workspace(device: torch.device) -> torch.Tensor:
-    """``workspace(device)`` for entries that record a bad index there.  It is made once per device and
+# ---- operators around a key-value cache ------------------------------------------------------
+# Calls of a few microseconds on the device: a view is checked and turned into its slots in one go,
+# and the slots cross the C ABI as one array (see include/intent_b200.h).
+
+def _cuda_device(tensor) -> int:
+    """Index of the device that the call runs on, from its first tensor."""
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError("intent_b200 operators take torch.Tensor arguments")
+    if tensor.device.type != "cuda":
+        raise ValueError(f"intent_b200 executes on cuda, but an argument is on {tensor.device}")
+    return tensor.get_device()
+
+
+def _bound(name: str, tensor, dtype: torch.dtype, shape: tuple, device: int) -> tuple:
+    """The slots of a view that has this type, shape and device, or the error that says what it lacks."""
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if tensor.dtype is not dtype or tensor.shape != shape:
+        _expect(name, tensor, dtype, shape)
+    if tensor.get_device() != device:
+        _cuda_device(tensor)
+        raise ValueError("arguments span different devices")
+    return (tensor.data_ptr(), *shape, *tensor.stride())
+
+
+def _invoke(name: str, device: int, slots: tuple, *tail) -> None:
+    packed = array("q", slots)
+    address, count = packed.buffer_info()
+    if torch.cuda.current_device() == device:
+        status = _native.entry(name)(address, count, *tail, torch._C._cuda_getCurrentRawStream(device))
+    else:
+        with torch.cuda.device(device):
+            status = _native.entry(name)(address, count, *tail, torch._C._cuda_getCurrentRawStream(device))
+    if status != _native.OK:
+        _native.check(name, status)
+
+
+_status_slots: dict[int, tuple] = {}
+
+
+def _status(device: int) -> tuple:
+    """The slots of ``workspace(device)``, where an entry records a bad index.  It is made once per device and
     shared by all streams, so the first call may not fall into a graph capture, whose replays would
     clear it, and its zeros have to be there before any other stream writes to it."""
-    if device not in _workspaces:
-        with torch.cuda.device(device):
+    if device not in _status_slots:
+        where = torch.device("cuda", device)
+        with torch.cuda.device(where):
             if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("call intent_b200.ops.workspace(device) once before capturing this operator into a graph")
-            workspace(device)
-            torch.cuda.current_stream(device).synchronize()
-    return _workspaces[device]
+                raise RuntimeError("call this operator once outside a graph capture before capturing it")
+            space = workspace(where)
+            torch.cuda.current_stream(where).synchronize()
+        _status_slots[device] = tuple(_slots(space))
+    return _status_slots[device]
 
 
-def _scratch_size(name: str, device: torch.device, *arguments) -> int:
+@lru_cache(maxsize=4096)
+def _scratch_size(name: str, device: int, *arguments) -> int:
     size = ctypes.c_int64(0)
-    _call(name, device, *arguments, ctypes.byref(size))
+    _call(name, torch.device("cuda", device), *arguments, ctypes.byref(size))
     return size.value
 
 
-def _rotary_operands(q, k, q_weight, k_weight, cos, sin, positions) -> None:
+def _shape(name: str, tensor, rank: int, axes: str) -> tuple:
+    if not isinstance(tensor, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if tensor.dim() != rank:
+        raise ValueError(f"{name} is a {axes} tensor, got {tuple(tensor.shape)}")
+    return tuple(tensor.shape)
+
+
+def _rotary_shapes(q, k, cos) -> tuple:
+    shape = _shape("q", q, 3, "(tokens, heads, head_dim)")
+    k_shape = (shape[0], _shape("k", k, 3, "(tokens, heads, head_dim)")[1], shape[2])
     _float_type("q", q)
-    if q.dim() != 3 or k.dim() != 3 or cos.dim() != 2:
-        raise ValueError("q and k are (tokens, heads, head_dim) tensors, cos and sin (rows, pairs)")
-    _expect("k", k, q.dtype, (q.shape[0], k.shape[1], q.shape[2]))
-    _expect("q_weight", q_weight, q.dtype, (q.shape[2],))
-    _expect("k_weight", k_weight, q.dtype, (q.shape[2],))
-    _expect("cos", cos, torch.float32)
-    _expect("sin", sin, torch.float32, cos.shape)
-    _expect("positions", positions, torch.int32, (q.shape[0],))
+    return shape, k_shape, _shape("cos", cos, 2, "(rows, pairs)")
 
 
 def head_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, epsilon: float = 1e-6, *, interleaved: bool = False,
@@ -324,17 +372,20 @@ def head_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, epsilon: flo
     columns from ``2 * pairs`` on are not turned.  ``positions`` (tokens,) int32: a negative one marks
     padding, whose rows become zeros; one behind the tables gives zeros too and is reported by
     ``workspace_status``.  Returns ``(q_out, k_out)``; an output may be its input."""
-    device = _require_cuda(q, k, q_weight, k_weight, cos, sin, positions, *(t for t in (q_out, k_out) if t is not None))
-    _rotary_operands(q, k, q_weight, k_weight, cos, sin, positions)
+    device = _cuda_device(q)
+    shape, k_shape, table = _rotary_shapes(q, k, cos)
+    dtype = q.dtype
     if q_out is None:
-        q_out = torch.empty(q.shape, dtype=q.dtype, device=device)
+        q_out = q.new_empty(shape)
     if k_out is None:
-        k_out = torch.empty(k.shape, dtype=k.dtype, device=device)
-    _expect("q_out", q_out, q.dtype, q.shape)
-    _expect("k_out", k_out, k.dtype, k.shape)
-    _call("b200_head_norm_rotary", device, *_slots(q), *_slots(k), *_slots(q_weight), *_slots(k_weight), *_slots(cos),
-          *_slots(sin), *_slots(positions), *_slots(q_out), *_slots(k_out), float(epsilon),
-          *_slots(_status_workspace(device)), _CODES[q.dtype], int(bool(interleaved)), _stream(q))
+        k_out = q.new_empty(k_shape)
+    _invoke("b200_head_norm_rotary", device,
+            (*_bound("q", q, dtype, shape, device), *_bound("k", k, dtype, k_shape, device),
+             *_bound("q_weight", q_weight, dtype, shape[2:], device), *_bound("k_weight", k_weight, dtype, shape[2:], device),
+             *_bound("cos", cos, torch.float32, table, device), *_bound("sin", sin, torch.float32, table, device),
+             *_bound("positions", positions, torch.int32, shape[:1], device), *_bound("q_out", q_out, dtype, shape, device),
+             *_bound("k_out", k_out, dtype, k_shape, device), *_status(device)),
+            float(epsilon), _CODES[dtype], bool(interleaved))
     return q_out, k_out
 
 
@@ -343,136 +394,132 @@ def head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin
     """The gradients of ``head_norm_rotary``'s inputs from those of its outputs: ``(dq, dk, dq_weight,
     dk_weight)``, the weights' in f32.  Rows of padding get zeros and add nothing.  ``dq`` may be
     ``grad_q`` or ``q``, and ``dk`` likewise."""
-    device = _require_cuda(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions,
-                           *(t for t in (dq, dk) if t is not None))
-    _rotary_operands(q, k, q_weight, k_weight, cos, sin, positions)
-    _expect("grad_q", grad_q, q.dtype, q.shape)
-    _expect("grad_k", grad_k, k.dtype, k.shape)
+    device = _cuda_device(q)
+    shape, k_shape, table = _rotary_shapes(q, k, cos)
+    dtype, columns = q.dtype, shape[2:]
     if dq is None:
-        dq = torch.empty(q.shape, dtype=q.dtype, device=device)
+        dq = q.new_empty(shape)
     if dk is None:
-        dk = torch.empty(k.shape, dtype=k.dtype, device=device)
-    _expect("dq", dq, q.dtype, q.shape)
-    _expect("dk", dk, k.dtype, k.shape)
-    space = _status_workspace(device)
-    rows = _scratch_size("b200_head_norm_rotary_scratch", device, q.shape[0], q.shape[1], k.shape[1], q.shape[2])
-    partial = torch.empty((rows, q.shape[2]), dtype=torch.float32, device=device)
-    weights = torch.empty((2, q.shape[2]), dtype=torch.float32, device=device)
-    dq_weight, dk_weight = weights[0], weights[1]
-    _call("b200_head_norm_rotary_backward", device, *_slots(grad_q), *_slots(grad_k), *_slots(q), *_slots(k),
-          *_slots(q_weight), *_slots(k_weight), *_slots(cos), *_slots(sin), *_slots(positions), *_slots(dq), *_slots(dk),
-          *_slots(dq_weight), *_slots(dk_weight), *_slots(partial), float(epsilon), *_slots(space), _CODES[q.dtype],
-          int(bool(interleaved)), _stream(q))
+        dk = q.new_empty(k_shape)
+    rows = _scratch_size("b200_head_norm_rotary_scratch", device, shape[0], shape[1], k_shape[1], shape[2])
+    partial = q.new_empty((rows, shape[2]), dtype=torch.float32)    # the call's own: calls may overlap
+    dq_weight, dk_weight = q.new_empty(columns, dtype=torch.float32), q.new_empty(columns, dtype=torch.float32)
+    _invoke("b200_head_norm_rotary_backward", device,
+            (*_bound("grad_q", grad_q, dtype, shape, device), *_bound("grad_k", grad_k, dtype, k_shape, device),
+             *_bound("q", q, dtype, shape, device), *_bound("k", k, dtype, k_shape, device),
+             *_bound("q_weight", q_weight, dtype, columns, device), *_bound("k_weight", k_weight, dtype, columns, device),
+             *_bound("cos", cos, torch.float32, table, device), *_bound("sin", sin, torch.float32, table, device),
+             *_bound("positions", positions, torch.int32, shape[:1], device), *_bound("dq", dq, dtype, shape, device),
+             *_bound("dk", dk, dtype, k_shape, device), dq_weight.data_ptr(), shape[2], 1, dk_weight.data_ptr(), shape[2], 1,
+             partial.data_ptr(), rows, shape[2], shape[2], 1, *_status(device)),
+            float(epsilon), _CODES[dtype], bool(interleaved))
     return dq, dk, dq_weight, dk_weight
 
 
-_NO_SCALE = [None] + [0] * 6
+_NO_SCALES = (0,) * 14
+_CACHE_TYPES = (torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn)
 
 
-def _cache_operands(k_cache, v_cache, k_scale, v_scale) -> list:
-    """Checks a paged cache (pages, heads, page_size, head_dim) and returns its scales' slots."""
-    if k_cache.dtype not in (torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn):
-        raise TypeError(f"k_cache must be float16, bfloat16, int8 or float8_e4m3fn, got {k_cache.dtype}")
-    if k_cache.dim() != 4:
-        raise ValueError("a cache is a (pages, heads, page_size, head_dim) tensor")
-    _expect("v_cache", v_cache, k_cache.dtype, k_cache.shape)
-    if k_cache.element_size() == 2:
+def _cache_slots(k_cache, v_cache, k_scale, v_scale, device: int) -> tuple:
+    """Shape of a paged cache, its slots and its scales' slots."""
+    shape = _shape("k_cache", k_cache, 4, "(pages, heads, page_size, head_dim)")
+    dtype = k_cache.dtype
+    if dtype not in _CACHE_TYPES:
+        raise TypeError(f"k_cache must be float16, bfloat16, int8 or float8_e4m3fn, got {dtype}")
+    views = _bound("k_cache", k_cache, dtype, shape, device) + _bound("v_cache", v_cache, dtype, shape, device)
+    if dtype is torch.float16 or dtype is torch.bfloat16:
         if k_scale is not None or v_scale is not None:
             raise ValueError("a 16-bit cache has no scales")
-        return _NO_SCALE + _NO_SCALE
+        return shape, views, _NO_SCALES
     if k_scale is None or v_scale is None:
         raise ValueError("an 8-bit cache needs k_scale and v_scale")
-    _expect("k_scale", k_scale, torch.float32, k_cache.shape[:3])
-    _expect("v_scale", v_scale, torch.float32, k_cache.shape[:3])
-    return _slots(k_scale) + _slots(v_scale)
+    return shape, views, (_bound("k_scale", k_scale, torch.float32, shape[:3], device)
+                          + _bound("v_scale", v_scale, torch.float32, shape[:3], device))
 
 
 def cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
-    """Puts rows of keys and values (tokens, heads, head_dim), f16 or bf16, into the slots of a paged
-    cache (pages, heads, page_size, head_dim) of any memory order with a unit inner stride, in one launch;
-    slot = page * page_size + place, int64.  A cache of the rows' type gets them as they are.  One of int8 or float8_e4m3fn gets codes, and
-    ``k_scale`` / ``v_scale`` (pages, heads, page_size) f32 a scale for each row: the largest magnitude / 127, or
-    the power of two that brings it to at most 448; code * scale is the value.  A row with an infinity or a NaN reads
-    back as NaN throughout.  Negative slots mark padding and are skipped; so are slots behind the cache, which
-    ``workspace_status`` reports.  Slots of one call must differ.  Returns ``(k_cache, v_cache)``."""
-    scales = tuple(t for t in (k_scale, v_scale) if t is not None)
-    device = _require_cuda(k, v, slots, k_cache, v_cache, *scales)
-    _float_type("k", k, (torch.float16, torch.bfloat16))
-    scale_slots = _cache_operands(k_cache, v_cache, k_scale, v_scale)
-    if k_cache.element_size() == 2:
-        _expect("k_cache", k_cache, k.dtype)
-    if k.dim() != 3:
-        raise ValueError("k and v are (tokens, heads, head_dim) tensors")
-    _expect("k", k, k.dtype, (k.shape[0], k_cache.shape[1], k_cache.shape[3]))
-    _expect("v", v, k.dtype, k.shape)
-    _expect("slots", slots, torch.int64, (k.shape[0],))
-    _call("b200_cache_write", device, *_slots(k), *_slots(v), *_slots(slots), *_slots(k_cache), *_slots(v_cache), *scale_slots,
-          *_slots(_status_workspace(device)), _CODES[k.dtype], _CODES[k_cache.dtype], _stream(k))
+    """Puts rows of keys and values (tokens, heads, head_dim), f16 or bf16, into the slots of a paged cache
+    (pages, heads, page_size, head_dim) of any memory order with a unit inner stride, in one launch;
+    slot = page * page_size + place, int64.  A cache of the rows' type gets them as they are.  One of int8 or
+    float8_e4m3fn gets codes, and ``k_scale`` / ``v_scale`` (pages, heads, page_size) f32 a scale for each row:
+    the largest magnitude / 127, or the power of two that brings it to at most 448; code * scale is the value.
+    A row with an infinity or a NaN reads back as NaN throughout.  Negative slots mark padding and are
+    skipped; so are slots behind the cache, which ``workspace_status`` reports.  The slots of one call that are not
+    negative must differ.  Returns ``(k_cache, v_cache)``."""
+    device = _cuda_device(k)
+    dtype = _float_type("k", k, (torch.float16, torch.bfloat16))
+    cache, views, scales = _cache_slots(k_cache, v_cache, k_scale, v_scale, device)
+    if k_cache.dtype is not dtype and k_cache.element_size() == 2:
+        raise TypeError(f"k_cache must have dtype {dtype}, torch.int8 or torch.float8_e4m3fn, got {k_cache.dtype}")
+    shape = (_shape("k", k, 3, "(tokens, heads, head_dim)")[0], cache[1], cache[3])
+    _invoke("b200_cache_write", device,
+            (*_bound("k", k, dtype, shape, device), *_bound("v", v, dtype, shape, device),
+             *_bound("slots", slots, torch.int64, shape[:1], device), *views, *scales, *_status(device)),
+            _CODES[dtype], _CODES[k_cache.dtype])
     return k_cache, v_cache
 
 
 def cache_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, *, dtype=None, k_out=None, v_out=None):
-    """The rows of ``slots`` out of a cache that ``cache_write`` filled, ``(k, v)`` of shape (tokens, heads, head_dim):
-    of a 16-bit cache as they are, of an 8-bit one as code * scale in ``dtype`` (f16 or bf16, the default).
-    Negative slots give zeros, and so do slots behind the cache, which ``workspace_status`` reports."""
-    given = tuple(t for t in (k_scale, v_scale, k_out, v_out) if t is not None)
-    device = _require_cuda(k_cache, v_cache, slots, *given)
-    scale_slots = _cache_operands(k_cache, v_cache, k_scale, v_scale)
-    if slots.dim() != 1:
-        raise ValueError("slots has one axis")
-    _expect("slots", slots, torch.int64)
+    """The rows of ``slots`` out of a cache that ``cache_write`` filled, ``(k, v)`` of shape (tokens, heads,
+    head_dim): of a 16-bit cache as they are, of an 8-bit one as code * scale in ``dtype`` (f16 or bf16, the
+    default).  Negative slots give zeros, and so do slots behind the cache, which ``workspace_status`` reports."""
+    device = _cuda_device(k_cache)
+    cache, views, scales = _cache_slots(k_cache, v_cache, k_scale, v_scale, device)
+    wide = k_cache.element_size() == 2
     if dtype is None:
-        dtype = k_cache.dtype if k_cache.element_size() == 2 else k_out.dtype if k_out is not None else torch.bfloat16
+        dtype = k_cache.dtype if wide else torch.bfloat16 if k_out is None else k_out.dtype
     if dtype not in (torch.float16, torch.bfloat16):
         raise TypeError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
-    if k_cache.element_size() == 2 and dtype != k_cache.dtype:
+    if wide and dtype != k_cache.dtype:
         raise TypeError(f"a {k_cache.dtype} cache gives its rows as they are, not as {dtype}")
-    shape = (slots.shape[0], k_cache.shape[1], k_cache.shape[3])
+    shape = (_shape("slots", slots, 1, "(tokens,)")[0], cache[1], cache[3])
     if k_out is None:
-        k_out = torch.empty(shape, dtype=dtype, device=device)
+        k_out = k_cache.new_empty(shape, dtype=dtype)
     if v_out is None:
-        v_out = torch.empty(shape, dtype=dtype, device=device)
-    _expect("k_out", k_out, dtype, shape)
-    _expect("v_out", v_out, dtype, shape)
-    _call("b200_cache_read", device, *_slots(k_cache), *_slots(v_cache), *_slots(slots), *scale_slots, *_slots(k_out),
-          *_slots(v_out), *_slots(_status_workspace(device)), _CODES[dtype], _CODES[k_cache.dtype], _stream(k_cache))
+        v_out = k_cache.new_empty(shape, dtype=dtype)
+    _invoke("b200_cache_read", device,
+            (*views, *_bound("slots", slots, torch.int64, shape[:1], device), *scales,
+             *_bound("k_out", k_out, dtype, shape, device), *_bound("v_out", v_out, dtype, shape, device), *_status(device)),
+            _CODES[dtype], _CODES[k_cache.dtype])
     return k_out, v_out
 
 
 def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, k_scale=None, v_scale=None, out=None,
                     return_lse: bool = False):
-    """Attention of one new token a sequence: ``q`` (batch, heads, head_dim) over the first ``lengths[b]`` rows of each
-    sequence in a paged cache (``cache_write``), whose pages row ``b`` of ``block_table`` (batch, columns) names in
-    order; both int32.  heads is a multiple of the cache's heads, neighbouring query heads share a key head;
-    head_dim is 64 or 128.  A sequence of length 0 gets zeros (and lse -infinity).  What lies behind a sequence, in its last page or in
-    the table, is never used.  A page outside the cache is left out, a length past the table is cut there, and
-    ``workspace_status`` reports both.  Returns ``out``, or ``(out, lse)`` with the natural logarithm of the sums (f32)."""
-    given = tuple(t for t in (k_scale, v_scale, out) if t is not None)
-    device = _require_cuda(q, k_cache, v_cache, block_table, lengths, *given)
-    _float_type("q", q, (torch.float16, torch.bfloat16))
-    scale_slots = _cache_operands(k_cache, v_cache, k_scale, v_scale)
-    if k_cache.element_size() == 2:
-        _expect("k_cache", k_cache, q.dtype)
-    if q.dim() != 3 or block_table.dim() != 2:
-        raise ValueError("q is a (batch, heads, head_dim) tensor and block_table a (batch, columns) one")
-    if q.shape[2] != k_cache.shape[3]:
-        raise ValueError(f"q has head_dim {q.shape[2]}, the cache {k_cache.shape[3]}")
-    if k_cache.shape[1] < 1 or q.shape[1] < 1 or q.shape[1] % k_cache.shape[1]:
-        raise ValueError(f"{q.shape[1]} query heads are not a multiple of the cache's {k_cache.shape[1]}")
-    _expect("block_table", block_table, torch.int32, (q.shape[0], block_table.shape[1]))
-    _expect("lengths", lengths, torch.int32, (q.shape[0],))
-    if out is None:
-        out = torch.empty(q.shape, dtype=q.dtype, device=device)
-    _expect("out", out, q.dtype, q.shape)
-    lse = torch.empty(q.shape[:2], dtype=torch.float32, device=device) if return_lse else None
-    space = _status_workspace(device)
+    """Attention of one new token a sequence: ``q`` (batch, heads, head_dim) over the first ``lengths[b]`` rows of
+    each sequence in a paged cache (``cache_write``), whose pages row ``b`` of ``block_table`` (batch, columns)
+    names in order; both int32.  heads is a multiple of the cache's heads, neighbouring query heads share a key
+    head; head_dim is 64 or 128.  A sequence of length 0 gets zeros (and lse -infinity).  What lies behind a
+    sequence, in its last page or in the table, is never used.  A page outside the cache is left out, a length
+    past the table is cut there, and ``workspace_status`` reports both.  Returns ``out``, or ``(out, lse)``
+    with the natural logarithm of the sums (f32)."""
+    device = _cuda_device(q)
+    dtype = _float_type("q", q, (torch.float16, torch.bfloat16))
+    shape = _shape("q", q, 3, "(batch, heads, head_dim)")
+    cache, views, scales = _cache_slots(k_cache, v_cache, k_scale, v_scale, device)
+    if k_cache.dtype is not dtype and k_cache.element_size() == 2:
+        raise TypeError(f"k_cache must have dtype {dtype}, torch.int8 or torch.float8_e4m3fn, got {k_cache.dtype}")
+    batch, heads, columns = shape
+    if columns != cache[3]:
+        raise ValueError(f"q has head_dim {columns}, the cache {cache[3]}")
+    if cache[1] < 1 or heads < 1 or heads % cache[1]:
+        raise ValueError(f"{heads} query heads are not a multiple of the cache's {cache[1]}")
+    table = (batch, _shape("block_table", block_table, 2, "(batch, columns)")[1])
     store = _CODES[k_cache.dtype]
-    words = _scratch_size("b200_paged_attention_scratch", device, q.shape[0], q.shape[1], k_cache.shape[1], q.shape[2],
-                          block_table.shape[1] * k_cache.shape[2], store)
-    partial = torch.empty((words,), dtype=torch.float32, device=device)   # the call's own: calls may overlap
-    _call("b200_paged_attention", device, *_slots(q), *_slots(k_cache), *_slots(v_cache), *scale_slots, *_slots(block_table),
-          *_slots(lengths), *_slots(out), *(_slots(lse) if return_lse else [None] + [0] * 4), float(scale), *_slots(partial),
-          *_slots(space), _CODES[q.dtype], store, _stream(q))
+    if out is None:
+        out = q.new_empty(shape)
+    words = _scratch_size("b200_paged_attention_scratch", device, batch, heads, cache[1], columns, table[1] * cache[2], store)
+    partial = q.new_empty((words,), dtype=torch.float32)    # the call's own: calls may overlap
+    lse, lse_slots = None, (0,) * 5
+    if return_lse:
+        lse = q.new_empty((batch, heads), dtype=torch.float32)
+        lse_slots = (lse.data_ptr(), batch, heads, heads, 1)
+    _invoke("b200_paged_attention", device,
+            (*_bound("q", q, dtype, shape, device), *views, *scales,
+             *_bound("block_table", block_table, torch.int32, table, device),
+             *_bound("lengths", lengths, torch.int32, shape[:1], device), *_bound("out", out, dtype, shape, device), *lse_slots,
+             partial.data_ptr(), words, 1, *_status(device)),
+            float(scale), _CODES[dtype], store)
     return (out, lse) if return_lse else out
 
 

@@ -21,8 +21,9 @@ def view(*shape, address=BASE, strides=None):
 
 
 def call(name, *parts):
-    arguments = [x for part in parts for x in (part if isinstance(part, list) else [part])]
-    return _native.entry(name)(*arguments)
+    """The views among `parts` as one array of slots, then the rest."""
+    slots = [x or 0 for part in parts if isinstance(part, list) for x in part]
+    return _native.entry(name)((ctypes.c_int64 * len(slots))(*slots), len(slots), *(x for x in parts if not isinstance(x, list)))
 
 
 SPACE = view(64, address=BASE + (1 << 40))
@@ -172,6 +173,14 @@ def test_paged_attention_of_no_sequences_is_done():
     assert attend(q=view(0, 8, 64), out=view(0, 8, 64), table=view(0, 3), lengths=view(0)) == 0
 
 
+def test_a_wrong_number_of_slots_is_refused():
+    for name, tail in (("b200_head_norm_rotary", (1e-6, 0, 0)), ("b200_head_norm_rotary_backward", (1e-6, 0, 0)), ("b200_cache_write", (1, 1)),
+                       ("b200_cache_read", (1, 1)), ("b200_paged_attention", (1.0, 1, 1))):
+        words = (ctypes.c_int64 * 200)()
+        for address, count in ((words, 0), (words, 12), (words, 200), (None, 12), (None, 0)):
+            assert _native.entry(name)(address, count, *tail, None) == 1
+
+
 def test_scratch_entries_check_their_extents():
     words = ctypes.c_int64()
     size = _native.entry("b200_paged_attention_scratch")
@@ -189,9 +198,10 @@ def test_ops_check_before_any_call():
         ops.cache_write(k, k, torch.zeros(3, dtype=torch.int64), cache, cache)
     for wrong, message in (((cache, cache.half(), None, None), "v_cache must have dtype"),
                            ((cache, cache, None, None), "needs k_scale"), ((cache.half(), cache.half(), w, w), "has no scales"),
-                           ((cache.float(), cache.float(), None, None), "k_cache must be"), ((cache[0], cache[0], None, None), "a cache is")):
+                           ((cache.float(), cache.float(), None, None), "k_cache must be"), ((cache[0], cache[0], None, None), "k_cache is a"),
+                           ((cache, [1], None, None), "v_cache must be a torch.Tensor"), ((cache, cache[1:], w, w), "v_cache must have shape")):
         with pytest.raises((TypeError, ValueError), match=message):
-            ops._cache_operands(*wrong)
+            ops._cache_slots(*wrong, -1)
 
 
 # ------------------------------------------------------- the plain forms hold what they are held to

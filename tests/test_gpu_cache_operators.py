@@ -142,6 +142,18 @@ def test_rotary_edges():
     only_q = ops.head_norm_rotary_backward(k_out, k_out[:, :0], k, k[:, :0], qw, kw, cos, sin, positions)
     assert not only_q[3].any() and only_q[1].shape == (9, 0, 64)
     status_names(7)
+    # padding and heads that fill no whole unit add nothing even where a row of zeros has no norm
+    many = [randn(3000, n, 64, seed=n) for n in (5, 3, 5, 3)]
+    places = torch.arange(3000, device=DEV, dtype=torch.int32) % 64
+    places[::7] = -1
+    for t in many:
+        t[::7] = 0
+    grads = ops.head_norm_rotary_backward(*many, qw, kw, cos, sin, places, 0.0)
+    for i in range(2):
+        dx, dx_slack, dw, dw_slack = plain.norm_rotary_backward(many[i], torch.where(places[:, None, None] < 0, 1.0, many[2 + i]),
+                                                                (qw, kw)[i], cos, sin, places, 0.0, False)
+        plain.close(grads[i], dx, dx_slack)
+        plain.close(grads[2 + i], dw, dw_slack)
     with pytest.raises(TypeError):
         ops.head_norm_rotary(q, k, qw, kw, cos, sin, positions.long())
     with pytest.raises(NotImplementedError):

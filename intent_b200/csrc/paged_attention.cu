@@ -7,24 +7,24 @@
 // heads that share it.  What the kernel has to do is keep copies in flight on every SM, whatever
 // the lengths are.
 //
-// Work.  The unit is a step: WARPS * KEYS key positions of one (sequence, key head, row tile).  All
+// Work.  The unit is a step: WARPS * KEYS key positions of one (sequence, key head, tile of query heads).  All
 // steps of the call, sequence after sequence, are cut into as many equal runs as there are resident
-// blocks; a block finds its run by a scan of the lengths and crosses from one sequence to the next
+// blocks (of several heads abreast, see heads_abreast); a block finds its run by a scan of the lengths and crosses from one sequence to the next
 // without draining its copies.  A ragged batch therefore loads all SMs alike, a single long
 // sequence is spread over all of them, and a short one is not cut without need.  A piece
 // that is a whole (sequence, head) is finished in place; others leave their unnormalised sums and the
 // maxima they are relative to in `partial`, which a second kernel joins in the order of the blocks
-// (no atomics: results do not vary).  That kernel is placed while the first one runs and does its own
-// scan meanwhile.
+// (no atomics: results do not vary).  Only the borders between runs cut heads, so that kernel has a
+// block for each border and row, which the run's own note tells what it cuts.
 //
 // Inside a block every warp is on its own: it copies KEYS rows of K and V with cp.async into its own
 // ring in shared memory (16 bytes a lane, rows past the end zero-filled, so that nothing that an
-// unwritten slot holds reaches a product), and multiplies with mma.sync m16n8k16: the 16 rows are
-// query heads, which is why tcgen05 with its 64 or 128 rows is not used: the products are a
-// sixteenth of what those tiles would pad them to, and the copies, not the products, are the
-// time.  Up to 8 query heads fill half of the rows; the other half of the second product's
-// rows then carry what rounding P to 16 bits has dropped, so P enters with 22 (f16) or 16 (bf16) bits
-// and only the result is rounded.  For 9 and more heads that takes a second product.
+// unwritten slot holds reaches a product), and multiplies with mma.sync m16n8k16.  Keys (and in the second
+// product columns of V) are the 16 rows and query heads the 8 columns, so the group sizes of real
+// models fill the products without padding; tcgen05's smallest tiles would pad them 2 to 16 times and
+// take the weights through shared memory, to speed up what is not the time.  The weights enter the
+// second product as the sum of two halves of 16 bits, so that they count with 22 (f16) or 16 (bf16) bits
+// and only the result is rounded.
 //
 // 8-bit rows.  Codes become f16 exactly on their way into the products.  The query is scaled by a
 // power of two per row to fit f16; a key's scale multiplies its score.  A value's scale is folded into
@@ -45,8 +45,7 @@ using heads::View4;
 
 constexpr int kWarps = 4;
 constexpr int kBlock = kWarps * 32;
-constexpr int kBlocksPerSm = 2;
-constexpr int kJoinThreads = 256;
+constexpr int kJoinThreads = 256, kJoinRows = 2;
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 
 struct Problem {
@@ -65,28 +64,37 @@ struct Problem {
   float *lse;
   int64_t lse_batch, lse_head;
   float *partial;
-  int batch, kv_heads, group, row_tiles, page_size, pages, runs;
+  int batch, kv_heads, group, row_tiles, page_size, pages;
+  int runs, abreast;                             // blocks = runs * abreast
   int64_t most_keys;                             // slots that a row of the table names
   float scale_log2e;
   int *status;
 };
 
-template <int STORE, int D> struct Shape {
+template <int STORE, int D, int ROWS> struct Shape {
   static constexpr int kBytes = STORE == cache::kNative ? 2 : 1;
   static constexpr int kKeys = STORE == cache::kNative ? 16 : 32;   // key positions of a warp's tile
   static constexpr int kStep = kWarps * kKeys;
   static constexpr int kRowBytes = D * kBytes;
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kTileBytes = kKeys * kRowBytes;
-  static constexpr int kStages = D == 128 ? 3 : 4;                  // 64 KB of copies in flight on an SM, or more
+  static constexpr int kBlocksPerSm = ROWS == 8 ? 3 : 2;            // 168 or 255 registers
+  static constexpr int kStages = (ROWS == 8 ? 2 : 3) * (128 / D);   // about 200 KB of an SM's shared memory
   static constexpr int kScaleBytes = STORE == cache::kNative ? 0 : 2 * kKeys * 4;
   static constexpr int kStageBytes = 2 * kTileBytes + kScaleBytes;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
+  static constexpr int kSmemBytes = kRingBytes + kWarps * ROWS * 3 * 4;
+  static_assert(ROWS * D * 4 <= kStageBytes, "a warp's sums fit the stage that it has just used");
 };
-template <int STORE, int D, int ROWS> constexpr int smem_bytes() {
-  return Shape<STORE, D>::kRingBytes + ROWS * D * 4 + kWarps * ROWS * 3 * 4;
-}
 constexpr int partial_floats(int columns) { return columns + 4; }   // sums, m, l, M, unused
+
+// What a run begins with, for the kernel that joins: (sequence, head tile) and how many of its steps lie
+// before the run.
+struct Border {
+  int64_t total;
+  int b, head, step, steps;
+};
+static_assert(sizeof(Border) == 24, "six words");
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -95,9 +103,17 @@ __device__ __forceinline__ float exp2_fast(float x) {
 }
 __device__ __forceinline__ float finite_or_zero(float m) { return m == -INFINITY ? 0.0f : m; }
 
+__device__ __forceinline__ uint32_t transposed(uint32_t pair) {
+  uint32_t r;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(pair));
+  return r;
+}
 __device__ __forceinline__ uint32_t shared_address(const void *p) { return (uint32_t)__cvta_generic_to_shared(p); }
 __device__ __forceinline__ void copy16(uint32_t to, const void *from, bool live) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(live ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void copy16(uint32_t to, const void *from) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(to), "l"(from) : "memory");
 }
 __device__ __forceinline__ void copy4(uint32_t to, const void *from, bool live) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(live ? 4 : 0) : "memory");
@@ -117,10 +133,10 @@ __device__ __forceinline__ void load_matrix_transposed(uint32_t (&r)[4], uint32_
 template <typename M>
 __device__ __forceinline__ void multiply(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
   if constexpr (sizeof(M) == 2 && !std::is_same<M, __nv_bfloat16>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3]) : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 template <typename M> __device__ __forceinline__ uint32_t pack(float low, float high) {
@@ -132,15 +148,24 @@ template <typename M> __device__ __forceinline__ float unpack(uint32_t pair, int
   return Element<M>::widen(*reinterpret_cast<const M *>(&bits));
 }
 
-// Two 8-bit codes of `word`, at bytes I and J, as f16 (exact).
-template <int STORE, int I, int J> __device__ __forceinline__ uint32_t codes(uint32_t word) {
+// The four 8-bit codes of a word as f16 (exact): bytes 0, 1 and 2, 3, or with EVEN_ODD bytes 0, 2 and 1, 3.
+template <int STORE, bool EVEN_ODD> __device__ __forceinline__ void widen(uint32_t word, uint32_t &first, uint32_t &second) {
   if constexpr (STORE == cache::kInt8) {
     // 0x6400 + u is 1024 + u in f16; u = code + 128 (the sign bit flipped)
-    const uint32_t biased = __byte_perm(word ^ 0x80808080u, 0x64646464u, I | 4 << 4 | J << 8 | 4 << 12);
-    const __half2 less = __hsub2(*reinterpret_cast<const __half2 *>(&biased), __half2half2(__ushort_as_half(0x6480)));
-    return *reinterpret_cast<const uint32_t *>(&less);
+    const uint32_t biased = word ^ 0x80808080u;
+    const __half2 bias = __half2half2(__ushort_as_half(0x6480));
+    const uint32_t low = __byte_perm(biased, 0x64646464u, EVEN_ODD ? 0x4240 : 0x4140);
+    const uint32_t high = __byte_perm(biased, 0x64646464u, EVEN_ODD ? 0x4341 : 0x4342);
+    const __half2 a = __hsub2(*reinterpret_cast<const __half2 *>(&low), bias), b = __hsub2(*reinterpret_cast<const __half2 *>(&high), bias);
+    first = *reinterpret_cast<const uint32_t *>(&a);
+    second = *reinterpret_cast<const uint32_t *>(&b);
   } else {
-    return cache::f16x2_of_e4m3(__byte_perm(word, 0, I | J << 4));
+    const uint32_t ordered = EVEN_ODD ? __byte_perm(word, 0, 0x3120) : word;
+    asm("{\n\t.reg .b16 low, high;\n\t"
+        "mov.b32 {low, high}, %2;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %0, low;\n\t"
+        "cvt.rn.f16x2.e4m3x2 %1, high;\n\t}"
+        : "=r"(first), "=r"(second) : "r"(ordered));
   }
 }
 
@@ -183,8 +208,9 @@ struct Place {            // where in the sequence of steps a warp is
     --left;
     if (++step < steps) return;
     step = 0;
-    if (++head < p.kv_heads * p.row_tiles) return;
-    head = 0;
+    head += p.abreast;
+    if (head < p.kv_heads * p.row_tiles) return;
+    head = head % p.abreast;
     if (left <= 0) return;
     do {
       if (++b >= p.batch) {   // only if the lengths change under the kernel
@@ -198,12 +224,12 @@ struct Place {            // where in the sequence of steps a warp is
 };
 
 template <typename T, int STORE, int D, int ROWS>
-__global__ void __launch_bounds__(kBlock, kBlocksPerSm)
+__global__ void __launch_bounds__(kBlock, (Shape<STORE, D, ROWS>::kBlocksPerSm))
 paged_attention_kernel(const Problem p) {
-  using S = Shape<STORE, D>;
+  using S = Shape<STORE, D, ROWS>;
   using M = typename std::conditional<STORE == cache::kNative, T, __half>::type;   // type of the products
   constexpr bool kCodes = STORE != cache::kNative;
-  constexpr int kHalves = ROWS / 8, kTiles = S::kKeys / 8;
+  constexpr int kHeads = ROWS / 8, kTiles = S::kKeys / 16;   // tiles of 8 query heads and of 16 keys
   extern __shared__ __align__(128) unsigned char dynamic_smem[];
   __shared__ int64_t scan_scratch[kWarps];
   __shared__ int64_t start_rest;
@@ -212,31 +238,50 @@ paged_attention_kernel(const Problem p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
 
-  // ---- this block's run of steps
-  const int head_tiles = p.kv_heads * p.row_tiles;
-  int64_t total = 0, before = 0;
+  // ---- this block's run of steps, which it goes through for one of every `abreast` heads
+  const int head_tiles = p.kv_heads * p.row_tiles / p.abreast;
+  const int run = blockIdx.x / p.abreast, lane_head = blockIdx.x - run * p.abreast;
+  int64_t total = 0, before = 0, steps_here = 0;
   for (int base = 0; base < p.batch; base += kBlock) {
     const int b = base + threadIdx.x;
-    const int length = b < p.batch ? length_of(p, b) : 0;
-    if (blockIdx.x == 0 && b < p.batch && p.lengths[b * p.lengths_step] > p.most_keys) heads::report_index(p.status, b);
-    total += block_scan<kBlock>((length + S::kStep - 1) / S::kStep, before, scan_scratch);
+    const int given = b < p.batch ? p.lengths[b * p.lengths_step] : 0;
+    const int length = given <= 0 ? 0 : (int)min((int64_t)given, p.most_keys);
+    if (blockIdx.x == 0 && given > p.most_keys) heads::report_index(p.status, b);
+    steps_here = (length + S::kStep - 1) / S::kStep;
+    total += block_scan<kBlock>(steps_here, before, scan_scratch);
   }
   total *= head_tiles;
   const int64_t runs = min((int64_t)p.runs, total);   // none is empty, which the join relies on
-  if (blockIdx.x >= runs) return;
-  const int64_t begin = total * blockIdx.x / runs, end = total * (blockIdx.x + 1) / runs;
+  Border *border = reinterpret_cast<Border *>(p.partial + (int64_t)gridDim.x * 2 * ROWS * partial_floats(D)) + blockIdx.x;
+  // sequences that have not begun
+  for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
+    if (p.lengths[b * p.lengths_step] > 0 && p.most_keys > 0) continue;
+    T *out = static_cast<T *>(p.out) + b * p.out_batch;
+    for (int index = threadIdx.x; index < p.kv_heads * p.group * D; index += kBlock)
+      out[(index / D) * p.out_head + index % D] = Element<T>::narrow(0.0f);
+    for (int head = threadIdx.x; p.lse && head < p.kv_heads * p.group; head += kBlock)
+      p.lse[b * p.lse_batch + head * p.lse_head] = -INFINITY;
+  }
+  if (run >= runs) {
+    if (threadIdx.x == 0) border->step = 0;
+    return;
+  }
+  const int64_t begin = total * run / runs, end = total * (run + 1) / runs;
   int64_t carried = 0;
   for (int base = 0; base < p.batch; base += kBlock) {
     const int b = base + threadIdx.x;
-    const int64_t steps = b < p.batch ? (length_of(p, b) + S::kStep - 1) / S::kStep : 0;
-    const int64_t sum = block_scan<kBlock>(steps, before, scan_scratch);
-    const int64_t first = (carried + before) * head_tiles;
-    if (begin >= first && begin < first + steps * head_tiles) {
+    int64_t sum = total;
+    if (p.batch > kBlock) {   // else the scan above stands
+      steps_here = b < p.batch ? (length_of(p, b) + S::kStep - 1) / S::kStep : 0;
+      sum = block_scan<kBlock>(steps_here, before, scan_scratch) * head_tiles;
+    }
+    const int64_t first = carried + before * head_tiles;
+    if (begin >= first && begin < first + steps_here * head_tiles) {
       start_b = b;
       start_rest = begin - first;
     }
     carried += sum;
-    if (carried * head_tiles > begin) break;
+    if (carried > begin) break;
   }
   __syncthreads();
   Place load;             // where the next copies are from
@@ -245,14 +290,15 @@ paged_attention_kernel(const Problem p) {
   load.steps = (load.length + S::kStep - 1) / S::kStep;
   load.head = (int)(start_rest / load.steps);
   load.step = (int)(start_rest - (int64_t)load.head * load.steps);
+  load.head = load.head * p.abreast + lane_head;
   load.left = end - begin;
   Place use = load;       // what the next products take
+  if (threadIdx.x == 0) *border = Border{total, load.b, load.head, load.step, load.steps};
 
   // ---- copies: lane r looks row r of the tile up; a row's 16-byte pieces go to neighbouring lanes
   unsigned char *ring = dynamic_smem + warp * S::kStages * S::kStageBytes;
   const uint32_t ring_address = shared_address(ring);
-  float *merged = reinterpret_cast<float *>(dynamic_smem + S::kRingBytes);
-  float *stats = merged + ROWS * D;
+  float *stats = reinterpret_cast<float *>(dynamic_smem + S::kRingBytes);
   int entry = -1, offset = 0;
   bool inside = false;
   auto look_up = [&]() {
@@ -267,6 +313,11 @@ paged_attention_kernel(const Problem p) {
     }
   };
   const bool one_layout = p.k_page == p.v_page && p.k_head == p.v_head && p.k_slot == p.v_slot;
+  const bool whole_pages = p.page_size % 16 == 0;
+  constexpr int kRowsAtOnce = 32 / S::kChunks;
+  constexpr uint32_t kFull = S::kKeys == 32 ? 0xffffffffu : (1u << S::kKeys % 32) - 1;
+  const int chunk = lane % S::kChunks;
+  const int64_t k_lane = (lane / S::kChunks) * p.k_slot + chunk * 16, v_lane = (lane / S::kChunks) * p.v_slot + chunk * 16;
   uint32_t masks[S::kStages - 1];     // which rows of the tiles in flight are there, oldest first
   auto issue = [&](int stage) -> uint32_t {
     bool live = inside;
@@ -276,22 +327,36 @@ paged_attention_kernel(const Problem p) {
     }
     const uint32_t mask = __ballot_sync(0xffffffffu, live);
     if (mask == 0) return 0;
-    const int kv_head = load.head / p.row_tiles;
+    const int kv_head = p.row_tiles == 1 ? load.head : load.head / p.row_tiles;
     const int64_t page = live ? entry : 0;
     const int64_t k_row = page * p.k_page + kv_head * p.k_head + (live ? offset : 0) * p.k_slot;
-    const int64_t v_row = page * p.v_page + kv_head * p.v_head + (live ? offset : 0) * p.v_slot;
+    const int64_t v_row = one_layout ? k_row : page * p.v_page + kv_head * p.v_head + (live ? offset : 0) * p.v_slot;
     const uint32_t stage_address = ring_address + stage * S::kStageBytes;
-    constexpr int kRowsAtOnce = 32 / S::kChunks;
-    const int chunk = lane % S::kChunks;
+    if (whole_pages && mask == kFull) {
+      // 16 rows at a time lie one slot apart: one exchange for them
 #pragma unroll
-    for (int i = 0; i < S::kKeys / kRowsAtOnce; ++i) {
-      const int row = i * kRowsAtOnce + lane / S::kChunks;
-      const bool row_live = mask >> row & 1;
-      const int64_t from = __shfl_sync(0xffffffffu, k_row, row);
-      const uint32_t to = stage_address + row * S::kRowBytes + swizzled<S::kChunks>(row, chunk) * 16;
-      copy16(to, p.k + from + chunk * 16, row_live);
-      const int64_t v_from = one_layout ? from : __shfl_sync(0xffffffffu, v_row, row);
-      copy16(to + S::kTileBytes, p.v + v_from + chunk * 16, row_live);
+      for (int t = 0; t < S::kKeys / 16; ++t) {
+        const uint8_t *k = p.k + __shfl_sync(0xffffffffu, k_row, 16 * t) + k_lane;
+        const uint8_t *v = p.v + __shfl_sync(0xffffffffu, v_row, 16 * t) + v_lane;
+#pragma unroll
+        for (int i = 0; i < 16 / kRowsAtOnce; ++i) {
+          const int row = 16 * t + i * kRowsAtOnce + lane / S::kChunks;
+          const uint32_t to = stage_address + row * S::kRowBytes + swizzled<S::kChunks>(row, chunk) * 16;
+          copy16(to, k);
+          copy16(to + S::kTileBytes, v);
+          k += kRowsAtOnce * p.k_slot;
+          v += kRowsAtOnce * p.v_slot;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < S::kKeys / kRowsAtOnce; ++i) {
+        const int row = i * kRowsAtOnce + lane / S::kChunks;
+        const bool row_live = mask >> row & 1;
+        const uint32_t to = stage_address + row * S::kRowBytes + swizzled<S::kChunks>(row, chunk) * 16;
+        copy16(to, p.k + __shfl_sync(0xffffffffu, k_row, row) + chunk * 16, row_live);
+        copy16(to + S::kTileBytes, p.v + __shfl_sync(0xffffffffu, v_row, row) + chunk * 16, row_live);
+      }
     }
     if constexpr (kCodes) {
       const uint32_t to = stage_address + 2 * S::kTileBytes + lane * 4;
@@ -311,33 +376,40 @@ paged_attention_kernel(const Problem p) {
     return mask;
   };
 
-  // ---- the query rows of the current head, as the products' left operand
-  uint32_t query[D / 16][2 * kHalves];
-  float row_scale[kHalves];
-  auto load_query = [&]() {
-    const int kv_head = use.head / p.row_tiles, row0 = (use.head - kv_head * p.row_tiles) * ROWS;
+  // ---- the query heads of the current tile, as the first product's right operand: thread (g, c) holds
+  // head g's columns 16 i + 2 c, + 1 and 16 i + 8 + 2 c, + 1 (of codes: 16 i + 4 c .. + 3)
+  uint2 query[D / 16][kHeads];
+  float head_scale[kHeads][2];        // of heads 2 c, 2 c + 1, whose scores the thread will hold
+  auto fetch_query = [&](const Place &at) {
+    const int kv_head = at.head / p.row_tiles, row0 = (at.head - kv_head * p.row_tiles) * ROWS;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
+    for (int h = 0; h < kHeads; ++h) {
       const int row = row0 + h * 8 + g;
-      const T *source = static_cast<const T *>(p.q) + use.b * p.q_batch + (kv_head * p.group + min(row, p.group - 1)) * p.q_head;
-      const bool live = row < p.group;
-      if constexpr (!kCodes) {
-        row_scale[h] = p.scale_log2e;
+      const T *source = static_cast<const T *>(p.q) + at.b * p.q_batch + (kv_head * p.group + min(row, p.group - 1)) * p.q_head;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {   // columns 16 i + 2 c, + 1 and 16 i + 8 + 2 c, + 1
-          query[i][h] = live ? *reinterpret_cast<const uint32_t *>(source + 16 * i + 2 * c) : 0u;
-          query[i][kHalves + h] = live ? *reinterpret_cast<const uint32_t *>(source + 16 * i + 8 + 2 * c) : 0u;
+      for (int i = 0; i < D / 16; ++i) {
+        query[i][h] = make_uint2(0, 0);
+        if (row >= p.group) continue;
+        if constexpr (kCodes) {
+          query[i][h] = *reinterpret_cast<const uint2 *>(source + 16 * i + 4 * c);
+        } else {
+          query[i][h].x = *reinterpret_cast<const uint32_t *>(source + 16 * i + 2 * c);
+          query[i][h].y = *reinterpret_cast<const uint32_t *>(source + 16 * i + 8 + 2 * c);
         }
-      } else {
-        uint2 raw[D / 16];
+      }
+    }
+  };
+  auto scale_query = [&]() {
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      head_scale[h][0] = head_scale[h][1] = p.scale_log2e;
+      if constexpr (kCodes) {
         float most = 0.0f;
 #pragma unroll
-        for (int i = 0; i < D / 16; ++i) {   // columns 16 i + 4 c .. + 3
-          raw[i] = live ? *reinterpret_cast<const uint2 *>(source + 16 * i + 4 * c) : make_uint2(0, 0);
+        for (int i = 0; i < D / 16; ++i)
 #pragma unroll
           for (int j = 0; j < 2; ++j)
-            most = fmaxf(most, fmaxf(fabsf(unpack<T>(raw[i].x, j)), fabsf(unpack<T>(raw[i].y, j))));
-        }
+            most = fmaxf(most, fmaxf(fabsf(unpack<T>(query[i][h].x, j)), fabsf(unpack<T>(query[i][h].y, j))));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 1));
         most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, 2));
         // the power of two that brings the row's largest entry into [16, 32): f16 then holds all of a bf16's
@@ -346,265 +418,250 @@ paged_attention_kernel(const Problem p) {
         const bool scaled = most > 0.0f && most < INFINITY;
         const int shift = scaled ? min(4 - exponent, 120) : 0;
         const float up = __uint_as_float((uint32_t)(127 + shift) << 23);
-        row_scale[h] = p.scale_log2e * __uint_as_float((uint32_t)(127 - shift) << 23);
+        const float down = p.scale_log2e * __uint_as_float((uint32_t)(127 - shift) << 23);
+        head_scale[h][0] = __shfl_sync(0xffffffffu, down, 8 * c);
+        head_scale[h][1] = __shfl_sync(0xffffffffu, down, 8 * c + 4);
 #pragma unroll
         for (int i = 0; i < D / 16; ++i) {
-          query[i][h] = pack<__half>(unpack<T>(raw[i].x, 0) * up, unpack<T>(raw[i].x, 1) * up);
-          query[i][kHalves + h] = pack<__half>(unpack<T>(raw[i].y, 0) * up, unpack<T>(raw[i].y, 1) * up);
+          const uint2 raw = query[i][h];
+          query[i][h] = make_uint2(pack<__half>(unpack<T>(raw.x, 0) * up, unpack<T>(raw.x, 1) * up),
+                                   pack<__half>(unpack<T>(raw.y, 0) * up, unpack<T>(raw.y, 1) * up));
         }
       }
     }
   };
 
-  // ---- running state of a piece
-  float sums[D / 8][4], m[kHalves], l[kHalves], weight_max[kHalves];
+  // ---- running state of a piece; sums: columns (of V) x heads
+  float sums[D / 16][kHeads][4], m[kHeads][2], l[kHeads][2], weight_max[kHeads][2];
   int piece_first = use.step;
   auto reset = [&]() {
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i)
+    for (int h = 0; h < kHeads; ++h) {
 #pragma unroll
-      for (int j = 0; j < 4; ++j) sums[i][j] = 0.0f;
+      for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) { m[h] = weight_max[h] = -INFINITY; l[h] = 0.0f; }
+        for (int j = 0; j < 4; ++j) sums[i][h][j] = 0.0f;
+#pragma unroll
+      for (int j = 0; j < 2; ++j) { m[h][j] = weight_max[h][j] = -INFINITY; l[h][j] = 0.0f; }
+    }
     piece_first = use.step;
   };
 
   auto consume = [&](int stage, uint32_t mask) {
     const uint32_t k_address = ring_address + stage * S::kStageBytes, v_address = k_address + S::kTileBytes;
-    const float *k_scales = reinterpret_cast<const float *>(ring + stage * S::kStageBytes + 2 * S::kTileBytes);
-    float s[kTiles][4];
+    const float *scales = reinterpret_cast<const float *>(ring + stage * S::kStageBytes + 2 * S::kTileBytes);
+    float s[kTiles][kHeads][4];       // scores: keys 16 t + g and + 8, heads 2 c and 2 c + 1
 #pragma unroll
     for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[t][j] = 0.0f;
-    const int low_row = lane & 7;
-    // scores: four chunks of eight keys at a time
+      for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-    for (int i = 0; i < S::kChunks / 4; ++i) {
+        for (int j = 0; j < 4; ++j) s[t][h][j] = 0.0f;
+#pragma unroll
+    for (int i = 0; i < S::kChunks / 2; ++i) {
 #pragma unroll
       for (int t = 0; t < kTiles; ++t) {
-        uint32_t r[4];
-        const int row = 8 * t + low_row;
-        load_matrix(r, k_address + row * S::kRowBytes + swizzled<S::kChunks>(row, 4 * i + (lane >> 3)) * 16);
+        uint32_t r[4];                // two chunks of keys 16 t .. + 7 and + 8 .. + 15
+        const int row = 16 * t + (lane & 15);
+        load_matrix(r, k_address + row * S::kRowBytes + swizzled<S::kChunks>(row, 2 * i + (lane >> 4)) * 16);
         if constexpr (!kCodes) {
 #pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const uint32_t *a = query[2 * i + j];
-            multiply<M>(s[t], a[0], kHalves == 2 ? a[1] : 0u, a[kHalves], kHalves == 2 ? a[3] : 0u, r[2 * j], r[2 * j + 1]);
-          }
+          for (int h = 0; h < kHeads; ++h) multiply<M>(s[t][h], r[0], r[1], r[2], r[3], query[i][h].x, query[i][h].y);
         } else {
 #pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const uint32_t *a = query[4 * i + j];
-            multiply<M>(s[t], a[0], kHalves == 2 ? a[1] : 0u, a[kHalves], kHalves == 2 ? a[3] : 0u,
-                        codes<STORE, 0, 1>(r[j]), codes<STORE, 2, 3>(r[j]));
+          for (int j = 0; j < 2; ++j) {
+            uint32_t a0, a1, a2, a3;
+            widen<STORE, false>(r[2 * j], a0, a2);
+            widen<STORE, false>(r[2 * j + 1], a1, a3);
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h) multiply<M>(s[t][h], a0, a1, a2, a3, query[2 * i + j][h].x, query[2 * i + j][h].y);
           }
         }
       }
     }
-    // weights: thread (g, c) holds keys 8 t + 2 c, + 1 of rows g and, with 16 rows, g + 8
     float log_scale[kTiles][2];
 #pragma unroll
-    for (int t = 0; t < kTiles; ++t) {
-      const uint32_t bits = mask >> (8 * t + 2 * c);
-      float2 ks = make_float2(1.0f, 1.0f);
-      if constexpr (kCodes) {
-        ks = *reinterpret_cast<const float2 *>(k_scales + 8 * t + 2 * c);
-        const float2 vs = *reinterpret_cast<const float2 *>(k_scales + S::kKeys + 8 * t + 2 * c);
-        log_scale[t][0] = __log2f(vs.x);
-        log_scale[t][1] = __log2f(vs.y);
-      }
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        s[t][2 * h] = bits & 1 ? s[t][2 * h] * (row_scale[h] * ks.x) : -INFINITY;
-        s[t][2 * h + 1] = bits & 2 ? s[t][2 * h + 1] * (row_scale[h] * ks.y) : -INFINITY;
+      for (int k = 0; k < 2; ++k) {
+        const int key = 16 * t + 8 * k + g;
+        const bool live = mask >> key & 1;
+        float key_scale = 1.0f;
+        if constexpr (kCodes) {
+          key_scale = scales[key];
+          log_scale[t][k] = __log2f(scales[S::kKeys + key]);
+        }
+#pragma unroll
+        for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) s[t][h][2 * k + j] = live ? s[t][h][2 * k + j] * (head_scale[h][j] * key_scale) : -INFINITY;
       }
-    }
-    float new_m[kHalves], new_max[kHalves];
+    // The bases m and weight_max move only when a score passes them by more than 8 (log2 units): until then
+    // weights reach 2^8, well inside every type here.
     bool grown = false;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      new_m[h] = m[h];
+    for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-      for (int t = 0; t < kTiles; ++t) new_m[h] = fmaxf(new_m[h], fmaxf(s[t][2 * h], s[t][2 * h + 1]));
-      new_m[h] = fmaxf(new_m[h], __shfl_xor_sync(0xffffffffu, new_m[h], 1));
-      new_m[h] = fmaxf(new_m[h], __shfl_xor_sync(0xffffffffu, new_m[h], 2));
-      new_max[h] = new_m[h];
-      if constexpr (kCodes) {
-        new_max[h] = weight_max[h];
+      for (int j = 0; j < 2; ++j)
 #pragma unroll
-        for (int t = 0; t < kTiles; ++t)
-          new_max[h] = fmaxf(new_max[h], fmaxf(s[t][2 * h] + log_scale[t][0], s[t][2 * h + 1] + log_scale[t][1]));
-        new_max[h] = fmaxf(new_max[h], __shfl_xor_sync(0xffffffffu, new_max[h], 1));
-        new_max[h] = fmaxf(new_max[h], __shfl_xor_sync(0xffffffffu, new_max[h], 2));
-      }
-      grown |= new_m[h] > m[h] || new_max[h] > weight_max[h];
-    }
+        for (int t = 0; t < kTiles; ++t) {
+          grown |= fmaxf(s[t][h][j], s[t][h][2 + j]) > m[h][j] + 8.0f;
+          if constexpr (kCodes) grown |= fmaxf(s[t][h][j] + log_scale[t][0], s[t][h][2 + j] + log_scale[t][1]) > weight_max[h][j] + 8.0f;
+        }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
-      for (int h = 0; h < kHalves; ++h) {
-        l[h] *= exp2_fast(m[h] - finite_or_zero(new_m[h]));
-        const float shrink = exp2_fast(weight_max[h] - finite_or_zero(new_max[h]));
-#pragma unroll
-        for (int i = 0; i < D / 8; ++i) {
-          sums[i][2 * h] *= shrink;
-          sums[i][2 * h + 1] *= shrink;
-          if (kHalves == 1) {   // the other half of the rows belongs to the same heads
-            sums[i][2] *= shrink;
-            sums[i][3] *= shrink;
-          }
-        }
-        m[h] = new_m[h];
-        weight_max[h] = new_max[h];
-      }
-    }
-    uint32_t high[kTiles][kHalves], rest[kTiles][kHalves];
-#pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      const float base = finite_or_zero(m[h]), weight_base = finite_or_zero(weight_max[h]);
-#pragma unroll
-      for (int t = 0; t < kTiles; ++t) {
-        float w0 = exp2_fast(s[t][2 * h] - base), w1 = exp2_fast(s[t][2 * h + 1] - base);
-        l[h] += w0 + w1;
-        if constexpr (kCodes) {   // log2 of a masked key's zero scale is -infinity: its weight is 0
-          w0 = exp2_fast(s[t][2 * h] + log_scale[t][0] - weight_base);
-          w1 = exp2_fast(s[t][2 * h + 1] + log_scale[t][1] - weight_base);
-        }
-        high[t][h] = pack<M>(w0, w1);
-        rest[t][h] = pack<M>(w0 - unpack<M>(high[t][h], 0), w1 - unpack<M>(high[t][h], 1));
-      }
-    }
-    // sums += weights . values: two chunks of sixteen keys at a time
-#pragma unroll
-    for (int b = 0; b < S::kKeys / 16; ++b) {
-#pragma unroll
-      for (int i = 0; i < S::kChunks / 2; ++i) {
-        uint32_t r[4];
-        const int row = 16 * b + low_row + (lane & 8);
-        load_matrix_transposed(r, v_address + row * S::kRowBytes + swizzled<S::kChunks>(row, 2 * i + (lane >> 4)) * 16);
-        const uint32_t *h0 = high[2 * b], *h1 = high[2 * b + 1], *r0 = rest[2 * b], *r1 = rest[2 * b + 1];
+      for (int h = 0; h < kHeads; ++h) {
+        float shrink[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          if constexpr (!kCodes) {
-            float(&to)[4] = sums[2 * i + j];
-            if constexpr (kHalves == 1) {
-              multiply<M>(to, h0[0], r0[0], h1[0], r1[0], r[2 * j], r[2 * j + 1]);
-            } else {
-              multiply<M>(to, h0[0], h0[1], h1[0], h1[1], r[2 * j], r[2 * j + 1]);
-              multiply<M>(to, r0[0], r0[1], r1[0], r1[1], r[2 * j], r[2 * j + 1]);
-            }
-          } else {   // a 16-bit unit holds two neighbouring columns: even and odd ones make a tile each
-            const uint32_t even0 = codes<STORE, 0, 2>(r[2 * j]), even1 = codes<STORE, 0, 2>(r[2 * j + 1]);
-            const uint32_t odd0 = codes<STORE, 1, 3>(r[2 * j]), odd1 = codes<STORE, 1, 3>(r[2 * j + 1]);
-            float(&to_even)[4] = sums[2 * (2 * i + j)];
-            float(&to_odd)[4] = sums[2 * (2 * i + j) + 1];
-            if constexpr (kHalves == 1) {
-              multiply<M>(to_even, h0[0], r0[0], h1[0], r1[0], even0, even1);
-              multiply<M>(to_odd, h0[0], r0[0], h1[0], r1[0], odd0, odd1);
-            } else {
-              multiply<M>(to_even, h0[0], h0[1], h1[0], h1[1], even0, even1);
-              multiply<M>(to_odd, h0[0], h0[1], h1[0], h1[1], odd0, odd1);
-              multiply<M>(to_even, r0[0], r0[1], r1[0], r1[1], even0, even1);
-              multiply<M>(to_odd, r0[0], r0[1], r1[0], r1[1], odd0, odd1);
-            }
+          float top = m[h][j], weight_top = weight_max[h][j];
+#pragma unroll
+          for (int t = 0; t < kTiles; ++t) {
+            top = fmaxf(top, fmaxf(s[t][h][j], s[t][h][2 + j]));
+            if constexpr (kCodes) weight_top = fmaxf(weight_top, fmaxf(s[t][h][j] + log_scale[t][0], s[t][h][2 + j] + log_scale[t][1]));
           }
+#pragma unroll
+          for (int other = 4; other < 32; other <<= 1) {
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, other));
+            if constexpr (kCodes) weight_top = fmaxf(weight_top, __shfl_xor_sync(0xffffffffu, weight_top, other));
+          }
+          if constexpr (!kCodes) weight_top = top;
+          l[h][j] *= exp2_fast(m[h][j] - finite_or_zero(top));
+          shrink[j] = exp2_fast(weight_max[h][j] - finite_or_zero(weight_top));
+          m[h][j] = top;
+          weight_max[h][j] = weight_top;
+        }
+#pragma unroll
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) sums[i][h][j] *= shrink[j & 1];
+      }
+    }
+    uint32_t high[kTiles][kHeads][2], rest[kTiles][kHeads][2];   // head g, keys 16 t + 2 c, + 1 and + 8, + 9
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h) {
+      const float base[2] = {finite_or_zero(m[h][0]), finite_or_zero(m[h][1])};
+      const float weight_base[2] = {finite_or_zero(weight_max[h][0]), finite_or_zero(weight_max[h][1])};
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          float w[2];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            w[j] = exp2_fast(s[t][h][2 * k + j] - base[j]);
+            l[h][j] += w[j];
+            // log2 of a masked key's zero scale is -infinity: its weight is 0
+            if constexpr (kCodes) w[j] = exp2_fast(s[t][h][2 * k + j] + log_scale[t][k] - weight_base[j]);
+          }
+          const uint32_t pair = pack<M>(w[0], w[1]);
+          high[t][h][k] = transposed(pair);
+          rest[t][h][k] = transposed(pack<M>(w[0] - unpack<M>(pair, 0), w[1] - unpack<M>(pair, 1)));
+        }
+    }
+    // sums += values (transposed) . weights
+#pragma unroll
+    for (int t = 0; t < kTiles; ++t) {
+#pragma unroll
+      for (int i = 0; i < S::kChunks / 2; ++i) {
+        uint32_t r[4];                // two chunks of keys 16 t .. + 7, the same of keys + 8 .. + 15
+        const int row = 16 * t + (lane & 7) + (lane >> 4) * 8;
+        load_matrix_transposed(r, v_address + row * S::kRowBytes + swizzled<S::kChunks>(row, 2 * i + (lane >> 3 & 1)) * 16);
+        if constexpr (!kCodes) {
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) multiply<M>(sums[i][h], r[0], r[1], r[2], r[3], high[t][h][0], high[t][h][1]);
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h) multiply<M>(sums[i][h], r[0], r[1], r[2], r[3], rest[t][h][0], rest[t][h][1]);
+        } else {                      // a 16-bit unit holds two neighbouring columns: even ones are rows 0 .. 7, odd ones 8 .. 15
+          uint32_t v[2][4];
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            widen<STORE, true>(r[j], v[j][0], v[j][1]);
+            widen<STORE, true>(r[2 + j], v[j][2], v[j][3]);
+          }
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              multiply<M>(sums[2 * i + j][h], v[j][0], v[j][1], v[j][2], v[j][3], high[t][h][0], high[t][h][1]);
+#pragma unroll
+          for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+            for (int j = 0; j < 2; ++j)
+              multiply<M>(sums[2 * i + j][h], v[j][0], v[j][1], v[j][2], v[j][3], rest[t][h][0], rest[t][h][1]);
         }
       }
     }
   };
 
-  // ---- the end of a piece: the warps' states are added up, warp after warp
-  auto finish = [&](bool whole) {
+  // ---- the end of a piece: every warp leaves its sums in the stage that it used last, then the block
+  // adds them up
+  auto finish = [&](const Place &at, bool whole, int stage) {
+    float *mine = reinterpret_cast<float *>(ring + stage * S::kStageBytes);
+    // (row, column) of a warp's sums: eight lanes' columns and four lanes' rows all on different banks
+    auto spot = [](int row, int column) { return row * D + (column ^ (row >> 1 & 3) * 8); };
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) {
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-      l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-      if (c == 0) {
-        float *mine = stats + (warp * ROWS + h * 8 + g) * 3;
-        mine[0] = m[h];
-        mine[1] = l[h];
-        mine[2] = weight_max[h];
-      }
-    }
-    __syncthreads();
-    auto most = [&](int row, int word) {
-      float v = -INFINITY;
+    for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) v = fmaxf(v, stats[(w * ROWS + row) * 3 + word]);
-      return v;
-    };
-    float shrink[kHalves];
+      for (int j = 0; j < 2; ++j) {
+        const int row = h * 8 + 2 * c + j;
 #pragma unroll
-    for (int h = 0; h < kHalves; ++h) shrink[h] = exp2_fast(weight_max[h] - finite_or_zero(most(h * 8 + g, 2)));
-    for (int w = 0; w < kWarps; ++w) {
-      if (w == warp) {
-#pragma unroll
-        for (int h = 0; h < kHalves; ++h) {
-          float *row = merged + (h * 8 + g) * D;
-#pragma unroll
-          for (int i = 0; i < D / 16; ++i) {
-            float x[4];
-#pragma unroll
-            for (int j = 0; j < 2; ++j)
-#pragma unroll
-              for (int n = 0; n < 2; ++n) {
-                const float(&from)[4] = sums[2 * i + n];
-                x[2 * n + j] = (kHalves == 1 ? from[j] + from[2 + j] : from[2 * h + j]) * shrink[h];
-              }
-            if constexpr (!kCodes) {   // tiles 2 i, 2 i + 1: columns 16 i + 2 c, + 1 and 16 i + 8 + 2 c, + 1
-              float2 *to0 = reinterpret_cast<float2 *>(row + 16 * i + 2 * c), *to1 = to0 + 4;
-              const float2 old0 = w ? *to0 : make_float2(0.0f, 0.0f), old1 = w ? *to1 : make_float2(0.0f, 0.0f);
-              *to0 = make_float2(old0.x + x[0], old0.y + x[1]);
-              *to1 = make_float2(old1.x + x[2], old1.y + x[3]);
-            } else {                   // even and odd columns of 16 i + 4 c .. + 3
-              float4 *to = reinterpret_cast<float4 *>(row + 16 * i + 4 * c);
-              const float4 old = w ? *to : make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-              *to = make_float4(old.x + x[0], old.y + x[2], old.z + x[1], old.w + x[3]);
-            }
-          }
+        for (int other = 4; other < 32; other <<= 1) l[h][j] += __shfl_xor_sync(0xffffffffu, l[h][j], other);
+        if (g == 0) {
+          float *state = stats + (warp * ROWS + row) * 3;
+          state[0] = m[h][j];
+          state[1] = l[h][j];
+          state[2] = weight_max[h][j];
         }
-      }
-      __syncthreads();
-    }
-    const int kv_head = use.head / p.row_tiles, row0 = (use.head - kv_head * p.row_tiles) * ROWS;
-    const int rows = min(ROWS, p.group - row0);
-    for (int index = threadIdx.x; index < rows * D; index += kBlock) {
-      const int row = index / D, column = index % D;
-      const float top = most(row, 0), weight_top = most(row, 2);
-      float denominator = 0.0f;
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        denominator += stats[(w * ROWS + row) * 3 + 1] * exp2_fast(stats[(w * ROWS + row) * 3] - finite_or_zero(top));
+        for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+          for (int k = 0; k < 2; ++k) mine[spot(row, 16 * i + (kCodes ? 2 * g + k : 8 * k + g))] = sums[i][h][2 * k + j];
+      }
+    __syncthreads();
+    const int kv_head = at.head / p.row_tiles, row0 = (at.head - kv_head * p.row_tiles) * ROWS;
+    const int rows = min(ROWS, p.group - row0);
+    const int column = threadIdx.x % D;
+    for (int row = threadIdx.x / D; row < rows; row += kBlock / D) {
+      float top = -INFINITY, weight_top = -INFINITY, denominator = 0.0f, sum = 0.0f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        top = fmaxf(top, stats[(w * ROWS + row) * 3]);
+        weight_top = fmaxf(weight_top, stats[(w * ROWS + row) * 3 + 2]);
+      }
+      const float base = finite_or_zero(top), weight_base = finite_or_zero(weight_top);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float *state = stats + (w * ROWS + row) * 3;
+        const float *from = reinterpret_cast<const float *>(dynamic_smem + (w * S::kStages + stage) * S::kStageBytes);
+        denominator += state[1] * exp2_fast(state[0] - base);
+        sum += from[spot(row, column)] * exp2_fast(state[2] - weight_base);
+      }
       const int head = kv_head * p.group + row0 + row;
       if (whole) {
-        const float unit = kCodes ? exp2_fast(finite_or_zero(weight_top) - finite_or_zero(top)) : 1.0f;
-        static_cast<T *>(p.out)[use.b * p.out_batch + head * p.out_head + column] =
-            Element<T>::narrow(__fdiv_rn(merged[index] * unit, denominator));
-        if (column == 0 && p.lse) p.lse[use.b * p.lse_batch + head * p.lse_head] = (finite_or_zero(top) + log2f(denominator)) * kLn2;
+        const float unit = kCodes ? exp2_fast(weight_base - base) : 1.0f;
+        static_cast<T *>(p.out)[at.b * p.out_batch + head * p.out_head + column] = Element<T>::narrow(__fdiv_rn(sum * unit, denominator));
+        if (column == 0 && p.lse) p.lse[at.b * p.lse_batch + head * p.lse_head] = (base + log2f(denominator)) * kLn2;
       } else {
         // slot 1 if the piece begins its head (only a run's last piece may then be unfinished), else slot 0
         float *to = p.partial + (((int64_t)blockIdx.x * 2 + (piece_first == 0)) * ROWS + row) * partial_floats(D);
-        to[column] = merged[index];
-        if (column == 0) {
-          to[D] = top;
-          to[D + 1] = denominator;
-          to[D + 2] = weight_top;
-        }
+        to[column] = sum;
+        if (column == 0) *reinterpret_cast<float4 *>(to + D) = make_float4(top, denominator, weight_top, 0.0f);
       }
     }
-    __syncthreads();   // `merged` and `stats` are free again
+    __syncthreads();   // the stage and `stats` are free again
   };
 
   // ---- the run
   look_up();
 #pragma unroll
   for (int i = 0; i < S::kStages - 1; ++i) masks[i] = produce(i);
-  load_query();
+  fetch_query(use);
+  scale_query();
   reset();
   int stage = 0;
   while (use.left > 0) {
-    const int free_stage = stage == 0 ? S::kStages - 1 : stage - 1;
-    const uint32_t newest = produce(free_stage);
+    const uint32_t newest = produce(stage == 0 ? S::kStages - 1 : stage - 1);
     copies_wait<S::kStages - 1>();
     __syncwarp();
     if (masks[0]) consume(stage, masks[0]);
@@ -612,140 +669,149 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
     for (int i = 0; i < S::kStages - 2; ++i) masks[i] = masks[i + 1];
     masks[S::kStages - 2] = newest;
-    stage = stage == S::kStages - 1 ? 0 : stage + 1;
     const bool ends = use.step == use.steps - 1;
     if (ends || use.left == 1) {
-      finish(ends && piece_first == 0);
+      const Place done = use;
       use.advance<S::kStep>(p);
+      if (use.left > 0) fetch_query(use);   // on its way while the piece is finished
+      finish(done, ends && piece_first == 0, stage);
       if (use.left > 0) {
-        load_query();
+        scale_query();
         reset();
       }
     } else {
       use.advance<S::kStep>(p);
     }
+    stage = stage == S::kStages - 1 ? 0 : stage + 1;
   }
   copies_wait<0>();
 }
 
-// One block joins the pieces of one query head: the runs that hold its steps are contiguous, the
-// first piece lies in its run's slot 1 and the others in slot 0.  Heads that one run held are done.
-template <typename T, int D, int ROWS, int STEP>
+// Block (x, y) joins the pieces of two rows of the head that a border between runs cuts, if it is the
+// first border that does: the runs that hold the head's steps are contiguous, its first piece lies in
+// its run's slot 1 and the others in slot 0.  Heads that no border cuts are done.  Every thread takes four
+// columns of some of the pieces as they come, with a running maximum of its own.
+struct State {
+  float4 sum;
+  float denominator, top, weight_top;
+  __device__ __forceinline__ void add(const float4 &x, float other_denominator, float other_top, float other_weight_top) {
+    const float new_top = fmaxf(top, other_top), new_weight_top = fmaxf(weight_top, other_weight_top);
+    const float base = finite_or_zero(new_top), weight_base = finite_or_zero(new_weight_top);
+    const float mine = exp2_fast(weight_top - weight_base), others = exp2_fast(other_weight_top - weight_base);
+    denominator = denominator * exp2_fast(top - base) + other_denominator * exp2_fast(other_top - base);
+    sum = make_float4(sum.x * mine + x.x * others, sum.y * mine + x.y * others, sum.z * mine + x.z * others, sum.w * mine + x.w * others);
+    top = new_top;
+    weight_top = new_weight_top;
+  }
+};
+
+template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_attention_join_kernel(const Problem p) {
-  constexpr int kLanes = D / 4;                       // threads of a row of sums, four columns each
-  constexpr int kRows = kJoinThreads / kLanes;        // pieces at a time
-  __shared__ int64_t scratch[kJoinThreads / 32];
-  __shared__ float tops[kJoinThreads / 32][2];
-  __shared__ float joined[kRows][D + 4];
-  const int b = blockIdx.y, head = blockIdx.x;
-  const int kv_head = head / p.group, in_group = head - kv_head * p.group;
-  const int tile = in_group / ROWS, row = in_group - tile * ROWS;
-  const int head_tiles = p.kv_heads * p.row_tiles;
-  int64_t total = 0, first = 0, unused;
-  for (int base = 0; base < p.batch; base += kJoinThreads) {
-    const int other = base + threadIdx.x;
-    const int64_t steps = other < p.batch ? (length_of(p, other) + STEP - 1) / STEP : 0;
-    total += block_scan<kJoinThreads>(steps, unused, scratch);
-    first += block_scan<kJoinThreads>(other < b ? steps : 0, unused, scratch);
-  }
-  const int length = length_of(p, b), steps = (length + STEP - 1) / STEP;
-  total *= head_tiles;
-  first = first * head_tiles + (int64_t)(kv_head * p.row_tiles + tile) * steps;
+  constexpr int kLanes = D / 4;                       // threads of a row of sums
+  constexpr int kParts = kJoinThreads / kLanes / kJoinRows;   // pieces at a time
+  __shared__ float4 part_sums[kParts][kJoinRows][kLanes];
+  __shared__ float part_states[kParts][kJoinRows][3];
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  T *out = static_cast<T *>(p.out) + b * p.out_batch + head * p.out_head;
-  if (steps == 0) {
-    if (threadIdx.x < D) out[threadIdx.x] = Element<T>::narrow(0.0f);
-    if (threadIdx.x == 0 && p.lse) p.lse[b * p.lse_batch + head * p.lse_head] = -INFINITY;
-    return;
-  }
+  const int run = blockIdx.y / p.abreast + 1, lane_head = blockIdx.y % p.abreast;
+  const Border border =
+      reinterpret_cast<const Border *>(p.partial + (int64_t)p.runs * p.abreast * 2 * ROWS * partial_floats(D))[run * p.abreast + lane_head];
+  if (border.step == 0) return;
+  const int64_t runs = min((int64_t)p.runs, border.total), first = border.total * run / runs - border.step;
+  if (border.total * (run - 1) / runs > first) return;
+  const int lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes, part = slot / kJoinRows, mine = slot % kJoinRows;
+  const int row = blockIdx.x * kJoinRows + mine;
+  const int kv_head = border.head / p.row_tiles, in_group = (border.head - kv_head * p.row_tiles) * ROWS + row;
+  const bool live = row < ROWS && in_group < p.group;
+  const int head = kv_head * p.group + in_group, run0 = run - 1;
   // the run of step s is the largest r with total * r / runs <= s
-  const int64_t runs = min((int64_t)p.runs, total);
-  const int run0 = (int)(((first + 1) * runs - 1) / total), run1 = (int)(((first + steps) * runs - 1) / total);
-  if (run0 == run1) return;
-  const int pieces = run1 - run0 + 1;
-  auto piece = [&](int i) {
-    return p.partial + (((int64_t)(run0 + i) * 2 + (i == 0)) * ROWS + row) * partial_floats(D);
-  };
-  float top = -INFINITY, weight_top = -INFINITY;
-  for (int i = threadIdx.x; i < pieces; i += kJoinThreads) {
-    const float *from = piece(i);
-    top = fmaxf(top, from[D]);
-    weight_top = fmaxf(weight_top, from[D + 2]);
-  }
-  top = warp_max(top);
-  weight_top = warp_max(weight_top);
-  if ((threadIdx.x & 31) == 0) {
-    tops[threadIdx.x >> 5][0] = top;
-    tops[threadIdx.x >> 5][1] = weight_top;
-  }
-  __syncthreads();
-#pragma unroll
-  for (int w = 0; w < kJoinThreads / 32; ++w) {
-    top = fmaxf(top, tops[w][0]);
-    weight_top = fmaxf(weight_top, tops[w][1]);
-  }
-  top = finite_or_zero(top);
-  weight_top = finite_or_zero(weight_top);
-  const int lane = threadIdx.x % kLanes, part = threadIdx.x / kLanes;
-  float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
-  float denominator = 0.0f;
+  const int pieces = (int)(((first + border.steps) * runs - 1) / border.total) - run0 + 1;
+  State state{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -INFINITY, -INFINITY};
+  if (live) {
 #pragma unroll 4
-  for (int i = part; i < pieces; i += kRows) {
-    const float *from = piece(i);
-    const float4 x = reinterpret_cast<const float4 *>(from)[lane], state = reinterpret_cast<const float4 *>(from)[D / 4];
-    const float shrink = exp2_fast(state.z - weight_top);
-    denominator += state.y * exp2_fast(state.x - top);
-    sum.x += x.x * shrink;
-    sum.y += x.y * shrink;
-    sum.z += x.z * shrink;
-    sum.w += x.w * shrink;
+    for (int i = part; i < pieces; i += kParts) {
+      const float4 *from = reinterpret_cast<const float4 *>(
+          p.partial + (((int64_t)((run0 + i) * p.abreast + lane_head) * 2 + (i == 0)) * ROWS + row) * partial_floats(D));
+      const float4 x = from[lane], other = from[D / 4];
+      state.add(x, other.y, other.x, other.z);
+    }
   }
-  *reinterpret_cast<float4 *>(&joined[part][4 * lane]) = sum;
-  if (lane == 0) joined[part][D] = denominator;
+  part_sums[part][mine][lane] = state.sum;
+  if (lane == 0) {
+    part_states[part][mine][0] = state.denominator;
+    part_states[part][mine][1] = state.top;
+    part_states[part][mine][2] = state.weight_top;
+  }
   __syncthreads();
-  if (threadIdx.x >= D) return;
-  float value = 0.0f;
-  denominator = 0.0f;
+  if (part != 0 || !live) return;
 #pragma unroll
-  for (int i = 0; i < kRows; ++i) {
-    value += joined[i][threadIdx.x];
-    denominator += joined[i][D];
-  }
-  out[threadIdx.x] = Element<T>::narrow(__fdiv_rn(value * exp2_fast(weight_top - top), denominator));
-  if (threadIdx.x == 0 && p.lse) p.lse[b * p.lse_batch + head * p.lse_head] = (top + log2f(denominator)) * kLn2;
+  for (int i = 1; i < kParts; ++i)
+    state.add(part_sums[i][mine][lane], part_states[i][mine][0], part_states[i][mine][1], part_states[i][mine][2]);
+  const float base = finite_or_zero(state.top), unit = exp2_fast(finite_or_zero(state.weight_top) - base);
+  T *out = static_cast<T *>(p.out) + border.b * p.out_batch + head * p.out_head + 4 * lane;
+  const float values[4] = {state.sum.x, state.sum.y, state.sum.z, state.sum.w};
+  uint32_t packed[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+    packed[i] = pack<T>(__fdiv_rn(values[2 * i] * unit, state.denominator), __fdiv_rn(values[2 * i + 1] * unit, state.denominator));
+  *reinterpret_cast<uint2 *>(out) = make_uint2(packed[0], packed[1]);
+  if (lane == 0 && p.lse) p.lse[border.b * p.lse_batch + head * p.lse_head] = (base + log2f(state.denominator)) * kLn2;
 }
 
 // --------------------------------------------------------------------- host
 int rows_of(int64_t group) { return group <= 8 ? 8 : 16; }
-int step_of(int store) { return store == B200_I8 || store == B200_E4M3 ? Shape<cache::kInt8, 128>::kStep : Shape<cache::kNative, 128>::kStep; }
+int step_of(int store) {
+  return store == B200_I8 || store == B200_E4M3 ? Shape<cache::kInt8, 128, 8>::kStep : Shape<cache::kNative, 128, 8>::kStep;
+}
+
+// Key heads (and tiles of query heads) that go through a run side by side, in neighbouring blocks: they
+// want the same pages at the same time, and what lies next to one another in them.  With token-major pages
+// that is the scales of 8 heads in 32 bytes, which heads that follow one another each read from HBM again
+// (64 sequences of 4096 keys, 8 heads in e4m3: 119.6 us, abreast 98.6).  The largest divisor up to 16 that
+// leaves at most 3% of the resident blocks without a run.
+int heads_abreast(int64_t head_tiles, int64_t resident) {
+  for (int64_t n = 16; n > 1; --n)
+    if (head_tiles % n == 0 && resident / n * n * 100 >= resident * 97) return (int)n;
+  return 1;
+}
 
 // As many runs as blocks are resident, or as there can be steps.
-int64_t runs_of(int64_t batch, int64_t kv_heads, int64_t group, int64_t most_keys, int store) {
+struct Split {
+  int64_t runs, abreast;
+};
+Split split_of(int64_t batch, int64_t kv_heads, int64_t group, int64_t most_keys, int store) {
   const int64_t rows = rows_of(group), tiles = kv_heads * ((group + rows - 1) / rows), step = step_of(store);
-  const int64_t each = (most_keys + step - 1) / step, resident = (int64_t)kBlocksPerSm * sm_count();
-  if (batch == 0 || tiles == 0 || each == 0) return 1;
-  if (batch >= resident || tiles >= resident || each >= resident || batch * tiles >= resident) return resident;
-  return batch * tiles * each < resident ? batch * tiles * each : resident;
+  const int64_t each = (most_keys + step - 1) / step;
+  const int64_t resident = (int64_t)(rows == 8 ? Shape<cache::kNative, 128, 8>::kBlocksPerSm : Shape<cache::kNative, 128, 16>::kBlocksPerSm) * sm_count();
+  if (batch == 0 || tiles == 0 || each == 0) return {1, 1};
+  const int64_t abreast = heads_abreast(tiles, resident), most = resident / abreast, groups = tiles / abreast;
+  if (batch >= most || groups >= most || each >= most || batch * groups >= most) return {most, abreast};
+  return {batch * groups * each < most ? batch * groups * each : most, abreast};
+}
+
+// Words of scratch: two unfinished pieces and a border a block.
+int64_t scratch_words(const Split &split, int64_t group, int64_t columns) {
+  return split.runs * split.abreast * (2 * rows_of(group) * partial_floats((int)columns) + (int64_t)(sizeof(Border) / 4));
 }
 
 template <typename T, int STORE, int D, int ROWS> int launch(const Problem &p, cudaStream_t stream) {
   const auto kernel = paged_attention_kernel<T, STORE, D, ROWS>;
-  const size_t bytes = smem_bytes<STORE, D, ROWS>();
+  const size_t bytes = Shape<STORE, D, ROWS>::kSmemBytes;
   B200_CUDA_TRY(opt_in_dynamic_smem(kernel, bytes));
-  kernel<<<p.runs, kBlock, bytes, stream>>>(p);
+  kernel<<<p.runs * p.abreast, kBlock, bytes, stream>>>(p);
   B200_CUDA_TRY(cudaGetLastError());
+  if (p.runs == 1) return B200_OK;   // no border
   // placed while the first kernel still runs; it waits for that kernel's end on the device
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(p.kv_heads * p.group, p.batch);
+  config.gridDim = dim3(((p.group < ROWS ? p.group : ROWS) + kJoinRows - 1) / kJoinRows, (p.runs - 1) * p.abreast);
   config.blockDim = dim3(kJoinThreads);
   config.stream = stream;
   config.attrs = &early;
   config.numAttrs = 1;
-  B200_CUDA_TRY(cudaLaunchKernelEx(&config, paged_attention_join_kernel<T, D, ROWS, Shape<STORE, D>::kStep>, p));
+  B200_CUDA_TRY(cudaLaunchKernelEx(&config, paged_attention_join_kernel<T, D, ROWS>, p));
   return B200_OK;
 }
 template <typename T, int STORE, int D> int by_rows(const Problem &p, cudaStream_t stream) {
@@ -770,7 +836,7 @@ extern "C" int b200_paged_attention_scratch(int64_t batch, int64_t heads, int64_
   if (!words || batch < 0 || heads < 0 || kv_heads < 1 || heads % kv_heads || heads > 65536 || keys < 0 || head_dim < 1 || head_dim > 256)
     return fail(B200_ERR_INVALID_ARGUMENT, "paged_attention_scratch: an extent is out of range");
   const int64_t group = heads / kv_heads;
-  *words = runs_of(batch, kv_heads, group ? group : 1, keys, store) * 2 * rows_of(group) * partial_floats((int)head_dim);
+  *words = scratch_words(split_of(batch, kv_heads, group ? group : 1, keys, store), group, head_dim);
   return B200_OK;
 }
 
@@ -814,10 +880,11 @@ extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float s
   if (k.d2 && table.d1 > (INT32_MAX - 4096) / k.d2)   // key positions and steps are counted in int32
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: a row of the block table names 2^31 positions or more", what);
   const int64_t most_keys = table.d1 * k.d2;
-  const int64_t group = q.d1 / k.d1, runs = runs_of(q.d0, k.d1, group, most_keys, store);
+  const int64_t group = q.d1 / k.d1;
+  const Split split = split_of(q.d0, k.d1, group, most_keys, store);
   if (!q.data || !out.data || !lengths.data || (table.d1 && !table.data) || !partial.data)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  if (partial.d0 < runs * 2 * rows_of(group) * partial_floats((int)q.d2) || partial.s0 != 1 || !aligned16(partial.data))
+  if (partial.d0 < scratch_words(split, group, q.d2) || partial.s0 != 1 || !aligned16(partial.data))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the scratch is too short, not contiguous or not 16-byte aligned", what);
   if (!heads::vector_rows(q, 2) || !heads::vector_rows(out, 2))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT,
@@ -843,7 +910,8 @@ extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float s
   p.partial = static_cast<float *>(const_cast<void *>(partial.data));
   p.batch = (int)q.d0; p.kv_heads = (int)k.d1; p.group = (int)group;
   p.row_tiles = (int)((group + rows_of(group) - 1) / rows_of(group));
-  p.page_size = (int)k.d2; p.pages = (int)k.d0; p.runs = (int)runs;
+  p.page_size = (int)k.d2; p.pages = (int)k.d0;
+  p.runs = (int)split.runs; p.abreast = (int)split.abreast;
   p.most_keys = most_keys;
   p.scale_log2e = scale * kLog2e;
   p.status = static_cast<int *>(const_cast<void *>(workspace.data));

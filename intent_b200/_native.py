@@ -9,6 +9,8 @@ from __future__ import annotations
 
 import ctypes
 import os
+from importlib.machinery import ExtensionFileLoader
+from importlib.util import module_from_spec, spec_from_file_location
 from pathlib import Path
 from threading import Lock
 
@@ -103,6 +105,28 @@ def entry(name: str):
     if name not in SIGNATURES:
         raise KeyError(f"{name} is not an entry of the intent_b200 C ABI")
     return getattr(library(), name)
+
+
+BINDING_PATH = LIBRARY_PATH.with_name("binding.so")
+_binding = None
+
+
+def binding():
+    """The module that calls entries which take their views as one array (``csrc/binding.cpp``)."""
+    global _binding
+    with _lock:
+        if _binding is None:
+            if not BINDING_PATH.exists():
+                raise NativeLibraryMissing(f"{BINDING_PATH} is missing: build it with `python -m intent_b200.build`.")
+            loader = ExtensionFileLoader("binding", str(BINDING_PATH))
+            _binding = module_from_spec(spec_from_file_location("binding", str(BINDING_PATH), loader=loader))
+            loader.exec_module(_binding)
+    return _binding
+
+
+def address(name: str) -> int:
+    """Where an entry is, as a number."""
+    return ctypes.cast(entry(name), _P).value
 
 
 def last_error() -> str:

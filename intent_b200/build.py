@@ -3,6 +3,7 @@
 ``python -m intent_b200.build`` compiles
 
 * ``intent_b200/csrc/*.cu``  -> ``intent_b200/lib/libintent_b200.so``  (nvcc, sm_100a only)
+* ``intent_b200/csrc/binding.cpp`` -> ``intent_b200/lib/binding.so`` (g++, against torch's headers)
 * ``intent_b200/compiler/b200_compile.cpp`` -> ``intent_b200/bin/b200-compile`` (g++)
 
 nvcc cross-compiles without a GPU, so this runs anywhere the CUDA toolkit is
@@ -88,6 +89,27 @@ def build_library(*, force: bool = False, verbose: bool = False, resource_usage:
     return library
 
 
+BINDING = PACKAGE / "lib" / "binding.so"
+
+
+def build_binding(*, force: bool = False) -> Path:
+    """The module that packs torch tensors for the entries that take their views as one array."""
+    source = CSRC / "binding.cpp"
+    BINDING.parent.mkdir(parents=True, exist_ok=True)
+    if force or _stale(BINDING, [source]):
+        import sysconfig
+
+        import torch
+        from torch.utils import cpp_extension
+        cuda = Path(_nvcc()).resolve().parents[1]
+        includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(cuda / "include")]
+        libraries = Path(torch.__file__).resolve().parent / "lib"
+        _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{path}" for path in includes),
+              str(source), "-o", str(BINDING), f"-L{libraries}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
+    return BINDING
+
+
 STRUCTURES = PACKAGE / "compiler" / "structures.inc"
 
 
@@ -163,6 +185,7 @@ def install_reference() -> Path | None:
 def build_all(*, force: bool = False, verbose: bool = False) -> None:
     build_library(force=force, verbose=verbose)
     build_library(force=force, verbose=verbose, checked=True)
+    build_binding(force=force)
     build_compiler(force=force)
     install_reference()
 

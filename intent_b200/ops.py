@@ -13,7 +13,6 @@ buffers: contiguous ``torch.empty`` on the argument device
 from __future__ import annotations
 
 import ctypes
-from array import array
 from functools import lru_cache
 
 import torch
@@ -288,58 +287,74 @@ def attention_backward_dq(q, k, v, grad_output, lse, delta, scale: float, *, hea
 
 
 # ---- operators around a key-value cache ------------------------------------------------------
-# Calls of a few microseconds on the device: a view is checked and turned into its slots in one go,
-# and the slots cross the C ABI as one array (see include/intent_b200.h).
+# Calls of a few microseconds on the device, so their views are not packed here but by a native module.
 
 def _cuda_device(tensor) -> int:
     """Index of the device that the call runs on, from its first tensor."""
     if not isinstance(tensor, torch.Tensor):
         raise TypeError("intent_b200 operators take torch.Tensor arguments")
-    if tensor.device.type != "cuda":
+    if not tensor.is_cuda:
         raise ValueError(f"intent_b200 executes on cuda, but an argument is on {tensor.device}")
     return tensor.get_device()
 
 
-def _bound(name: str, tensor, dtype: torch.dtype, shape: tuple, device: int) -> tuple:
-    """The slots of a view that has this type, shape and device, or the error that says what it lacks."""
+_addresses: dict[str, int] = {}
+_native_invoke = None
+
+
+def _invoke(name: str, device: int, views: tuple, number, code: int, other: int) -> tuple:
+    """Calls an entry that takes its views as one array of slots, and returns the tensors that were made for it.
+    ``views``: (name, tensor, dtype, shape), with ``...`` for the tensor if it is to be made, (name, ..., dtype, shape,
+    True) for scratch, (name, None, rank) for a view that is not there; ``number``: the entry's f32 argument, if it
+    has one.  Everything made is a contiguous allocation of the call's own in the current stream's order, so
+    calls may overlap."""
+    global _native_invoke
+    entry = _addresses.get(name)
+    if entry is None:
+        _native_invoke = _native.binding().invoke
+        entry = _addresses[name] = _native.address(name)
+    made = _native_invoke(entry, device, views, number, code, other)
+    if type(made) is not tuple:
+        if made < 0:
+            _refuse(views[-1 - made], device)
+        _native.check(name, made)
+    return made
+
+
+def _refuse(view: tuple, device: int) -> None:
+    """Raises what is wrong with a view."""
+    name, tensor, dtype, shape = view
     if not isinstance(tensor, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
-    if tensor.dtype is not dtype or tensor.shape != shape:
-        _expect(name, tensor, dtype, shape)
-    if tensor.get_device() != device:
-        _cuda_device(tensor)
+    _expect(name, tensor, dtype, shape)
+    if _cuda_device(tensor) != device:
         raise ValueError("arguments span different devices")
-    return (tensor.data_ptr(), *shape, *tensor.stride())
+    raise ValueError(f"{name} must be a strided tensor")
 
 
-def _invoke(name: str, device: int, slots: tuple, *tail) -> None:
-    packed = array("q", slots)
-    address, count = packed.buffer_info()
-    if torch.cuda.current_device() == device:
-        status = _native.entry(name)(address, count, *tail, torch._C._cuda_getCurrentRawStream(device))
-    else:
-        with torch.cuda.device(device):
-            status = _native.entry(name)(address, count, *tail, torch._C._cuda_getCurrentRawStream(device))
-    if status != _native.OK:
-        _native.check(name, status)
+def _outputs(made: tuple, *given) -> tuple:
+    """The outputs of a call: those that the caller gave, and for the others what was made, in order."""
+    rest = iter(made)
+    return tuple(next(rest) if tensor is None else tensor for tensor in given)
 
 
-_status_slots: dict[int, tuple] = {}
+_status_spaces: dict[int, tuple] = {}
 
 
 def _status(device: int) -> tuple:
-    """The slots of ``workspace(device)``, where an entry records a bad index.  It is made once per device and
+    """The view of ``workspace(device)``, where an entry records a bad index.  It is made once per device and
     shared by all streams, so the first call may not fall into a graph capture, whose replays would
     clear it, and its zeros have to be there before any other stream writes to it."""
-    if device not in _status_slots:
+    view = _status_spaces.get(device)
+    if view is None:
         where = torch.device("cuda", device)
         with torch.cuda.device(where):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call this operator once outside a graph capture before capturing it")
             space = workspace(where)
             torch.cuda.current_stream(where).synchronize()
-        _status_slots[device] = tuple(_slots(space))
-    return _status_slots[device]
+        view = _status_spaces[device] = ("workspace", space, torch.int32, (_native.WORKSPACE_WORDS,))
+    return view
 
 
 @lru_cache(maxsize=4096)
@@ -374,19 +389,14 @@ def head_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, epsilon: flo
     ``workspace_status``.  Returns ``(q_out, k_out)``; an output may be its input."""
     device = _cuda_device(q)
     shape, k_shape, table = _rotary_shapes(q, k, cos)
-    dtype = q.dtype
-    if q_out is None:
-        q_out = q.new_empty(shape)
-    if k_out is None:
-        k_out = q.new_empty(k_shape)
-    _invoke("b200_head_norm_rotary", device,
-            (*_bound("q", q, dtype, shape, device), *_bound("k", k, dtype, k_shape, device),
-             *_bound("q_weight", q_weight, dtype, shape[2:], device), *_bound("k_weight", k_weight, dtype, shape[2:], device),
-             *_bound("cos", cos, torch.float32, table, device), *_bound("sin", sin, torch.float32, table, device),
-             *_bound("positions", positions, torch.int32, shape[:1], device), *_bound("q_out", q_out, dtype, shape, device),
-             *_bound("k_out", k_out, dtype, k_shape, device), *_status(device)),
-            float(epsilon), _CODES[dtype], bool(interleaved))
-    return q_out, k_out
+    dtype, columns = q.dtype, shape[2:]
+    made = _invoke(
+        "b200_head_norm_rotary", device,
+        (("q", q, dtype, shape), ("k", k, dtype, k_shape), ("q_weight", q_weight, dtype, columns),
+         ("k_weight", k_weight, dtype, columns), ("cos", cos, torch.float32, table), ("sin", sin, torch.float32, table),
+         ("positions", positions, torch.int32, shape[:1]), ("q_out", ... if q_out is None else q_out, dtype, shape),
+         ("k_out", ... if k_out is None else k_out, dtype, k_shape), _status(device)), float(epsilon), _CODES[dtype], bool(interleaved))
+    return _outputs(made, q_out, k_out)
 
 
 def head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions, epsilon: float = 1e-6, *,
@@ -397,44 +407,36 @@ def head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin
     device = _cuda_device(q)
     shape, k_shape, table = _rotary_shapes(q, k, cos)
     dtype, columns = q.dtype, shape[2:]
-    if dq is None:
-        dq = q.new_empty(shape)
-    if dk is None:
-        dk = q.new_empty(k_shape)
     rows = _scratch_size("b200_head_norm_rotary_scratch", device, shape[0], shape[1], k_shape[1], shape[2])
-    partial = q.new_empty((rows, shape[2]), dtype=torch.float32)    # the call's own: calls may overlap
-    dq_weight, dk_weight = q.new_empty(columns, dtype=torch.float32), q.new_empty(columns, dtype=torch.float32)
-    _invoke("b200_head_norm_rotary_backward", device,
-            (*_bound("grad_q", grad_q, dtype, shape, device), *_bound("grad_k", grad_k, dtype, k_shape, device),
-             *_bound("q", q, dtype, shape, device), *_bound("k", k, dtype, k_shape, device),
-             *_bound("q_weight", q_weight, dtype, columns, device), *_bound("k_weight", k_weight, dtype, columns, device),
-             *_bound("cos", cos, torch.float32, table, device), *_bound("sin", sin, torch.float32, table, device),
-             *_bound("positions", positions, torch.int32, shape[:1], device), *_bound("dq", dq, dtype, shape, device),
-             *_bound("dk", dk, dtype, k_shape, device), dq_weight.data_ptr(), shape[2], 1, dk_weight.data_ptr(), shape[2], 1,
-             partial.data_ptr(), rows, shape[2], shape[2], 1, *_status(device)),
-            float(epsilon), _CODES[dtype], bool(interleaved))
-    return dq, dk, dq_weight, dk_weight
+    made = _invoke(
+        "b200_head_norm_rotary_backward", device,
+        (("grad_q", grad_q, dtype, shape), ("grad_k", grad_k, dtype, k_shape), ("q", q, dtype, shape), ("k", k, dtype, k_shape),
+         ("q_weight", q_weight, dtype, columns), ("k_weight", k_weight, dtype, columns), ("cos", cos, torch.float32, table),
+         ("sin", sin, torch.float32, table), ("positions", positions, torch.int32, shape[:1]),
+         ("dq", ... if dq is None else dq, dtype, shape), ("dk", ... if dk is None else dk, dtype, k_shape),
+         ("dq_weight", ..., torch.float32, columns), ("dk_weight", ..., torch.float32, columns), ("partial", ..., torch.float32, (rows, shape[2]), True),
+         _status(device)), float(epsilon), _CODES[dtype], bool(interleaved))
+    return _outputs(made, dq, dk, None, None)
 
 
-_NO_SCALES = (0,) * 14
+_NO_SCALES = (("k_scale", None, 3), ("v_scale", None, 3))
 _CACHE_TYPES = (torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn)
 
 
-def _cache_slots(k_cache, v_cache, k_scale, v_scale, device: int) -> tuple:
-    """Shape of a paged cache, its slots and its scales' slots."""
+def _cache_views(k_cache, v_cache, k_scale, v_scale) -> tuple:
+    """Shape of a paged cache, its views and its scales' views."""
     shape = _shape("k_cache", k_cache, 4, "(pages, heads, page_size, head_dim)")
     dtype = k_cache.dtype
     if dtype not in _CACHE_TYPES:
         raise TypeError(f"k_cache must be float16, bfloat16, int8 or float8_e4m3fn, got {dtype}")
-    views = _bound("k_cache", k_cache, dtype, shape, device) + _bound("v_cache", v_cache, dtype, shape, device)
+    views = (("k_cache", k_cache, dtype, shape), ("v_cache", v_cache, dtype, shape))
     if dtype is torch.float16 or dtype is torch.bfloat16:
         if k_scale is not None or v_scale is not None:
             raise ValueError("a 16-bit cache has no scales")
         return shape, views, _NO_SCALES
     if k_scale is None or v_scale is None:
         raise ValueError("an 8-bit cache needs k_scale and v_scale")
-    return shape, views, (_bound("k_scale", k_scale, torch.float32, shape[:3], device)
-                          + _bound("v_scale", v_scale, torch.float32, shape[:3], device))
+    return shape, views, (("k_scale", k_scale, torch.float32, shape[:3]), ("v_scale", v_scale, torch.float32, shape[:3]))
 
 
 def cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
@@ -448,14 +450,13 @@ def cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     negative must differ.  Returns ``(k_cache, v_cache)``."""
     device = _cuda_device(k)
     dtype = _float_type("k", k, (torch.float16, torch.bfloat16))
-    cache, views, scales = _cache_slots(k_cache, v_cache, k_scale, v_scale, device)
+    cache, views, scales = _cache_views(k_cache, v_cache, k_scale, v_scale)
     if k_cache.dtype is not dtype and k_cache.element_size() == 2:
         raise TypeError(f"k_cache must have dtype {dtype}, torch.int8 or torch.float8_e4m3fn, got {k_cache.dtype}")
     shape = (_shape("k", k, 3, "(tokens, heads, head_dim)")[0], cache[1], cache[3])
     _invoke("b200_cache_write", device,
-            (*_bound("k", k, dtype, shape, device), *_bound("v", v, dtype, shape, device),
-             *_bound("slots", slots, torch.int64, shape[:1], device), *views, *scales, *_status(device)),
-            _CODES[dtype], _CODES[k_cache.dtype])
+            (("k", k, dtype, shape), ("v", v, dtype, shape), ("slots", slots, torch.int64, shape[:1]), *views, *scales,
+             _status(device)), None, _CODES[dtype], _CODES[k_cache.dtype])
     return k_cache, v_cache
 
 
@@ -464,7 +465,7 @@ def cache_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, *, dtype=Non
     head_dim): of a 16-bit cache as they are, of an 8-bit one as code * scale in ``dtype`` (f16 or bf16, the
     default).  Negative slots give zeros, and so do slots behind the cache, which ``workspace_status`` reports."""
     device = _cuda_device(k_cache)
-    cache, views, scales = _cache_slots(k_cache, v_cache, k_scale, v_scale, device)
+    cache, views, scales = _cache_views(k_cache, v_cache, k_scale, v_scale)
     wide = k_cache.element_size() == 2
     if dtype is None:
         dtype = k_cache.dtype if wide else torch.bfloat16 if k_out is None else k_out.dtype
@@ -473,15 +474,11 @@ def cache_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, *, dtype=Non
     if wide and dtype != k_cache.dtype:
         raise TypeError(f"a {k_cache.dtype} cache gives its rows as they are, not as {dtype}")
     shape = (_shape("slots", slots, 1, "(tokens,)")[0], cache[1], cache[3])
-    if k_out is None:
-        k_out = k_cache.new_empty(shape, dtype=dtype)
-    if v_out is None:
-        v_out = k_cache.new_empty(shape, dtype=dtype)
-    _invoke("b200_cache_read", device,
-            (*views, *_bound("slots", slots, torch.int64, shape[:1], device), *scales,
-             *_bound("k_out", k_out, dtype, shape, device), *_bound("v_out", v_out, dtype, shape, device), *_status(device)),
-            _CODES[dtype], _CODES[k_cache.dtype])
-    return k_out, v_out
+    made = _invoke(
+        "b200_cache_read", device,
+        (*views, ("slots", slots, torch.int64, shape[:1]), *scales, ("k_out", ... if k_out is None else k_out, dtype, shape),
+         ("v_out", ... if v_out is None else v_out, dtype, shape), _status(device)), None, _CODES[dtype], _CODES[k_cache.dtype])
+    return _outputs(made, k_out, v_out)
 
 
 def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, k_scale=None, v_scale=None, out=None,
@@ -496,7 +493,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, 
     device = _cuda_device(q)
     dtype = _float_type("q", q, (torch.float16, torch.bfloat16))
     shape = _shape("q", q, 3, "(batch, heads, head_dim)")
-    cache, views, scales = _cache_slots(k_cache, v_cache, k_scale, v_scale, device)
+    cache, views, scales = _cache_views(k_cache, v_cache, k_scale, v_scale)
     if k_cache.dtype is not dtype and k_cache.element_size() == 2:
         raise TypeError(f"k_cache must have dtype {dtype}, torch.int8 or torch.float8_e4m3fn, got {k_cache.dtype}")
     batch, heads, columns = shape
@@ -506,21 +503,14 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, 
         raise ValueError(f"{heads} query heads are not a multiple of the cache's {cache[1]}")
     table = (batch, _shape("block_table", block_table, 2, "(batch, columns)")[1])
     store = _CODES[k_cache.dtype]
-    if out is None:
-        out = q.new_empty(shape)
     words = _scratch_size("b200_paged_attention_scratch", device, batch, heads, cache[1], columns, table[1] * cache[2], store)
-    partial = q.new_empty((words,), dtype=torch.float32)    # the call's own: calls may overlap
-    lse, lse_slots = None, (0,) * 5
-    if return_lse:
-        lse = q.new_empty((batch, heads), dtype=torch.float32)
-        lse_slots = (lse.data_ptr(), batch, heads, heads, 1)
-    _invoke("b200_paged_attention", device,
-            (*_bound("q", q, dtype, shape, device), *views, *scales,
-             *_bound("block_table", block_table, torch.int32, table, device),
-             *_bound("lengths", lengths, torch.int32, shape[:1], device), *_bound("out", out, dtype, shape, device), *lse_slots,
-             partial.data_ptr(), words, 1, *_status(device)),
-            float(scale), _CODES[dtype], store)
-    return (out, lse) if return_lse else out
+    made = _invoke(
+        "b200_paged_attention", device,
+        (("q", q, dtype, shape), *views, *scales, ("block_table", block_table, torch.int32, table),
+         ("lengths", lengths, torch.int32, shape[:1]), ("out", ... if out is None else out, dtype, shape),
+         ("lse", ..., torch.float32, shape[:2]) if return_lse else ("lse", None, 2),
+         ("partial", ..., torch.float32, (words,), True), _status(device)), float(scale), _CODES[dtype], store)
+    return _outputs(made, out, None) if return_lse else out if out is not None else made[0]
 
 
 def gather_probe(table: torch.Tensor, gathers: int, *, variant: int = 1, hints: bool = True) -> None:

@@ -196,12 +196,27 @@ def test_ops_check_before_any_call():
     cache = torch.zeros(2, 2, 16, 64, dtype=torch.int8)
     with pytest.raises(ValueError, match="executes on cuda"):
         ops.cache_write(k, k, torch.zeros(3, dtype=torch.int64), cache, cache)
-    for wrong, message in (((cache, cache.half(), None, None), "v_cache must have dtype"),
-                           ((cache, cache, None, None), "needs k_scale"), ((cache.half(), cache.half(), w, w), "has no scales"),
-                           ((cache.float(), cache.float(), None, None), "k_cache must be"), ((cache[0], cache[0], None, None), "k_cache is a"),
-                           ((cache, [1], None, None), "v_cache must be a torch.Tensor"), ((cache, cache[1:], w, w), "v_cache must have shape")):
+    for wrong, message in (((cache, cache, None, None), "needs k_scale"), ((cache.half(), cache.half(), w, w), "has no scales"),
+                           ((cache.float(), cache.float(), None, None), "k_cache must be"), ((cache[0], cache[0], None, None), "k_cache is a")):
         with pytest.raises((TypeError, ValueError), match=message):
-            ops._cache_slots(*wrong, -1)
+            ops._cache_views(*wrong)
+
+
+def test_a_view_that_is_not_what_it_should_be_is_named():
+    """The native module finds it before any call, ops says what is wrong with it."""
+    t = torch.zeros(3, 4)
+    good = ("first", None, 2)
+    for bad, error, message in ((("x", t.half(), torch.float32, (3, 4)), TypeError, "x must have dtype torch.float32"),
+                                (("x", t, torch.float32, (4, 3)), ValueError, r"x must have shape \(4, 3\), got \(3, 4\)"),
+                                (("x", t, torch.float32, (3, 4, 1)), ValueError, "x must have shape"),
+                                (("x", [1.0], torch.float32, (1,)), TypeError, "x must be a torch.Tensor"),
+                                (("x", None, torch.float32, (1,)), TypeError, "x must be a torch.Tensor"),
+                                (("x", t, torch.float32, (3, 4)), ValueError, "executes on cuda")):
+        with pytest.raises(error, match=message):
+            ops._invoke("b200_cache_write", 0, (good, bad), None, 1, 1)
+    for wrong in ((1, 0, [good], None, 1, 1), (1, 0, (good,), None, 1), (1, 0, ("x",), None, 1, 1), (1, 0, (good,), "x", 1, 1)):
+        with pytest.raises(TypeError):
+            _native.binding().invoke(*wrong)
 
 
 # ------------------------------------------------------- the plain forms hold what they are held to

@@ -45,7 +45,7 @@ using heads::View4;
 
 constexpr int kWarps = 4;
 constexpr int kBlock = kWarps * 32;
-constexpr int kJoinThreads = 256, kJoinRows = 2;
+constexpr int kJoinThreads = 1024;
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 
 struct Problem {
@@ -89,12 +89,14 @@ template <int STORE, int D, int ROWS> struct Shape {
 constexpr int partial_floats(int columns) { return columns + 4; }   // sums, m, l, M, unused
 
 // What a run begins with, for the kernel that joins: (sequence, head tile) and how many of its steps lie
-// before the run.
+// before the run.  (What follows from it is worked out there: 64-bit divisions here cost the main loop
+// registers and the call 5%.)
 struct Border {
   int64_t total;
   int b, head, step, steps;
+  int64_t unused;
 };
-static_assert(sizeof(Border) == 24, "six words");
+static_assert(sizeof(Border) == 32, "two vectors");
 
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
@@ -293,7 +295,7 @@ paged_attention_kernel(const Problem p) {
   load.head = load.head * p.abreast + lane_head;
   load.left = end - begin;
   Place use = load;       // what the next products take
-  if (threadIdx.x == 0) *border = Border{total, load.b, load.head, load.step, load.steps};
+  if (threadIdx.x == 0) *border = Border{total, load.b, load.head, load.step, load.steps, 0};
 
   // ---- copies: lane r looks row r of the tile up; a row's 16-byte pieces go to neighbouring lanes
   unsigned char *ring = dynamic_smem + warp * S::kStages * S::kStageBytes;
@@ -687,75 +689,94 @@ paged_attention_kernel(const Problem p) {
   copies_wait<0>();
 }
 
-// Block (x, y) joins the pieces of two rows of the head that a border between runs cuts, if it is the
-// first border that does: the runs that hold the head's steps are contiguous, its first piece lies in
-// its run's slot 1 and the others in slot 0.  Heads that no border cuts are done.  Every thread takes four
-// columns of some of the pieces as they come, with a running maximum of its own.
+// Block y joins the pieces of the head that border y cuts, if it is the first one that does: the runs that
+// hold the head's steps are contiguous, its first piece lies in its run's slot 1 and the others in slot 0.
+// Heads that no border cuts are done.  D / 4 threads take a row, four columns each; more of them take more
+// pieces of it, four at a time, with a running maximum of their own.
 struct State {
   float4 sum;
   float denominator, top, weight_top;
-  __device__ __forceinline__ void add(const float4 &x, float other_denominator, float other_top, float other_weight_top) {
-    const float new_top = fmaxf(top, other_top), new_weight_top = fmaxf(weight_top, other_weight_top);
-    const float base = finite_or_zero(new_top), weight_base = finite_or_zero(new_weight_top);
-    const float mine = exp2_fast(weight_top - weight_base), others = exp2_fast(other_weight_top - weight_base);
-    denominator = denominator * exp2_fast(top - base) + other_denominator * exp2_fast(other_top - base);
-    sum = make_float4(sum.x * mine + x.x * others, sum.y * mine + x.y * others, sum.z * mine + x.z * others, sum.w * mine + x.w * others);
-    top = new_top;
-    weight_top = new_weight_top;
-  }
 };
+template <int COUNT> __device__ __forceinline__ void add(State &state, const float4 (&x)[COUNT], const float4 (&other)[COUNT]) {
+  float top = state.top, weight_top = state.weight_top;
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j) {
+    top = fmaxf(top, other[j].x);
+    weight_top = fmaxf(weight_top, other[j].z);
+  }
+  const float base = finite_or_zero(top), weight_base = finite_or_zero(weight_top);
+  const float mine = exp2_fast(state.weight_top - weight_base);
+  state.denominator *= exp2_fast(state.top - base);
+  state.sum = make_float4(state.sum.x * mine, state.sum.y * mine, state.sum.z * mine, state.sum.w * mine);
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j) {
+    const float shrink = exp2_fast(other[j].z - weight_base);
+    state.denominator += other[j].y * exp2_fast(other[j].x - base);
+    state.sum.x += x[j].x * shrink;
+    state.sum.y += x[j].y * shrink;
+    state.sum.z += x[j].z * shrink;
+    state.sum.w += x[j].w * shrink;
+  }
+  state.top = top;
+  state.weight_top = weight_top;
+}
 
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_attention_join_kernel(const Problem p) {
-  constexpr int kLanes = D / 4;                       // threads of a row of sums
-  constexpr int kParts = kJoinThreads / kLanes / kJoinRows;   // pieces at a time
-  __shared__ float4 part_sums[kParts][kJoinRows][kLanes];
-  __shared__ float part_states[kParts][kJoinRows][3];
+  constexpr int kLanes = D / 4, kMost = kJoinThreads / kLanes, kAtOnce = 4;
+  __shared__ float4 part_sums[kMost][kLanes];
+  __shared__ float4 part_states[kMost];
+  const int rows = min(p.group, ROWS), lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
+  const int parts = blockDim.x / (kLanes * rows), part = slot / rows, row = slot - part * rows;
+  const int block = blockIdx.x + p.abreast, run = block / p.abreast;   // blocks of the first run have no border
+  const Border *border = reinterpret_cast<const Border *>(p.partial + (int64_t)p.runs * p.abreast * 2 * ROWS * partial_floats(D)) + block;
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int run = blockIdx.y / p.abreast + 1, lane_head = blockIdx.y % p.abreast;
-  const Border border =
-      reinterpret_cast<const Border *>(p.partial + (int64_t)p.runs * p.abreast * 2 * ROWS * partial_floats(D))[run * p.abreast + lane_head];
-  if (border.step == 0) return;
-  const int64_t runs = min((int64_t)p.runs, border.total), first = border.total * run / runs - border.step;
-  if (border.total * (run - 1) / runs > first) return;
-  const int lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes, part = slot / kJoinRows, mine = slot % kJoinRows;
-  const int row = blockIdx.x * kJoinRows + mine;
-  const int kv_head = border.head / p.row_tiles, in_group = (border.head - kv_head * p.row_tiles) * ROWS + row;
-  const bool live = row < ROWS && in_group < p.group;
-  const int head = kv_head * p.group + in_group, run0 = run - 1;
+  const Border cut = *border;
+  if (cut.step == 0) return;
+  const int64_t runs = min((int64_t)p.runs, cut.total), first = cut.total * run / runs - cut.step;
+  if (cut.total * (run - 1) / runs > first) return;
   // the run of step s is the largest r with total * r / runs <= s
-  const int pieces = (int)(((first + border.steps) * runs - 1) / border.total) - run0 + 1;
+  const int pieces = (int)(((first + cut.steps) * runs - 1) / cut.total) - run + 2;
+  const int kv_head = cut.head / p.row_tiles, in_group = (cut.head - kv_head * p.row_tiles) * ROWS + row;
+  const int head = kv_head * p.group + in_group;
   State state{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -INFINITY, -INFINITY};
-  if (live) {
-#pragma unroll 4
-    for (int i = part; i < pieces; i += kParts) {
-      const float4 *from = reinterpret_cast<const float4 *>(
-          p.partial + (((int64_t)((run0 + i) * p.abreast + lane_head) * 2 + (i == 0)) * ROWS + row) * partial_floats(D));
-      const float4 x = from[lane], other = from[D / 4];
-      state.add(x, other.y, other.x, other.z);
-    }
-  }
-  part_sums[part][mine][lane] = state.sum;
-  if (lane == 0) {
-    part_states[part][mine][0] = state.denominator;
-    part_states[part][mine][1] = state.top;
-    part_states[part][mine][2] = state.weight_top;
-  }
-  __syncthreads();
-  if (part != 0 || !live) return;
+  for (int base = part; base < pieces; base += kAtOnce * parts) {
+    float4 x[kAtOnce], other[kAtOnce];
 #pragma unroll
-  for (int i = 1; i < kParts; ++i)
-    state.add(part_sums[i][mine][lane], part_states[i][mine][0], part_states[i][mine][1], part_states[i][mine][2]);
+    for (int j = 0; j < kAtOnce; ++j) {
+      const int i = base + j * parts;
+      x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+      other[j] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
+      if (i < pieces) {
+        const float4 *from = reinterpret_cast<const float4 *>(
+            p.partial + (((int64_t)(block + (i - 1) * p.abreast) * 2 + (i == 0)) * ROWS + row) * partial_floats(D));
+        x[j] = from[lane];
+        other[j] = from[D / 4];
+      }
+    }
+    add(state, x, other);
+  }
+  if (parts > 1) {
+    part_sums[slot][lane] = state.sum;
+    if (lane == 0) part_states[slot] = make_float4(state.top, state.denominator, state.weight_top, 0.0f);
+    __syncthreads();
+    if (part == 0)
+      for (int i = slot + rows; i < parts * rows; i += rows) {
+        const float4 x[1] = {part_sums[i][lane]}, other[1] = {part_states[i]};
+        add(state, x, other);
+      }
+  }
+  if (part != 0 || in_group >= p.group) return;
   const float base = finite_or_zero(state.top), unit = exp2_fast(finite_or_zero(state.weight_top) - base);
-  T *out = static_cast<T *>(p.out) + border.b * p.out_batch + head * p.out_head + 4 * lane;
+  T *out = static_cast<T *>(p.out) + cut.b * p.out_batch + head * p.out_head + 4 * lane;
   const float values[4] = {state.sum.x, state.sum.y, state.sum.z, state.sum.w};
   uint32_t packed[2];
 #pragma unroll
   for (int i = 0; i < 2; ++i)
     packed[i] = pack<T>(__fdiv_rn(values[2 * i] * unit, state.denominator), __fdiv_rn(values[2 * i + 1] * unit, state.denominator));
   *reinterpret_cast<uint2 *>(out) = make_uint2(packed[0], packed[1]);
-  if (lane == 0 && p.lse) p.lse[border.b * p.lse_batch + head * p.lse_head] = (base + log2f(state.denominator)) * kLn2;
+  if (lane == 0 && p.lse) p.lse[cut.b * p.lse_batch + head * p.lse_head] = (base + log2f(state.denominator)) * kLn2;
 }
 
 // --------------------------------------------------------------------- host
@@ -806,8 +827,12 @@ template <typename T, int STORE, int D, int ROWS> int launch(const Problem &p, c
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(((p.group < ROWS ? p.group : ROWS) + kJoinRows - 1) / kJoinRows, (p.runs - 1) * p.abreast);
-  config.blockDim = dim3(kJoinThreads);
+  // threads for all the pieces that a head has if all are alike, four to a thread, as far as a block goes
+  const int lanes = (p.group < ROWS ? p.group : ROWS) * D / 4;
+  const int64_t heads = (int64_t)p.batch * (p.kv_heads * p.row_tiles / p.abreast), want = (p.runs / heads + 2 + 3) / 4;
+  const int parts = (int)(want < kJoinThreads / lanes ? want : kJoinThreads / lanes);
+  config.gridDim = dim3((p.runs - 1) * p.abreast);
+  config.blockDim = dim3(lanes * parts);
   config.stream = stream;
   config.attrs = &early;
   config.numAttrs = 1;

@@ -66,6 +66,8 @@ struct Problem {
   float *partial;
   int batch, kv_heads, group, row_tiles, page_size, pages;
   int runs, abreast;                             // blocks = runs * abreast
+  uint32_t page_magic, page_shift, runs_magic;   // for divisions by page_size and by runs
+  double inverse_runs;
   int64_t most_keys;                             // slots that a row of the table names
   float scale_log2e;
   int *status;
@@ -83,18 +85,16 @@ template <int STORE, int D, int ROWS> struct Shape {
   static constexpr int kScaleBytes = STORE == cache::kNative ? 0 : 2 * kKeys * 4;
   static constexpr int kStageBytes = 2 * kTileBytes + kScaleBytes;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-  static constexpr int kSmemBytes = kRingBytes + kWarps * ROWS * 3 * 4;
+  static constexpr int kSmemBytes = kRingBytes + kWarps * ROWS * 16 + ROWS * 4;
   static_assert(ROWS * D * 4 <= kStageBytes, "a warp's sums fit the stage that it has just used");
 };
 constexpr int partial_floats(int columns) { return columns + 4; }   // sums, m, l, M, unused
 
 // What a run begins with, for the kernel that joins: (sequence, head tile) and how many of its steps lie
-// before the run.  (What follows from it is worked out there: 64-bit divisions here cost the main loop
-// registers and the call 5%.)
+// before the run; and what a run holds.
 struct Border {
-  int64_t total;
-  int b, head, step, steps;
-  int64_t unused;
+  int64_t each;
+  int rest, b, head, step, steps, unused;
 };
 static_assert(sizeof(Border) == 32, "two vectors");
 
@@ -203,6 +203,12 @@ template <int THREADS> __device__ __forceinline__ int64_t block_scan(int64_t v, 
   return total;
 }
 
+// The first step of a run: floor(total * run / runs) for total = each * runs + rest, by parts that need no
+// 64-bit division: rest * run is below 2^18, where the rounded-up reciprocal is exact.
+__device__ __forceinline__ int64_t run_begin(const Problem &p, int64_t each, int rest, int run) {
+  return each * run + __umulhi((uint32_t)(rest * run), p.runs_magic);
+}
+
 struct Place {            // where in the sequence of steps a warp is
   int b, head, step, steps, length;
   int64_t left;
@@ -253,7 +259,15 @@ paged_attention_kernel(const Problem p) {
     total += block_scan<kBlock>(steps_here, before, scan_scratch);
   }
   total *= head_tiles;
-  const int64_t runs = min((int64_t)p.runs, total);   // none is empty, which the join relies on
+  // runs of each or each + 1 steps; none is empty, which the join relies on
+  int64_t each = 1;
+  int rest = 0;
+  if (total >= p.runs) {
+    each = (int64_t)((double)total * p.inverse_runs);
+    rest = (int)(total - each * p.runs);
+    if (rest < 0) { --each; rest += p.runs; }
+    if (rest >= p.runs) { ++each; rest -= p.runs; }
+  }
   Border *border = reinterpret_cast<Border *>(p.partial + (int64_t)gridDim.x * 2 * ROWS * partial_floats(D)) + blockIdx.x;
   // sequences that have not begun
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
@@ -264,11 +278,11 @@ paged_attention_kernel(const Problem p) {
     for (int head = threadIdx.x; p.lse && head < p.kv_heads * p.group; head += kBlock)
       p.lse[b * p.lse_batch + head * p.lse_head] = -INFINITY;
   }
-  if (run >= runs) {
+  if (run >= min((int64_t)p.runs, total)) {
     if (threadIdx.x == 0) border->step = 0;
     return;
   }
-  const int64_t begin = total * run / runs, end = total * (run + 1) / runs;
+  const int64_t begin = run_begin(p, each, rest, run), end = run_begin(p, each, rest, run + 1);
   int64_t carried = 0;
   for (int base = 0; base < p.batch; base += kBlock) {
     const int b = base + threadIdx.x;
@@ -290,17 +304,18 @@ paged_attention_kernel(const Problem p) {
   load.b = start_b;
   load.length = length_of(p, load.b);
   load.steps = (load.length + S::kStep - 1) / S::kStep;
-  load.head = (int)(start_rest / load.steps);
+  load.head = start_rest >> 32 ? (int)(start_rest / load.steps) : (int)((uint32_t)start_rest / (uint32_t)load.steps);
   load.step = (int)(start_rest - (int64_t)load.head * load.steps);
   load.head = load.head * p.abreast + lane_head;
   load.left = end - begin;
   Place use = load;       // what the next products take
-  if (threadIdx.x == 0) *border = Border{total, load.b, load.head, load.step, load.steps, 0};
+  if (threadIdx.x == 0) *border = Border{each, rest, load.b, load.head, load.step, load.steps, 0};
 
   // ---- copies: lane r looks row r of the tile up; a row's 16-byte pieces go to neighbouring lanes
   unsigned char *ring = dynamic_smem + warp * S::kStages * S::kStageBytes;
   const uint32_t ring_address = shared_address(ring);
-  float *stats = reinterpret_cast<float *>(dynamic_smem + S::kRingBytes);
+  float4 *stats = reinterpret_cast<float4 *>(dynamic_smem + S::kRingBytes);   // m, l, weight_max of the warps' rows
+  float *units = reinterpret_cast<float *>(stats + kWarps * ROWS);
   int entry = -1, offset = 0;
   bool inside = false;
   auto look_up = [&]() {
@@ -309,7 +324,8 @@ paged_attention_kernel(const Problem p) {
     const int64_t key = (int64_t)(load.step * kWarps + warp) * S::kKeys + lane;
     inside = lane < S::kKeys && key < load.length;
     if (inside) {
-      const uint32_t column = (uint32_t)key / (uint32_t)p.page_size;
+      // key / page_size: key is below 2^31, so the sum does not carry
+      const uint32_t column = (__umulhi((uint32_t)key, p.page_magic) + (uint32_t)key) >> p.page_shift;
       offset = (int)((uint32_t)key - column * (uint32_t)p.page_size);
       entry = __ldg(p.table + load.b * p.table_row + column * p.table_column);
     }
@@ -596,9 +612,18 @@ paged_attention_kernel(const Problem p) {
     }
   };
 
-  // ---- the end of a piece: every warp leaves its sums in the stage that it used last, then the block
-  // adds them up
+  // ---- the end of a piece.  The warps exchange their maxima, bring their sums to the common one and
+  // leave them in the stage that they used last; the block adds them up, four columns a thread.
   auto finish = [&](const Place &at, bool whole, int stage) {
+#pragma unroll
+    for (int h = 0; h < kHeads; ++h)
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+#pragma unroll
+        for (int other = 4; other < 32; other <<= 1) l[h][j] += __shfl_xor_sync(0xffffffffu, l[h][j], other);
+        if (g == 0) stats[warp * ROWS + h * 8 + 2 * c + j] = make_float4(m[h][j], l[h][j], weight_max[h][j], 0.0f);
+      }
+    __syncthreads();
     float *mine = reinterpret_cast<float *>(ring + stage * S::kStageBytes);
     // (row, column) of a warp's sums: eight lanes' columns and four lanes' rows all on different banks
     auto spot = [](int row, int column) { return row * D + (column ^ (row >> 1 & 3) * 8); };
@@ -607,51 +632,58 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int row = h * 8 + 2 * c + j;
+        float weight_top = weight_max[h][j];
 #pragma unroll
-        for (int other = 4; other < 32; other <<= 1) l[h][j] += __shfl_xor_sync(0xffffffffu, l[h][j], other);
-        if (g == 0) {
-          float *state = stats + (warp * ROWS + row) * 3;
-          state[0] = m[h][j];
-          state[1] = l[h][j];
-          state[2] = weight_max[h][j];
-        }
+        for (int w = 1; w < kWarps; ++w) weight_top = fmaxf(weight_top, stats[(warp ^ w) * ROWS + row].z);
+        const float shrink = exp2_fast(weight_max[h][j] - finite_or_zero(weight_top));
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
-          for (int k = 0; k < 2; ++k) mine[spot(row, 16 * i + (kCodes ? 2 * g + k : 8 * k + g))] = sums[i][h][2 * k + j];
+          for (int k = 0; k < 2; ++k) mine[spot(row, 16 * i + (kCodes ? 2 * g + k : 8 * k + g))] = sums[i][h][2 * k + j] * shrink;
       }
-    __syncthreads();
     const int kv_head = at.head / p.row_tiles, row0 = (at.head - kv_head * p.row_tiles) * ROWS;
-    const int rows = min(ROWS, p.group - row0);
-    const int column = threadIdx.x % D;
-    for (int row = threadIdx.x / D; row < rows; row += kBlock / D) {
-      float top = -INFINITY, weight_top = -INFINITY, denominator = 0.0f, sum = 0.0f;
+    const int rows = min(ROWS, p.group - row0), head0 = kv_head * p.group + row0;
+    // slot 1 if the piece begins its head (only a run's last piece may then be unfinished), else slot 0
+    float *to = p.partial + ((int64_t)blockIdx.x * 2 + (piece_first == 0)) * ROWS * partial_floats(D);
+    if (threadIdx.x < rows) {
+      const int row = threadIdx.x;
+      float4 state[kWarps];
+      float top = -INFINITY, weight_top = -INFINITY, denominator = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        top = fmaxf(top, stats[(w * ROWS + row) * 3]);
-        weight_top = fmaxf(weight_top, stats[(w * ROWS + row) * 3 + 2]);
+        state[w] = stats[w * ROWS + row];
+        top = fmaxf(top, state[w].x);
+        weight_top = fmaxf(weight_top, state[w].z);
       }
-      const float base = finite_or_zero(top), weight_base = finite_or_zero(weight_top);
+      const float base = finite_or_zero(top);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const float *state = stats + (w * ROWS + row) * 3;
-        const float *from = reinterpret_cast<const float *>(dynamic_smem + (w * S::kStages + stage) * S::kStageBytes);
-        denominator += state[1] * exp2_fast(state[0] - base);
-        sum += from[spot(row, column)] * exp2_fast(state[2] - weight_base);
-      }
-      const int head = kv_head * p.group + row0 + row;
+      for (int w = 0; w < kWarps; ++w) denominator += state[w].y * exp2_fast(state[w].x - base);
+      units[row] = __fdiv_rn(kCodes ? exp2_fast(finite_or_zero(weight_top) - base) : 1.0f, denominator);
       if (whole) {
-        const float unit = kCodes ? exp2_fast(weight_base - base) : 1.0f;
-        static_cast<T *>(p.out)[at.b * p.out_batch + head * p.out_head + column] = Element<T>::narrow(__fdiv_rn(sum * unit, denominator));
-        if (column == 0 && p.lse) p.lse[at.b * p.lse_batch + head * p.lse_head] = (base + log2f(denominator)) * kLn2;
+        if (p.lse) p.lse[at.b * p.lse_batch + (head0 + row) * p.lse_head] = (base + log2f(denominator)) * kLn2;
       } else {
-        // slot 1 if the piece begins its head (only a run's last piece may then be unfinished), else slot 0
-        float *to = p.partial + (((int64_t)blockIdx.x * 2 + (piece_first == 0)) * ROWS + row) * partial_floats(D);
-        to[column] = sum;
-        if (column == 0) *reinterpret_cast<float4 *>(to + D) = make_float4(top, denominator, weight_top, 0.0f);
+        *reinterpret_cast<float4 *>(to + row * partial_floats(D) + D) = make_float4(top, denominator, weight_top, 0.0f);
       }
     }
-    __syncthreads();   // the stage and `stats` are free again
+    __syncthreads();
+    for (int index = threadIdx.x; index < rows * (D / 4); index += kBlock) {
+      const int row = index / (D / 4), column = index % (D / 4) * 4;
+      float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float4 x = *reinterpret_cast<const float4 *>(
+            reinterpret_cast<const float *>(dynamic_smem + (w * S::kStages + stage) * S::kStageBytes) + spot(row, column));
+        sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+      }
+      if (whole) {
+        const float unit = units[row];
+        *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at.b * p.out_batch + (head0 + row) * p.out_head + column) =
+            make_uint2(pack<T>(sum.x * unit, sum.y * unit), pack<T>(sum.z * unit, sum.w * unit));
+      } else {
+        *reinterpret_cast<float4 *>(to + row * partial_floats(D) + column) = sum;
+      }
+    }
+    __syncthreads();   // the stage, `stats` and `units` are free again
   };
 
   // ---- the run
@@ -734,10 +766,11 @@ paged_attention_join_kernel(const Problem p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Border cut = *border;
   if (cut.step == 0) return;
-  const int64_t runs = min((int64_t)p.runs, cut.total), first = cut.total * run / runs - cut.step;
-  if (cut.total * (run - 1) / runs > first) return;
-  // the run of step s is the largest r with total * r / runs <= s
-  const int pieces = (int)(((first + cut.steps) * runs - 1) / cut.total) - run + 2;
+  const int64_t first = run_begin(p, cut.each, cut.rest, run) - cut.step;
+  if (run_begin(p, cut.each, cut.rest, run - 1) > first) return;
+  // the head's later runs are those that begin before its end: as many as whole runs fit, or some more
+  int pieces = 2 + (cut.each < cut.steps ? (cut.steps - cut.step - 1) / ((int)cut.each + 1) : 0);
+  while (run_begin(p, cut.each, cut.rest, run - 1 + pieces) < first + cut.steps) ++pieces;
   const int kv_head = cut.head / p.row_tiles, in_group = (cut.head - kv_head * p.row_tiles) * ROWS + row;
   const int head = kv_head * p.group + in_group;
   State state{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -INFINITY, -INFINITY};
@@ -937,7 +970,12 @@ extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float s
   p.row_tiles = (int)((group + rows_of(group) - 1) / rows_of(group));
   p.page_size = (int)k.d2; p.pages = (int)k.d0;
   p.runs = (int)split.runs; p.abreast = (int)split.abreast;
+  p.inverse_runs = 1.0 / (double)split.runs;
+  p.runs_magic = (uint32_t)(((int64_t(1) << 32) + split.runs - 1) / split.runs - (split.runs == 1));
   p.most_keys = most_keys;
+  // 2^shift >= page_size; (magic + 2^32) / 2^(32 + shift) is 1 / page_size to within what 31-bit numbers show
+  while ((int64_t(1) << p.page_shift) < k.d2) ++p.page_shift;
+  if (k.d2) p.page_magic = (uint32_t)(((int64_t(1) << 32) * ((int64_t(1) << p.page_shift) - k.d2)) / k.d2 + 1);
   p.scale_log2e = scale * kLog2e;
   p.status = static_cast<int *>(const_cast<void *>(workspace.data));
   cudaStream_t s = static_cast<cudaStream_t>(stream);

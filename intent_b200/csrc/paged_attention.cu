@@ -45,7 +45,7 @@ using heads::View4;
 
 constexpr int kWarps = 4;
 constexpr int kBlock = kWarps * 32;
-constexpr int kJoinThreads = 1024;
+constexpr int kJoinThreads = 512, kJoinAtOnce = 8;
 constexpr float kLn2 = 0.6931471805599453f, kLog2e = 1.4426950408889634f;
 
 struct Problem {
@@ -724,7 +724,7 @@ paged_attention_kernel(const Problem p) {
 // Block y joins the pieces of the head that border y cuts, if it is the first one that does: the runs that
 // hold the head's steps are contiguous, its first piece lies in its run's slot 1 and the others in slot 0.
 // Heads that no border cuts are done.  D / 4 threads take a row, four columns each; more of them take more
-// pieces of it, four at a time, with a running maximum of their own.
+// pieces of it, eight at a time, with a running maximum of their own.
 struct State {
   float4 sum;
   float denominator, top, weight_top;
@@ -756,13 +756,15 @@ template <int COUNT> __device__ __forceinline__ void add(State &state, const flo
 template <typename T, int D, int ROWS>
 __global__ void __launch_bounds__(kJoinThreads)
 paged_attention_join_kernel(const Problem p) {
-  constexpr int kLanes = D / 4, kMost = kJoinThreads / kLanes, kAtOnce = 4;
+  constexpr int kLanes = D / 4, kMost = kJoinThreads / kLanes, kAtOnce = kJoinAtOnce;
   __shared__ float4 part_sums[kMost][kLanes];
   __shared__ float4 part_states[kMost];
   const int rows = min(p.group, ROWS), lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
   const int parts = blockDim.x / (kLanes * rows), part = slot / rows, row = slot - part * rows;
   const int block = blockIdx.x + p.abreast, run = block / p.abreast;   // blocks of the first run have no border
   const Border *border = reinterpret_cast<const Border *>(p.partial + (int64_t)p.runs * p.abreast * 2 * ROWS * partial_floats(D)) + block;
+  // What follows is short on purpose: every block meets it cold, and instructions that come from L2 cost more
+  // than what they do.
   asm volatile("griddepcontrol.wait;" ::: "memory");
   const Border cut = *border;
   if (cut.step == 0) return;
@@ -771,22 +773,22 @@ paged_attention_join_kernel(const Problem p) {
   // the head's later runs are those that begin before its end: as many as whole runs fit, or some more
   int pieces = 2 + (cut.each < cut.steps ? (cut.steps - cut.step - 1) / ((int)cut.each + 1) : 0);
   while (run_begin(p, cut.each, cut.rest, run - 1 + pieces) < first + cut.steps) ++pieces;
-  const int kv_head = cut.head / p.row_tiles, in_group = (cut.head - kv_head * p.row_tiles) * ROWS + row;
-  const int head = kv_head * p.group + in_group;
   State state{make_float4(0.0f, 0.0f, 0.0f, 0.0f), 0.0f, -INFINITY, -INFINITY};
-  for (int base = part; base < pieces; base += kAtOnce * parts) {
+  const int64_t pitch = (int64_t)p.abreast * 2 * ROWS * partial_floats(D);      // from a run's pieces to the next one's
+  const float *origin = p.partial + ((int64_t)(block - p.abreast) * 2 * ROWS + row) * partial_floats(D);
+#pragma unroll 1
+  for (int i = part; i < pieces; i += kAtOnce * parts) {
     float4 x[kAtOnce], other[kAtOnce];
+    const float *from = origin + i * pitch + (i == 0 ? ROWS * partial_floats(D) : 0);
 #pragma unroll
     for (int j = 0; j < kAtOnce; ++j) {
-      const int i = base + j * parts;
       x[j] = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
       other[j] = make_float4(-INFINITY, 0.0f, -INFINITY, 0.0f);
-      if (i < pieces) {
-        const float4 *from = reinterpret_cast<const float4 *>(
-            p.partial + (((int64_t)(block + (i - 1) * p.abreast) * 2 + (i == 0)) * ROWS + row) * partial_floats(D));
-        x[j] = from[lane];
-        other[j] = from[D / 4];
+      if (i + j * parts < pieces) {
+        x[j] = reinterpret_cast<const float4 *>(from)[lane];
+        other[j] = reinterpret_cast<const float4 *>(from)[D / 4];
       }
+      from = origin + (i + (j + 1) * parts) * pitch;
     }
     add(state, x, other);
   }
@@ -795,21 +797,19 @@ paged_attention_join_kernel(const Problem p) {
     if (lane == 0) part_states[slot] = make_float4(state.top, state.denominator, state.weight_top, 0.0f);
     __syncthreads();
     if (part == 0)
+#pragma unroll 1
       for (int i = slot + rows; i < parts * rows; i += rows) {
         const float4 x[1] = {part_sums[i][lane]}, other[1] = {part_states[i]};
         add(state, x, other);
       }
   }
+  const int kv_head = cut.head / p.row_tiles, in_group = (cut.head - kv_head * p.row_tiles) * ROWS + row;
+  const int head = kv_head * p.group + in_group;
   if (part != 0 || in_group >= p.group) return;
-  const float base = finite_or_zero(state.top), unit = exp2_fast(finite_or_zero(state.weight_top) - base);
+  const float base = finite_or_zero(state.top), unit = __fdividef(exp2_fast(finite_or_zero(state.weight_top) - base), state.denominator);
   T *out = static_cast<T *>(p.out) + cut.b * p.out_batch + head * p.out_head + 4 * lane;
-  const float values[4] = {state.sum.x, state.sum.y, state.sum.z, state.sum.w};
-  uint32_t packed[2];
-#pragma unroll
-  for (int i = 0; i < 2; ++i)
-    packed[i] = pack<T>(__fdiv_rn(values[2 * i] * unit, state.denominator), __fdiv_rn(values[2 * i + 1] * unit, state.denominator));
-  *reinterpret_cast<uint2 *>(out) = make_uint2(packed[0], packed[1]);
-  if (lane == 0 && p.lse) p.lse[cut.b * p.lse_batch + head * p.lse_head] = (base + log2f(state.denominator)) * kLn2;
+  *reinterpret_cast<uint2 *>(out) = make_uint2(pack<T>(state.sum.x * unit, state.sum.y * unit), pack<T>(state.sum.z * unit, state.sum.w * unit));
+  if (lane == 0 && p.lse) p.lse[cut.b * p.lse_batch + head * p.lse_head] = (base + __log2f(state.denominator)) * kLn2;
 }
 
 // --------------------------------------------------------------------- host
@@ -860,9 +860,9 @@ template <typename T, int STORE, int D, int ROWS> int launch(const Problem &p, c
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  // threads for all the pieces that a head has if all are alike, four to a thread, as far as a block goes
+  // threads for all the pieces that a head has if all are alike, eight to a thread, as far as a block goes
   const int lanes = (p.group < ROWS ? p.group : ROWS) * D / 4;
-  const int64_t heads = (int64_t)p.batch * (p.kv_heads * p.row_tiles / p.abreast), want = (p.runs / heads + 2 + 3) / 4;
+  const int64_t heads = (int64_t)p.batch * (p.kv_heads * p.row_tiles / p.abreast), want = (p.runs / heads + 2 + kJoinAtOnce - 1) / kJoinAtOnce;
   const int parts = (int)(want < kJoinThreads / lanes ? want : kJoinThreads / lanes);
   config.gridDim = dim3((p.runs - 1) * p.abreast);
   config.blockDim = dim3(lanes * parts);

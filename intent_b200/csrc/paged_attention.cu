@@ -24,7 +24,8 @@
 // models fill the products without padding; tcgen05's smallest tiles would pad them 2 to 16 times and
 // take the weights through shared memory, to speed up what is not the time.  The weights enter the
 // second product as the sum of two halves of 16 bits, so that they count with 22 (f16) or 16 (bf16) bits
-// and only the result is rounded.
+// and only the result is rounded.  Up to four query heads stand in the columns twice: the first four carry
+// the weights' first halves and the other four the second ones, in one product instead of two.
 //
 // 8-bit rows.  Codes become f16 exactly on their way into the products.  The query is scaled by a
 // power of two per row to fit f16; a key's scale multiplies its score.  A value's scale is folded into
@@ -80,13 +81,14 @@ template <int STORE, int D, int ROWS> struct Shape {
   static constexpr int kRowBytes = D * kBytes;
   static constexpr int kChunks = kRowBytes / 16;
   static constexpr int kTileBytes = kKeys * kRowBytes;
-  static constexpr int kBlocksPerSm = ROWS == 8 ? 3 : 2;            // 168 or 255 registers
-  static constexpr int kStages = (ROWS == 8 ? 2 : 3) * (128 / D);   // about 200 KB of an SM's shared memory
+  static constexpr int kColumns = ROWS < 8 ? 8 : ROWS;              // of the products; a head's twice if ROWS is 4
+  static constexpr int kBlocksPerSm = ROWS <= 8 ? 3 : 2;            // 168 or 255 registers
+  static constexpr int kStages = (ROWS <= 8 ? 2 : 3) * (128 / D);   // about 200 KB of an SM's shared memory
   static constexpr int kScaleBytes = STORE == cache::kNative ? 0 : 2 * kKeys * 4;
   static constexpr int kStageBytes = 2 * kTileBytes + kScaleBytes;
   static constexpr int kRingBytes = kWarps * kStages * kStageBytes;
-  static constexpr int kSmemBytes = kRingBytes + kWarps * ROWS * 16 + ROWS * 4;
-  static_assert(ROWS * D * 4 <= kStageBytes, "a warp's sums fit the stage that it has just used");
+  static constexpr int kSmemBytes = kRingBytes + kWarps * kColumns * 16 + ROWS * 4;
+  static_assert(kColumns * D * 4 <= kStageBytes, "a warp's sums fit the stage that it has just used");
 };
 constexpr int partial_floats(int columns) { return columns + 4; }   // sums, m, l, M, unused
 
@@ -237,7 +239,8 @@ paged_attention_kernel(const Problem p) {
   using S = Shape<STORE, D, ROWS>;
   using M = typename std::conditional<STORE == cache::kNative, T, __half>::type;   // type of the products
   constexpr bool kCodes = STORE != cache::kNative;
-  constexpr int kHeads = ROWS / 8, kTiles = S::kKeys / 16;   // tiles of 8 query heads and of 16 keys
+  constexpr int kHeads = S::kColumns / 8, kTiles = S::kKeys / 16;   // tiles of 8 columns (query heads) and of 16 keys
+  constexpr bool kTwice = ROWS == 4;
   extern __shared__ __align__(128) unsigned char dynamic_smem[];
   __shared__ int64_t scan_scratch[kWarps];
   __shared__ int64_t start_rest;
@@ -315,7 +318,7 @@ paged_attention_kernel(const Problem p) {
   unsigned char *ring = dynamic_smem + warp * S::kStages * S::kStageBytes;
   const uint32_t ring_address = shared_address(ring);
   float4 *stats = reinterpret_cast<float4 *>(dynamic_smem + S::kRingBytes);   // m, l, weight_max of the warps' rows
-  float *units = reinterpret_cast<float *>(stats + kWarps * ROWS);
+  float *units = reinterpret_cast<float *>(stats + kWarps * S::kColumns);
   int entry = -1, offset = 0;
   bool inside = false;
   auto look_up = [&]() {
@@ -402,7 +405,7 @@ paged_attention_kernel(const Problem p) {
     const int kv_head = at.head / p.row_tiles, row0 = (at.head - kv_head * p.row_tiles) * ROWS;
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
-      const int row = row0 + h * 8 + g;
+      const int row = row0 + (kTwice ? g & 3 : h * 8 + g);
       const T *source = static_cast<const T *>(p.q) + at.b * p.q_batch + (kv_head * p.group + min(row, p.group - 1)) * p.q_head;
 #pragma unroll
       for (int i = 0; i < D / 16; ++i) {
@@ -503,7 +506,6 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
       for (int k = 0; k < 2; ++k) {
         const int key = 16 * t + 8 * k + g;
-        const bool live = mask >> key & 1;
         float key_scale = 1.0f;
         if constexpr (kCodes) {
           key_scale = scales[key];
@@ -512,8 +514,17 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
         for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-          for (int j = 0; j < 2; ++j) s[t][h][2 * k + j] = live ? s[t][h][2 * k + j] * (head_scale[h][j] * key_scale) : -INFINITY;
+          for (int j = 0; j < 2; ++j) s[t][h][2 * k + j] *= head_scale[h][j] * key_scale;
       }
+    if (mask != kFull) {
+#pragma unroll
+      for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+          if (!(mask >> (16 * t + 8 * k + g) & 1))
+#pragma unroll
+            for (int h = 0; h < kHeads; ++h) s[t][h][2 * k] = s[t][h][2 * k + 1] = -INFINITY;
+    }
     // The bases m and weight_max move only when a score passes them by more than 8 (log2 units): until then
     // weights reach 2^8, well inside every type here.
     bool grown = false;
@@ -572,9 +583,9 @@ paged_attention_kernel(const Problem p) {
             // log2 of a masked key's zero scale is -infinity: its weight is 0
             if constexpr (kCodes) w[j] = exp2_fast(s[t][h][2 * k + j] + log_scale[t][k] - weight_base[j]);
           }
-          const uint32_t pair = pack<M>(w[0], w[1]);
-          high[t][h][k] = transposed(pair);
-          rest[t][h][k] = transposed(pack<M>(w[0] - unpack<M>(pair, 0), w[1] - unpack<M>(pair, 1)));
+          const uint32_t pair = pack<M>(w[0], w[1]), left = pack<M>(w[0] - unpack<M>(pair, 0), w[1] - unpack<M>(pair, 1));
+          high[t][h][k] = transposed(kTwice && c >= 2 ? left : pair);
+          if constexpr (!kTwice) rest[t][h][k] = transposed(left);
         }
     }
     // sums += values (transposed) . weights
@@ -588,8 +599,10 @@ paged_attention_kernel(const Problem p) {
         if constexpr (!kCodes) {
 #pragma unroll
           for (int h = 0; h < kHeads; ++h) multiply<M>(sums[i][h], r[0], r[1], r[2], r[3], high[t][h][0], high[t][h][1]);
+          if constexpr (!kTwice) {
 #pragma unroll
-          for (int h = 0; h < kHeads; ++h) multiply<M>(sums[i][h], r[0], r[1], r[2], r[3], rest[t][h][0], rest[t][h][1]);
+            for (int h = 0; h < kHeads; ++h) multiply<M>(sums[i][h], r[0], r[1], r[2], r[3], rest[t][h][0], rest[t][h][1]);
+          }
         } else {                      // a 16-bit unit holds two neighbouring columns: even ones are rows 0 .. 7, odd ones 8 .. 15
           uint32_t v[2][4];
 #pragma unroll
@@ -602,11 +615,13 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
             for (int j = 0; j < 2; ++j)
               multiply<M>(sums[2 * i + j][h], v[j][0], v[j][1], v[j][2], v[j][3], high[t][h][0], high[t][h][1]);
+          if constexpr (!kTwice) {
 #pragma unroll
-          for (int h = 0; h < kHeads; ++h)
+            for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-            for (int j = 0; j < 2; ++j)
-              multiply<M>(sums[2 * i + j][h], v[j][0], v[j][1], v[j][2], v[j][3], rest[t][h][0], rest[t][h][1]);
+              for (int j = 0; j < 2; ++j)
+                multiply<M>(sums[2 * i + j][h], v[j][0], v[j][1], v[j][2], v[j][3], rest[t][h][0], rest[t][h][1]);
+          }
         }
       }
     }
@@ -621,7 +636,7 @@ paged_attention_kernel(const Problem p) {
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int other = 4; other < 32; other <<= 1) l[h][j] += __shfl_xor_sync(0xffffffffu, l[h][j], other);
-        if (g == 0) stats[warp * ROWS + h * 8 + 2 * c + j] = make_float4(m[h][j], l[h][j], weight_max[h][j], 0.0f);
+        if (g == 0) stats[warp * S::kColumns + h * 8 + 2 * c + j] = make_float4(m[h][j], l[h][j], weight_max[h][j], 0.0f);
       }
     __syncthreads();
     float *mine = reinterpret_cast<float *>(ring + stage * S::kStageBytes);
@@ -634,7 +649,7 @@ paged_attention_kernel(const Problem p) {
         const int row = h * 8 + 2 * c + j;
         float weight_top = weight_max[h][j];
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) weight_top = fmaxf(weight_top, stats[(warp ^ w) * ROWS + row].z);
+        for (int w = 1; w < kWarps; ++w) weight_top = fmaxf(weight_top, stats[(warp ^ w) * S::kColumns + row].z);
         const float shrink = exp2_fast(weight_max[h][j] - finite_or_zero(weight_top));
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
@@ -651,7 +666,7 @@ paged_attention_kernel(const Problem p) {
       float top = -INFINITY, weight_top = -INFINITY, denominator = 0.0f;
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        state[w] = stats[w * ROWS + row];
+        state[w] = stats[w * S::kColumns + row];
         top = fmaxf(top, state[w].x);
         weight_top = fmaxf(weight_top, state[w].z);
       }
@@ -671,9 +686,12 @@ paged_attention_kernel(const Problem p) {
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float4 x = *reinterpret_cast<const float4 *>(
-            reinterpret_cast<const float *>(dynamic_smem + (w * S::kStages + stage) * S::kStageBytes) + spot(row, column));
-        sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+        const float *from = reinterpret_cast<const float *>(dynamic_smem + (w * S::kStages + stage) * S::kStageBytes);
+#pragma unroll
+        for (int half = 0; half < (kTwice ? 2 : 1); ++half) {
+          const float4 x = *reinterpret_cast<const float4 *>(from + spot(row + 4 * half, column));
+          sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
+        }
       }
       if (whole) {
         const float unit = units[row];
@@ -813,7 +831,7 @@ paged_attention_join_kernel(const Problem p) {
 }
 
 // --------------------------------------------------------------------- host
-int rows_of(int64_t group) { return group <= 8 ? 8 : 16; }
+int rows_of(int64_t group) { return group <= 4 ? 4 : group <= 8 ? 8 : 16; }
 int step_of(int store) {
   return store == B200_I8 || store == B200_E4M3 ? Shape<cache::kInt8, 128, 8>::kStep : Shape<cache::kNative, 128, 8>::kStep;
 }
@@ -836,7 +854,7 @@ struct Split {
 Split split_of(int64_t batch, int64_t kv_heads, int64_t group, int64_t most_keys, int store) {
   const int64_t rows = rows_of(group), tiles = kv_heads * ((group + rows - 1) / rows), step = step_of(store);
   const int64_t each = (most_keys + step - 1) / step;
-  const int64_t resident = (int64_t)(rows == 8 ? Shape<cache::kNative, 128, 8>::kBlocksPerSm : Shape<cache::kNative, 128, 16>::kBlocksPerSm) * sm_count();
+  const int64_t resident = (int64_t)(rows <= 8 ? Shape<cache::kNative, 128, 8>::kBlocksPerSm : Shape<cache::kNative, 128, 16>::kBlocksPerSm) * sm_count();
   if (batch == 0 || tiles == 0 || each == 0) return {1, 1};
   const int64_t abreast = heads_abreast(tiles, resident), most = resident / abreast, groups = tiles / abreast;
   if (batch >= most || groups >= most || each >= most || batch * groups >= most) return {most, abreast};
@@ -873,6 +891,7 @@ template <typename T, int STORE, int D, int ROWS> int launch(const Problem &p, c
   return B200_OK;
 }
 template <typename T, int STORE, int D> int by_rows(const Problem &p, cudaStream_t stream) {
+  if (p.group <= 4) return launch<T, STORE, D, 4>(p, stream);
   return p.group <= 8 ? launch<T, STORE, D, 8>(p, stream) : launch<T, STORE, D, 16>(p, stream);
 }
 template <typename T, int STORE> int by_columns(const Problem &p, int columns, cudaStream_t stream) {

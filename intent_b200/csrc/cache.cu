@@ -73,6 +73,7 @@ constexpr int kWriteBlocks = 6, kReadBlocks = 8, kNativeBlocks = 6;
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads, kWriteBlocks)
 cache_write_codes_kernel(Rows rows, Pages pages, Extents x) {
+  heads::await_stream();
   const int e = threadIdx.x % LANES;
   const uint32_t unit = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const int token = (int)(unit / (uint32_t)x.heads), head = (int)(unit - (uint32_t)token * x.heads);
@@ -120,6 +121,7 @@ cache_write_codes_kernel(Rows rows, Pages pages, Extents x) {
 template <typename T, int LANES>
 __global__ void __launch_bounds__(kThreads, kReadBlocks)
 cache_read_codes_kernel(Rows rows, Pages pages, Extents x) {
+  heads::await_stream();
   const int e = threadIdx.x % LANES;
   const uint32_t unit = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const int token = (int)(unit / (uint32_t)x.heads), head = (int)(unit - (uint32_t)token * x.heads);
@@ -156,6 +158,7 @@ cache_read_codes_kernel(Rows rows, Pages pages, Extents x) {
 template <typename T, int LANES, bool WRITE>
 __global__ void __launch_bounds__(kThreads, kNativeBlocks)
 cache_copy_kernel(Rows rows, Pages pages, Extents x) {
+  heads::await_stream();
   const int e = threadIdx.x % LANES;
   const uint32_t unit = blockIdx.x * (kThreads / LANES) + threadIdx.x / LANES;
   const int token = (int)(unit / (uint32_t)x.heads), head = (int)(unit - (uint32_t)token * x.heads);
@@ -271,15 +274,10 @@ template <typename T, int LANES> int launch(const Arguments &a, bool write, cuda
   pack(a, rows, pages, x);
   const int64_t units = (int64_t)x.tokens * x.heads, per_block = kThreads / LANES;
   const unsigned blocks = (unsigned)((units + per_block - 1) / per_block);
-  if (x.store == cache::kNative && write)
-    cache_copy_kernel<T, LANES, true><<<blocks, kThreads, 0, stream>>>(rows, pages, x);
-  else if (x.store == cache::kNative)
-    cache_copy_kernel<T, LANES, false><<<blocks, kThreads, 0, stream>>>(rows, pages, x);
-  else if (write)
-    cache_write_codes_kernel<T, LANES><<<blocks, kThreads, 0, stream>>>(rows, pages, x);
-  else
-    cache_read_codes_kernel<T, LANES><<<blocks, kThreads, 0, stream>>>(rows, pages, x);
-  B200_CUDA_TRY(cudaGetLastError());
+  const auto kernel = x.store == cache::kNative ? (write ? cache_copy_kernel<T, LANES, true> : cache_copy_kernel<T, LANES, false>)
+                      : write                   ? cache_write_codes_kernel<T, LANES>
+                                                : cache_read_codes_kernel<T, LANES>;
+  B200_CUDA_TRY(heads::launch_early(kernel, blocks, kThreads, 0, stream, rows, pages, x));
   return B200_OK;
 }
 

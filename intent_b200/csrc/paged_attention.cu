@@ -245,7 +245,7 @@ paged_attention_kernel(const Problem p) {
   __shared__ int64_t scan_scratch[kWarps];
   __shared__ int64_t start_rest;
   __shared__ int start_b;
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  heads::await_stream();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int g = lane >> 2, c = lane & 3;
 
@@ -783,7 +783,7 @@ paged_attention_join_kernel(const Problem p) {
   const Border *border = reinterpret_cast<const Border *>(p.partial + (int64_t)p.runs * p.abreast * 2 * ROWS * partial_floats(D)) + block;
   // What follows is short on purpose: every block meets it cold, and instructions that come from L2 cost more
   // than what they do.
-  asm volatile("griddepcontrol.wait;" ::: "memory");
+  heads::await_stream();
   const Border cut = *border;
   if (cut.step == 0) return;
   const int64_t first = run_begin(p, cut.each, cut.rest, run) - cut.step;
@@ -870,24 +870,13 @@ template <typename T, int STORE, int D, int ROWS> int launch(const Problem &p, c
   const auto kernel = paged_attention_kernel<T, STORE, D, ROWS>;
   const size_t bytes = Shape<STORE, D, ROWS>::kSmemBytes;
   B200_CUDA_TRY(opt_in_dynamic_smem(kernel, bytes));
-  kernel<<<p.runs * p.abreast, kBlock, bytes, stream>>>(p);
-  B200_CUDA_TRY(cudaGetLastError());
+  B200_CUDA_TRY(heads::launch_early(kernel, p.runs * p.abreast, kBlock, bytes, stream, p));
   if (p.runs == 1) return B200_OK;   // no border
-  // placed while the first kernel still runs; it waits for that kernel's end on the device
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
   // threads for all the pieces that a head has if all are alike, eight to a thread, as far as a block goes
   const int lanes = (p.group < ROWS ? p.group : ROWS) * D / 4;
   const int64_t heads = (int64_t)p.batch * (p.kv_heads * p.row_tiles / p.abreast), want = (p.runs / heads + 2 + kJoinAtOnce - 1) / kJoinAtOnce;
   const int parts = (int)(want < kJoinThreads / lanes ? want : kJoinThreads / lanes);
-  config.gridDim = dim3((p.runs - 1) * p.abreast);
-  config.blockDim = dim3(lanes * parts);
-  config.stream = stream;
-  config.attrs = &early;
-  config.numAttrs = 1;
-  B200_CUDA_TRY(cudaLaunchKernelEx(&config, paged_attention_join_kernel<T, D, ROWS>, p));
+  B200_CUDA_TRY(heads::launch_early(paged_attention_join_kernel<T, D, ROWS>, (p.runs - 1) * p.abreast, lanes * parts, 0, stream, p));
   return B200_OK;
 }
 template <typename T, int STORE, int D> int by_rows(const Problem &p, cudaStream_t stream) {

@@ -199,6 +199,7 @@ head_norm_rotary_kernel(Operand q, Operand k, Rotation r, int unit_rows, uint32_
   using Copies = Ring<2 * Eight<T>::kVectors, kStages>;
   extern __shared__ __align__(16) unsigned char dynamic_smem[];
   const Copies ring(dynamic_smem);
+  heads::await_stream();
   const int e = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const uint32_t slices = q.slices + k.slices, step = gridDim.x * kGroups;
   const bool inside = e * 16 < r.columns, interleaved = r.interleaved;
@@ -303,6 +304,7 @@ head_norm_rotary_backward_kernel(Operand q, Operand k, Rotation r, int unit_rows
   static_assert(Copies::kBytes >= kGroups * (LANES * 16 + 1) * 4, "the ring holds the block's sums in the end");
   extern __shared__ __align__(16) unsigned char dynamic_smem[];
   const Copies ring(dynamic_smem);
+  heads::await_stream();
   const int e = threadIdx.x % LANES, group = threadIdx.x / LANES;
   const bool is_key = (int)blockIdx.x >= q_blocks, interleaved = r.interleaved;
   const Operand o = is_key ? k : q;
@@ -420,14 +422,15 @@ head_norm_rotary_backward_kernel(Operand q, Operand k, Rotation r, int unit_rows
   }
 }
 
-// 32 columns x 32 lanes of rows: blockIdx.y 0 adds q's rows of `partial`, 1 adds k's.
+// 32 columns x 32 lanes of rows: even blocks add q's rows of `partial`, odd ones k's.
 __global__ void __launch_bounds__(1024)
 head_norm_rotary_reduce_kernel(const float *__restrict__ partial, int q_blocks, int blocks, int columns,
                                float *__restrict__ dq_weight, float *__restrict__ dk_weight) {
   __shared__ float sums[32][33];
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  const int column = blockIdx.x * 32 + threadIdx.x % 32, lane = threadIdx.x / 32;
-  const int begin = blockIdx.y ? q_blocks : 0, end = blockIdx.y ? blocks : q_blocks;
+  heads::await_stream();
+  const bool is_key = blockIdx.x & 1;
+  const int column0 = blockIdx.x / 2 * 32, column = column0 + threadIdx.x % 32, lane = threadIdx.x / 32;
+  const int begin = is_key ? q_blocks : 0, end = is_key ? blocks : q_blocks;
   float total = 0.0f;
   if (column < columns) {
 #pragma unroll 4
@@ -435,9 +438,9 @@ head_norm_rotary_reduce_kernel(const float *__restrict__ partial, int q_blocks, 
   }
   sums[lane][threadIdx.x % 32] = total;
   __syncthreads();
-  total = warp_sum(sums[threadIdx.x % 32][lane]);   // lane `lane` of the block now stands for column blockIdx.x * 32 + lane
-  const int result = blockIdx.x * 32 + lane;
-  if (threadIdx.x % 32 == 0 && result < columns) (blockIdx.y ? dk_weight : dq_weight)[result] = total;
+  total = warp_sum(sums[threadIdx.x % 32][lane]);   // warp `lane` now stands for column column0 + lane
+  const int result = column0 + lane;
+  if (threadIdx.x % 32 == 0 && result < columns) (is_key ? dk_weight : dq_weight)[result] = total;
 }
 
 // --------------------------------------------------------------------- host
@@ -582,8 +585,8 @@ int launch_forward(const Operand &q, const Operand &k, const Rotation &r, int un
   B200_CUDA_TRY(opt_in_dynamic_smem(kernel, kBytes));
   const int64_t units = (int64_t)r.tokens * (q.slices + k.slices), need = (units + kGroups - 1) / kGroups;
   const int64_t resident = (int64_t)kBlocksPerSm * sm_count();
-  kernel<<<(unsigned)(need < resident ? need : resident), kThreads, kBytes, stream>>>(q, k, r, unit_rows, (uint32_t)units);
-  B200_CUDA_TRY(cudaGetLastError());
+  B200_CUDA_TRY(heads::launch_early(kernel, (unsigned)(need < resident ? need : resident), kThreads, kBytes, stream, q, k, r, unit_rows,
+                                    (uint32_t)units));
   return B200_OK;
 }
 
@@ -629,8 +632,7 @@ cudaError_t launch_backward(const Operand &q, const Operand &k, const Rotation &
   const auto kernel = head_norm_rotary_backward_kernel<T, LANES>;
   const cudaError_t error = opt_in_dynamic_smem(kernel, kBytes);
   if (error != cudaSuccess) return error;
-  kernel<<<shape.blocks, kThreads, kBytes, stream>>>(q, k, r, shape.unit_rows, shape.q_blocks, partial);
-  return cudaGetLastError();
+  return heads::launch_early(kernel, shape.blocks, kThreads, kBytes, stream, q, k, r, shape.unit_rows, shape.q_blocks, partial);
 }
 
 template <typename T>
@@ -651,18 +653,8 @@ int backward(const Arguments &a, const View3 &grad_q, const View3 &grad_k, const
   default: error = launch_backward<T, 16>(q, k, r, shape, partial, stream); break;
   }
   if (error != cudaSuccess) return cuda_fail(error, "head_norm_rotary_backward");
-  // the reduction is placed while the first kernel still runs and waits for its end on the device
-  cudaLaunchAttribute early{};
-  early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  early.val.programmaticStreamSerializationAllowed = 1;
-  cudaLaunchConfig_t config{};
-  config.gridDim = dim3((r.columns + 31) / 32, 2);
-  config.blockDim = dim3(1024);
-  config.stream = stream;
-  config.attrs = &early;
-  config.numAttrs = shape.blocks ? 1 : 0;
-  B200_CUDA_TRY(cudaLaunchKernelEx(&config, head_norm_rotary_reduce_kernel, (const float *)partial, shape.q_blocks, shape.blocks,
-                                   r.columns, dq_weight, dk_weight));
+  B200_CUDA_TRY(heads::launch_early(head_norm_rotary_reduce_kernel, 2 * ((r.columns + 31) / 32), 1024, 0, stream, partial,
+                                    shape.q_blocks, shape.blocks, r.columns, dq_weight, dk_weight));
   return B200_OK;
 }
 

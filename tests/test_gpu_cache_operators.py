@@ -491,6 +491,63 @@ def test_in_a_graph_with_new_contents():
     no_status()
 
 
+def test_in_a_graph_behind_copies_and_other_streams():
+    """Kernels that may be placed early keep the order that the stream gives them: behind a copy, behind a fill,
+    behind two streams at once, eagerly and captured."""
+    case = attention_case([300, 77], 2, 4, 128, 16, BF16, I8, "heads", seed=31)
+    q, k, qw, kw, cos, sin, positions = rotary_inputs(2, 8, 2, 128, 64, BF16, seed=32)
+    next_q, next_k = [randn(*t.shape, dtype=BF16, seed=40 + i) for i, t in enumerate((q, k))]
+    v = randn(2, 2, 128, dtype=BF16, seed=33)
+    slots = torch.zeros(2, dtype=torch.int64, device=DEV)
+    for b, n in enumerate((300, 77)):
+        slots[b] = int(case["block_table"][b, n // 16]) * 16 + n % 16 if n % 16 else -1
+    case["lengths"] = int32([300 + (300 % 16 > 0), 77 + (77 % 16 > 0)])
+    held = [t.clone() for t in (case["k_cache"], case["v_cache"], case["k_scale"], case["v_scale"])]
+    staged_q, staged_k, staged_v = torch.empty_like(next_q), torch.empty_like(next_k), torch.empty_like(v)
+
+    def work(side):
+        main = torch.cuda.current_stream()
+        staged_q.copy_(next_q)
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            staged_v.fill_(0)
+            staged_v.copy_(v)
+        staged_k.copy_(next_k)
+        turned = ops.head_norm_rotary(staged_q, staged_k, qw, kw, cos, sin, positions)
+        main.wait_stream(side)
+        ops.cache_write(turned[1], staged_v, slots, case["k_cache"], case["v_cache"], case["k_scale"], case["v_scale"])
+        out, lse = attend(case | {"q": turned[0]})
+        grads = ops.head_norm_rotary_backward(turned[0], turned[1], staged_q, staged_k, qw, kw, cos, sin, positions)
+        back = ops.cache_read(case["k_cache"], case["v_cache"], slots, case["k_scale"], case["v_scale"], dtype=BF16)
+        staged_q.fill_(float("nan"))          # behind all readers
+        staged_k.fill_(float("nan"))
+        return (*turned, out, lse, *grads, *back)
+
+    want = [t.clone() for t in work(torch.cuda.Stream())]
+    torch.cuda.synchronize()
+    assert all(t.isfinite().all() for t in want)
+    plain.close(want[0], *plain.norm_rotary(next_q, qw, cos, sin, positions, 1e-6, False))
+    for t, old in zip((case["k_cache"], case["v_cache"], case["k_scale"], case["v_scale"]), held):
+        t.copy_(old)
+    graph = torch.cuda.CUDAGraph()
+    side = torch.cuda.Stream()
+    with torch.cuda.graph(graph):
+        got = work(side)
+    for _ in range(20):
+        graph.replay()
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(20):                       # eagerly, back to back, on streams in turn
+        for stream in streams:
+            stream.wait_stream(streams[0] if stream is streams[1] else streams[1])
+            with torch.cuda.stream(stream):
+                again = work(side)
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, b) for a, b in zip(again, want))
+    no_status()
+
+
 # -------------------------------------------------------------------------- all of them in a row
 @pytest.mark.parametrize("store", [BF16, I8, E4M3])
 def test_a_prompt_and_new_tokens(store):

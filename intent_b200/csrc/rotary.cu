@@ -502,29 +502,32 @@ int check(const char *what, const Arguments &a, const View3 *const *rows, int ro
   return B200_OK;
 }
 
-// An output is written row by row after the row has been read: it may BE an input view (same base
-// and strides), but may not overlap one in any other way, nor another output.
-int check_output(const char *what, const View3 &out, int size, const View3 *const *inputs, int count, const View3 *other) {
-  if (!heads::distinct(out)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: an output's elements overlap one another", what);
-  const heads::Span span = heads::span(out, size);
-  for (int i = 0; i < count; ++i) {
-    const View3 &in = *inputs[i];
-    const bool same = in.data == out.data && in.d1 == out.d1 && (in.d0 <= 1 || in.s0 == out.s0) && (in.d1 <= 1 || in.s1 == out.s1);
-    // two views of one fused projection interleave in memory: rows of the same pitch that never meet
-    const int64_t gap = ((const char *)in.data - (const char *)out.data) / size;
-    const int64_t pitch = out.s0;
-    const bool aside = !same && in.s0 == pitch && pitch > 0 && in.s1 > 0 && out.s1 > 0 &&
-                       ((gap > 0 && gap >= (out.d1 - 1) * out.s1 + out.d2 && gap + (in.d1 - 1) * in.s1 + in.d2 <= pitch) ||
-                        (gap < 0 && -gap >= (in.d1 - 1) * in.s1 + in.d2 && -gap + (out.d1 - 1) * out.s1 + out.d2 <= pitch));
-    if (!same && !aside && heads::overlap(span, heads::span(in, size)))
-      return fail(B200_ERR_INVALID_ARGUMENT, "%s: an output overlaps an input that it is not", what);
-  }
-  if (other) {
-    const View3 *const one[] = {other};
-    const bool same = other->data == out.data && out.d0 && out.d1 && other->d1;
-    if (same) return fail(B200_ERR_INVALID_ARGUMENT, "%s: the outputs overlap", what);
-    return check_output(what, out, size, one, 1, nullptr);
-  }
+// Whether two views interleave in memory without meeting: rows of one pitch, side by side (slices of one
+// fused projection).
+bool side_by_side(const View3 &a, const View3 &b, int size) {
+  const int64_t gap = ((const char *)b.data - (const char *)a.data) / size;
+  if (a.s0 != b.s0 || a.s0 <= 0 || a.s1 <= 0 || b.s1 <= 0) return false;
+  if (gap < 0) return side_by_side(b, a, size);
+  return gap >= (a.d1 - 1) * a.s1 + a.d2 && gap + (b.d1 - 1) * b.s1 + b.d2 <= a.s0;
+}
+bool same_view(const View3 &a, const View3 &b) {
+  return a.data == b.data && a.d1 == b.d1 && (a.d0 <= 1 || a.s0 == b.s0) && (a.d1 <= 1 || a.s1 == b.s1);
+}
+bool meet(const View3 &a, const View3 &b, int size) {
+  return heads::overlap(heads::span(a, size), heads::span(b, size)) && !side_by_side(a, b, size);
+}
+
+// Outputs: rows[count - 2] of q and rows[count - 1] of k; before them inputs of q and k in turn.  A row is
+// written after it has been read, so an output may BE an input of its own rows, but it meets no other one,
+// nor the other output, nor itself.
+int check_outputs(const char *what, const View3 *const *rows, int count, int size) {
+  const View3 &to_q = *rows[count - 2], &to_k = *rows[count - 1];
+  if (!heads::distinct(to_q) || !heads::distinct(to_k)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: an output's elements overlap one another", what);
+  if (meet(to_q, to_k, size)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: the outputs overlap", what);
+  for (int o = 0; o < 2; ++o)
+    for (int i = 0; i < count - 2; ++i)
+      if (meet(*rows[count - 2 + o], *rows[i], size) && !(i % 2 == o && same_view(*rows[count - 2 + o], *rows[i])))
+        return fail(B200_ERR_INVALID_ARGUMENT, "%s: an output overlaps an input that it is not", what);
   return B200_OK;
 }
 
@@ -686,8 +689,7 @@ extern "C" int b200_head_norm_rotary(const int64_t *slots, int64_t count, float 
   if (status != B200_OK) return status;
   if (a.q.d0 == 0 || a.q.d1 + a.k.d1 == 0) return B200_OK;
   const int size = heads::element_size(dtype);
-  status = check_output(what, to_q, size, rows, 2, &to_k);
-  if (status == B200_OK) status = check_output(what, to_k, size, rows, 2, nullptr);
+  status = check_outputs(what, rows, 4, size);
   if (status != B200_OK) return status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
@@ -739,8 +741,7 @@ extern "C" int b200_head_norm_rotary_backward(const int64_t *slots, int64_t coun
   if (partial.s1 != 1 || (shape.blocks > 1 && partial.s0 != partial.d1))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the scratch is contiguous", what);
   const int size = heads::element_size(dtype);
-  status = check_output(what, to_q, size, rows, 4, &to_k);
-  if (status == B200_OK) status = check_output(what, to_k, size, rows, 4, nullptr);
+  status = check_outputs(what, rows, 6, size);
   if (status != B200_OK) return status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   float *scratch = static_cast<float *>(const_cast<void *>(partial.data));

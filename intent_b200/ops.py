@@ -70,8 +70,10 @@ _workspaces: dict[torch.device, torch.Tensor] = {}
 def workspace(device: torch.device) -> torch.Tensor:
     """The zero-initialised int32 status/workspace view the tensor-core entries take."""
     device = torch.device(device)
+    if device.type == "cuda" and device.index is None:
+        device = torch.device("cuda", torch.cuda.current_device())
     if device not in _workspaces:
-        _workspaces[device] = torch.zeros(_native.WORKSPACE_WORDS, dtype=torch.int32, device=device)
+        _workspaces.setdefault(device, torch.zeros(_native.WORKSPACE_WORDS, dtype=torch.int32, device=device))
     return _workspaces[device]
 
 

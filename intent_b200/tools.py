@@ -84,7 +84,7 @@ def doctor(device: int | None = 0, *, compiler=None) -> dict:
         if missing:
             raise ImportError(f"{_native.LIBRARY_PATH} lacks {missing}")
         return {"path": str(_native.LIBRARY_PATH), "abi_version": int(handle.b200_abi_version()),
-                "entries": len(_native.SIGNATURES)}
+                "entries": len(_native.SIGNATURES), "binding": _native.binding().__file__}
 
     def python_module(name):
         module = importlib.import_module(name)

@@ -77,6 +77,21 @@ def test_rotary_views_of_one_projection_are_taken_apart():
     assert rotary(q=q, k=k_over, qo=q, ko=k_over) == 1
 
 
+def test_an_output_may_only_be_the_input_of_its_own_rows():
+    """With as many key heads as query heads q's output could pass for k."""
+    even = {"k": view(5, 4, 64, address=FAR[1]), "ko": view(5, 4, 64, address=FAR[3])}
+    assert rotary(**even, qo=view(5, 4, 64, address=FAR[1])) == 1
+    assert rotary(**(even | {"ko": view(5, 4, 64, address=FAR[0])})) == 1
+    assert rotary(**(even | {"ko": view(5, 4, 64, address=FAR[2])})) == 1
+    grads = {"k": view(5, 4, 64, address=FAR[1]), "gk": view(5, 4, 64, address=FAR[5]), "dk": view(5, 4, 64, address=FAR[3]),
+             "partial": view(64, 64, address=FAR[8])}
+    for place in (FAR[1], FAR[5], FAR[3]):
+        assert backward(**grads, dq=view(5, 4, 64, address=place)) == 1
+    if not torch.cuda.is_available():
+        for place in (FAR[0], FAR[4]):
+            assert backward(**grads, dq=view(5, 4, 64, address=place)) == _native.ERR_CUDA
+
+
 def backward(**change):
     rows = ctypes.c_int64()
     assert _native.entry("b200_head_norm_rotary_scratch")(5, 4, 2, 64, ctypes.byref(rows)) == 0

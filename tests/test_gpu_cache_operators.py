@@ -162,6 +162,28 @@ def test_rotary_edges():
         ops.head_norm_rotary(q, k, qw, kw, cos, sin, positions, q_out=k)
 
 
+def test_rotary_strides_and_nothing():
+    """Positions, tables and heads that repeat (stride 0) or skip; no tokens; one output given."""
+    q, k, qw, kw, cos, sin, positions = rotary_inputs(12, 4, 4, 64, 32, F16, seed=9)
+    one = int32([17]).expand(12)
+    apart = torch.stack((positions, positions + 1), 1)[:, 0]
+    for places in (one, apart):
+        got = ops.head_norm_rotary(q[::2], k[::2], qw, kw, cos, sin, places[::2], 1e-5, k_out=torch.empty(6, 4, 64, dtype=F16, device=DEV))
+        for out, x, w in zip(got, (q[::2], k[::2]), (qw, kw)):
+            plain.close(out, *plain.norm_rotary(x, w, cos, sin, places[::2], 1e-5, False))
+    shared = k[:, :1].expand(12, 4, 64)
+    flat = cos[3:4].expand(64, 32), sin[3:4].expand(64, 32)
+    got = ops.head_norm_rotary(q, shared, qw, kw, *flat, positions, 1e-5)
+    plain.close(got[1], *plain.norm_rotary(shared, kw, *flat, positions, 1e-5, False))
+    assert ops.head_norm_rotary(q[:0], k[:0], qw, kw, cos, sin, positions[:0])[1].shape == (0, 4, 64)
+    assert ops.head_norm_rotary(q[:, :0], k, qw, kw, cos, sin, positions)[0].shape == (12, 0, 64)
+    with pytest.raises(ValueError):
+        ops.head_norm_rotary(q, k, qw, kw, cos, sin, positions, q_out=k)          # the other's input
+    with pytest.raises(ValueError):
+        ops.head_norm_rotary(q, shared, qw, kw, cos, sin, positions, k_out=shared)
+    no_status()
+
+
 # --------------------------------------------------------------------------------- the cache
 def cache_rows(tokens, heads, columns, dtype, seed=0):
     both = randn(tokens, 2 * heads + 1, columns, dtype=F32, seed=seed) * torch.exp(1.5 * randn(tokens, 2 * heads + 1, 1, seed=seed + 1))
@@ -261,6 +283,9 @@ def test_slots_outside_the_cache_are_left_out_and_reported(store):
     assert not back[0][[1, 3, 5]].any() and back[0][[0, 2, 4]].any()
     twice = ops.cache_read(kc, vc, torch.tensor([3, 3, 0, 3], device=DEV), ks, vs, dtype=BF16)     # reading a slot twice is fine
     assert torch.equal(twice[0][0], twice[0][3]) and torch.equal(twice[0][2], back[0][2])
+    empty = [None if t is None else t[:0] for t in (kc, vc, ks, vs)]                 # a cache of no pages holds no slot
+    ops.cache_write(k, v, slots, *empty)
+    status_names("[0234]")                                                            # any of the four that name one
     nothing = ops.cache_read(kc, vc, slots[:0], ks, vs)
     assert nothing[0].shape == (0, 2, 64)
     ops.cache_write(k[:0], v[:0], slots[:0], kc, vc, ks, vs)
@@ -409,6 +434,11 @@ def test_paged_attention_strides_outputs_and_shared_pages():
     target = torch.zeros(8, 3, 192, dtype=F16, device=DEV)
     out = ops.paged_attention(view, case["k_cache"], case["v_cache"], table, lengths, case["scale"], out=target[..., 64:].transpose(0, 1))
     assert torch.equal(out, expected) and not target[..., :64].any()
+    assert torch.equal(ops.paged_attention(case["q"], case["k_cache"], case["v_cache"], case["block_table"], case["lengths"],
+                                           case["scale"]), expected)
+    # one table and one length for all sequences, one query for all heads; a negative scale
+    check_attention(case | {"block_table": case["block_table"][:1].expand(3, -1), "lengths": int32([77]).expand(3),
+                            "q": case["q"][:, :1].expand(3, 8, 128), "scale": -0.2})
     with pytest.raises(ValueError):
         ops.paged_attention(case["q"], case["k_cache"], case["v_cache"], case["block_table"], case["lengths"], 0.1, out=case["q"])
     with pytest.raises(TypeError):

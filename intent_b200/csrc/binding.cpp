@@ -1,7 +1,7 @@
 // The way from torch tensors to an entry that takes its views as one array of slots
 // (include/intent_b200.h): types, shapes and devices are checked, outputs and scratch allocated, the slots
 // packed and the entry called on torch's current stream, without a Python object a view.  A small call of ten
-// views took 20 us of host time with ctypes and takes 10 this way; many of these kernels run for less.
+// views took 34 us of host time with ctypes and takes 8 this way; many of these kernels run for less.
 #include <ATen/Functions.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -14,93 +14,95 @@
 
 namespace {
 
-constexpr int kMostSlots = 256;
+constexpr int kMostSlots = 256, kMostSymbols = 16;
 
-// The extents that `shape`, a tuple of Python integers, asks for are the tensor's.
-bool same_shape(const at::Tensor &tensor, PyObject *shape) {
-  const Py_ssize_t rank = PyTuple_GET_SIZE(shape);
-  if (tensor.dim() != rank) return false;
-  for (Py_ssize_t i = 0; i < rank; ++i)
-    if (PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i)) != tensor.size(i)) return false;
-  return true;
-}
+// What a view of a call may be.
+enum Kind : long {
+  kGiven = 0,     // a tensor
+  kOutput = 1,    // a tensor, or ... for one to be made and returned
+  kScratch = 2,   // made, and given back to the allocator after the call, in stream order
+  kOptional = 3,  // a tensor, ... for one to be made and returned, or None for a view that is not there
+};
 
-bool extents_of(PyObject *shape, std::vector<int64_t> &extents) {
-  for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(shape); ++i) extents.push_back(PyLong_AsLongLong(PyTuple_GET_ITEM(shape, i)));
-  return !PyErr_Occurred();
-}
-
-// invoke(entry, device, views, number, code, other) -> the tensors made, or a status: the entry's, or -1 - i if
-// view i is not what it should be.  views: a tuple of
-//     (name, tensor, dtype, shape)         a tensor that has to be that
-//     (name, ..., dtype, shape)            one to be made and returned, contiguous
-//     (name, ..., dtype, shape, True)      scratch: made, and given back to the allocator after the call, in
-//                                          stream order
-//     (name, None, rank)                   a view that is not there
-// number: the entry's f32 argument, or None if it has none.
+// invoke(entry, device, plan, tensors, extents, number, code, other) -> the tensors made, or a status: the
+// entry's, or -1 - i if view i is not what it should be.  plan: for each view (name, dtype, symbols, kind);
+// dtype None is the type of the first such view.  A symbol, a small number, stands for an extent: the first
+// of `extents` are given, others are those of the first view that has them, and later views have to agree.
+// Everything made is contiguous and the call's own.  number: the entry's f32 argument, or None if it has none.
 PyObject *invoke(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
-  if (count != 6 || !PyTuple_Check(arguments[2])) {
-    PyErr_SetString(PyExc_TypeError, "invoke(entry, device, views, number, code, other)");
+  if (count != 8 || !PyTuple_Check(arguments[2]) || !PyTuple_Check(arguments[3]) || !PyTuple_Check(arguments[4]) ||
+      PyTuple_GET_SIZE(arguments[2]) != PyTuple_GET_SIZE(arguments[3])) {
+    PyErr_SetString(PyExc_TypeError, "invoke(entry, device, plan, tensors, extents, number, code, other)");
     return nullptr;
   }
   try {
     void *entry = PyLong_AsVoidPtr(arguments[0]);
     const long device = PyLong_AsLong(arguments[1]);
-    PyObject *views = arguments[2];
-    const double number = arguments[3] == Py_None ? 0.0 : PyFloat_AsDouble(arguments[3]);
-    const long code = PyLong_AsLong(arguments[4]), other = PyLong_AsLong(arguments[5]);
+    PyObject *plan = arguments[2], *tensors = arguments[3], *extents = arguments[4];
+    const double number = arguments[5] == Py_None ? 0.0 : PyFloat_AsDouble(arguments[5]);
+    const long code = PyLong_AsLong(arguments[6]), other = PyLong_AsLong(arguments[7]);
+    const Py_ssize_t views = PyTuple_GET_SIZE(plan), given = PyTuple_GET_SIZE(extents);
+    int64_t known[kMostSymbols];
+    for (int i = 0; i < kMostSymbols; ++i) known[i] = -1;
+    for (Py_ssize_t i = 0; i < given && i < kMostSymbols; ++i) known[i] = PyLong_AsLongLong(PyTuple_GET_ITEM(extents, i));
     if (PyErr_Occurred()) return nullptr;
+    at::ScalarType call_type = at::ScalarType::Undefined;
     // what is wrong is found before anything is made
-    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(views); ++i) {
-      PyObject *view = PyTuple_GET_ITEM(views, i);
-      if (!PyTuple_Check(view) || PyTuple_GET_SIZE(view) < 3) {
-        PyErr_SetString(PyExc_TypeError, "a view is (name, tensor, dtype, shape) or (name, None, rank)");
-        return nullptr;
-      }
-      PyObject *object = PyTuple_GET_ITEM(view, 1), *kind = PyTuple_GET_ITEM(view, 2);
-      if (PyTuple_GET_SIZE(view) == 3) {
-        if (object != Py_None || !PyLong_Check(kind)) return PyLong_FromSsize_t(-1 - i);
-        continue;
-      }
-      PyObject *shape = PyTuple_GET_ITEM(view, 3);
-      if (!THPDtype_Check(kind) || !PyTuple_Check(shape)) return PyLong_FromSsize_t(-1 - i);
-      if (object == Py_Ellipsis) continue;
-      if (!THPVariable_Check(object)) return PyLong_FromSsize_t(-1 - i);
+    for (Py_ssize_t i = 0; i < views; ++i) {
+      PyObject *view = PyTuple_GET_ITEM(plan, i), *object = PyTuple_GET_ITEM(tensors, i);
+      const long kind = PyLong_AsLong(PyTuple_GET_ITEM(view, 3));
+      if (object == Py_Ellipsis && kind != kGiven) continue;
+      if (object == Py_None && kind == kOptional) continue;
+      if (kind == kScratch || !THPVariable_Check(object)) return PyLong_FromSsize_t(-1 - i);
       const at::Tensor &tensor = THPVariable_Unpack(object);
-      if (tensor.layout() != at::kStrided || tensor.scalar_type() != reinterpret_cast<THPDtype *>(kind)->scalar_type ||
-          !tensor.is_cuda() || tensor.get_device() != device || !same_shape(tensor, shape))
-        return PyErr_Occurred() ? nullptr : PyLong_FromSsize_t(-1 - i);
+      PyObject *dtype = PyTuple_GET_ITEM(view, 1), *symbols = PyTuple_GET_ITEM(view, 2);
+      if (dtype == Py_None && call_type == at::ScalarType::Undefined) call_type = tensor.scalar_type();
+      const at::ScalarType wanted = dtype == Py_None ? call_type : reinterpret_cast<THPDtype *>(dtype)->scalar_type;
+      const Py_ssize_t rank = PyTuple_GET_SIZE(symbols);
+      if (tensor.layout() != at::kStrided || tensor.scalar_type() != wanted || !tensor.is_cuda() || tensor.get_device() != device ||
+          tensor.dim() != rank)
+        return PyLong_FromSsize_t(-1 - i);
+      for (Py_ssize_t j = 0; j < rank; ++j) {
+        int64_t &extent = known[PyLong_AsLong(PyTuple_GET_ITEM(symbols, j)) & (kMostSymbols - 1)];
+        if (extent < 0) extent = tensor.size(j);
+        if (extent != tensor.size(j)) return PyLong_FromSsize_t(-1 - i);
+      }
     }
     int64_t slots[kMostSlots];
     int used = 0;
     const c10::cuda::CUDAGuard guard(static_cast<c10::DeviceIndex>(device));
     std::vector<at::Tensor> made, scratch;
-    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(views); ++i) {
-      PyObject *view = PyTuple_GET_ITEM(views, i), *object = PyTuple_GET_ITEM(view, 1);
-      const bool absent = PyTuple_GET_SIZE(view) == 3;
-      at::Tensor fresh;
-      if (!absent && object == Py_Ellipsis) {
-        std::vector<int64_t> extents;
-        if (!extents_of(PyTuple_GET_ITEM(view, 3), extents)) return nullptr;
-        fresh = at::empty(extents, at::TensorOptions()
-                                       .dtype(reinterpret_cast<THPDtype *>(PyTuple_GET_ITEM(view, 2))->scalar_type)
-                                       .device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
-        (PyTuple_GET_SIZE(view) > 4 ? scratch : made).push_back(fresh);
-      }
-      const int64_t rank = absent ? PyLong_AsLong(PyTuple_GET_ITEM(view, 2)) : PyTuple_GET_SIZE(PyTuple_GET_ITEM(view, 3));
-      if (rank < 0 || used + 1 + 2 * rank > kMostSlots) return PyLong_FromSsize_t(-1 - i);
-      if (absent) {
-        for (int64_t j = 0; j < 1 + 2 * rank; ++j) slots[used++] = 0;
+    for (Py_ssize_t i = 0; i < views; ++i) {
+      PyObject *view = PyTuple_GET_ITEM(plan, i), *object = PyTuple_GET_ITEM(tensors, i), *symbols = PyTuple_GET_ITEM(view, 2);
+      const int rank = static_cast<int>(PyTuple_GET_SIZE(symbols));
+      if (used + 1 + 2 * rank > kMostSlots) return PyLong_FromSsize_t(-1 - i);
+      if (object == Py_None) {
+        for (int j = 0; j < 1 + 2 * rank; ++j) slots[used++] = 0;
         continue;
+      }
+      at::Tensor fresh;
+      if (object == Py_Ellipsis) {
+        PyObject *dtype = PyTuple_GET_ITEM(view, 1);
+        int64_t shape[kMostSymbols];
+        for (int j = 0; j < rank; ++j) {
+          shape[j] = known[PyLong_AsLong(PyTuple_GET_ITEM(symbols, j)) & (kMostSymbols - 1)];
+          if (shape[j] < 0) return PyLong_FromSsize_t(-1 - i);
+        }
+        fresh = at::empty(at::IntArrayRef(shape, rank),
+                          at::TensorOptions()
+                              .dtype(dtype == Py_None ? call_type : reinterpret_cast<THPDtype *>(dtype)->scalar_type)
+                              .device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+        (PyLong_AsLong(PyTuple_GET_ITEM(view, 3)) == kScratch ? scratch : made).push_back(fresh);
       }
       const at::Tensor &tensor = fresh.defined() ? fresh : THPVariable_Unpack(object);
       slots[used++] = reinterpret_cast<int64_t>(tensor.data_ptr());
-      for (int64_t j = 0; j < rank; ++j) slots[used++] = tensor.size(j);
-      for (int64_t j = 0; j < rank; ++j) slots[used++] = tensor.stride(j);
+      for (int j = 0; j < rank; ++j) slots[used++] = tensor.size(j);
+      for (int j = 0; j < rank; ++j) slots[used++] = tensor.stride(j);
     }
+    if (PyErr_Occurred()) return nullptr;
     void *stream = c10::cuda::getCurrentCUDAStream(static_cast<c10::DeviceIndex>(device)).stream();
     int status;
-    if (arguments[3] == Py_None)
+    if (arguments[5] == Py_None)
       status = reinterpret_cast<int (*)(const int64_t *, int64_t, int32_t, int32_t, void *)>(entry)(
           slots, used, static_cast<int32_t>(code), static_cast<int32_t>(other), stream);
     else
@@ -118,7 +120,7 @@ PyObject *invoke(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
 
 PyMethodDef methods[] = {
     {"invoke", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(invoke)), METH_FASTCALL,
-     "invoke(entry, device, views, number, code, other) -> the tensors made, or a status"},
+     "invoke(entry, device, plan, tensors, extents, number, code, other) -> the tensors made, or a status"},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef definition = {PyModuleDef_HEAD_INIT, "binding", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

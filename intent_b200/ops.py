@@ -289,7 +289,67 @@ def attention_backward_dq(q, k, v, grad_output, lse, delta, scale: float, *, hea
 
 
 # ---- operators around a key-value cache ------------------------------------------------------
-# Calls of a few microseconds on the device, so their views are not packed here but by a native module.
+# Calls of a few microseconds on the device, so their views are not checked and packed here but by a
+# native module, after a plan.
+
+_GIVEN, _OUTPUT, _SCRATCH, _OPTIONAL = range(4)
+
+
+class _Plan:
+    """The views of an entry that takes them as one array of slots, in its order.  ``views``: a line for each,
+    "name dtype axis axis ...", where dtype x is the call's own, and axes of one name have one extent.  A name that ends in ``=``
+    is an output, in ``~`` scratch, in ``?`` a view that may be missing.  ``given``: the axes whose extents a call passes."""
+
+    def __init__(self, entry: str, views: str, given: str = ""):
+        self.entry, self.address = entry, None
+        axes = {name: i for i, name in enumerate(given.split())}
+        types = {"x": None, "f32": torch.float32, "i32": torch.int32, "i64": torch.int64}
+        plan = []
+        for line in views.strip().splitlines():
+            name, dtype, *shape = line.split()
+            kind = {"=": _OUTPUT, "~": _SCRATCH, "?": _OPTIONAL}.get(name[-1], _GIVEN)
+            symbols = tuple(axes.setdefault(axis, len(axes)) for axis in shape)
+            plan.append((name.rstrip("=~?"), types.get(dtype, dtype), symbols, kind))
+        self.views, self.axes = tuple(plan), tuple(axes)
+
+    def typed(self, **types):
+        """The same plan with types in the place of names."""
+        plan = _Plan.__new__(_Plan)
+        plan.entry, plan.address, plan.axes = self.entry, None, self.axes
+        plan.views = tuple((name, types.get(dtype, dtype) if isinstance(dtype, str) else dtype, *rest)
+                           for name, dtype, *rest in self.views)
+        return plan
+
+    def __call__(self, device: int, tensors: tuple, extents: tuple, number, code: int, other: int) -> tuple:
+        """Calls the entry on the current stream and returns the tensors that were made for it: those given as ``...``.
+        They, and the scratch, are contiguous allocations of the call's own in the stream's order, so calls may overlap."""
+        if self.address is None:
+            self.invoke, self.address = _native.binding().invoke, _native.address(self.entry)
+        made = self.invoke(self.address, device, self.views, tensors, extents, number, code, other)
+        if type(made) is not tuple:
+            if made < 0:
+                self._refuse(-1 - made, device, tensors, extents)
+            _native.check(self.entry, made)
+        return made
+
+    def _refuse(self, bad: int, device: int, tensors: tuple, extents: tuple) -> None:
+        """Raises what is wrong with a view, given that those before it are right."""
+        known, call_type = dict(enumerate(extents)), None
+        for (name, dtype, symbols, _), tensor in zip(self.views[:bad + 1], tensors):
+            if tensor is ... or tensor is None and name != self.views[bad][0]:
+                continue
+            if not isinstance(tensor, torch.Tensor):
+                raise TypeError(f"{name} must be a torch.Tensor")
+            if tensor.dim() != len(symbols):
+                axes = ", ".join(self.axes[symbol] for symbol in symbols)
+                raise ValueError(f"{name} is a ({axes}{',' * (len(symbols) == 1)}) tensor, got {tuple(tensor.shape)}")
+            call_type = tensor.dtype if dtype is None and call_type is None else call_type
+            shape = tuple(known.setdefault(symbol, extent) for symbol, extent in zip(symbols, tensor.shape))
+            _expect(name, tensor, call_type if dtype is None else dtype, shape)
+            if _cuda_device(tensor) != device:
+                raise ValueError("arguments span different devices")
+        raise ValueError(f"{self.views[bad][0]} must be a strided tensor")
+
 
 def _cuda_device(tensor) -> int:
     """Index of the device that the call runs on, from its first tensor."""
@@ -300,63 +360,29 @@ def _cuda_device(tensor) -> int:
     return tensor.get_device()
 
 
-_addresses: dict[str, int] = {}
-_native_invoke = None
-
-
-def _invoke(name: str, device: int, views: tuple, number, code: int, other: int) -> tuple:
-    """Calls an entry that takes its views as one array of slots, and returns the tensors that were made for it.
-    ``views``: (name, tensor, dtype, shape), with ``...`` for the tensor if it is to be made, (name, ..., dtype, shape,
-    True) for scratch, (name, None, rank) for a view that is not there; ``number``: the entry's f32 argument, if it
-    has one.  Everything made is a contiguous allocation of the call's own in the current stream's order, so
-    calls may overlap."""
-    global _native_invoke
-    entry = _addresses.get(name)
-    if entry is None:
-        _native_invoke = _native.binding().invoke
-        entry = _addresses[name] = _native.address(name)
-    made = _native_invoke(entry, device, views, number, code, other)
-    if type(made) is not tuple:
-        if made < 0:
-            _refuse(views[-1 - made], device)
-        _native.check(name, made)
-    return made
-
-
-def _refuse(view: tuple, device: int) -> None:
-    """Raises what is wrong with a view."""
-    name, tensor, dtype, shape = view
-    if not isinstance(tensor, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    _expect(name, tensor, dtype, shape)
-    if _cuda_device(tensor) != device:
-        raise ValueError("arguments span different devices")
-    raise ValueError(f"{name} must be a strided tensor")
-
-
 def _outputs(made: tuple, *given) -> tuple:
     """The outputs of a call: those that the caller gave, and for the others what was made, in order."""
     rest = iter(made)
     return tuple(next(rest) if tensor is None else tensor for tensor in given)
 
 
-_status_spaces: dict[int, tuple] = {}
+_status_spaces: dict[int, torch.Tensor] = {}
 
 
-def _status(device: int) -> tuple:
-    """The view of ``workspace(device)``, where an entry records a bad index.  It is made once per device and
-    shared by all streams, so the first call may not fall into a graph capture, whose replays would
-    clear it, and its zeros have to be there before any other stream writes to it."""
-    view = _status_spaces.get(device)
-    if view is None:
+def _status(device: int) -> torch.Tensor:
+    """``workspace(device)``, where an entry records a bad index.  It is made once per device and shared by all
+    streams, so the first call may not fall into a graph capture, whose replays would clear it, and its
+    zeros have to be there before any other stream writes to it."""
+    space = _status_spaces.get(device)
+    if space is None:
         where = torch.device("cuda", device)
         with torch.cuda.device(where):
             if torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("call this operator once outside a graph capture before capturing it")
             space = workspace(where)
             torch.cuda.current_stream(where).synchronize()
-        view = _status_spaces[device] = ("workspace", space, torch.int32, (_native.WORKSPACE_WORDS,))
-    return view
+        _status_spaces[device] = space
+    return space
 
 
 @lru_cache(maxsize=4096)
@@ -366,19 +392,34 @@ def _scratch_size(name: str, device: int, *arguments) -> int:
     return size.value
 
 
-def _shape(name: str, tensor, rank: int, axes: str) -> tuple:
-    if not isinstance(tensor, torch.Tensor):
-        raise TypeError(f"{name} must be a torch.Tensor")
-    if tensor.dim() != rank:
-        raise ValueError(f"{name} is a {axes} tensor, got {tuple(tensor.shape)}")
-    return tuple(tensor.shape)
+_ROTARY = _Plan("b200_head_norm_rotary", """
+    q x tokens heads head_dim
+    k x tokens kv_heads head_dim
+    q_weight x head_dim
+    k_weight x head_dim
+    cos f32 rows pairs
+    sin f32 rows pairs
+    positions i32 tokens
+    q_out= x tokens heads head_dim
+    k_out= x tokens kv_heads head_dim
+    workspace i32 words""")
 
-
-def _rotary_shapes(q, k, cos) -> tuple:
-    shape = _shape("q", q, 3, "(tokens, heads, head_dim)")
-    k_shape = (shape[0], _shape("k", k, 3, "(tokens, heads, head_dim)")[1], shape[2])
-    _float_type("q", q)
-    return shape, k_shape, _shape("cos", cos, 2, "(rows, pairs)")
+_ROTARY_BACKWARD = _Plan("b200_head_norm_rotary_backward", """
+    grad_q x tokens heads head_dim
+    grad_k x tokens kv_heads head_dim
+    q x tokens heads head_dim
+    k x tokens kv_heads head_dim
+    q_weight x head_dim
+    k_weight x head_dim
+    cos f32 rows pairs
+    sin f32 rows pairs
+    positions i32 tokens
+    dq= x tokens heads head_dim
+    dk= x tokens kv_heads head_dim
+    dq_weight= f32 head_dim
+    dk_weight= f32 head_dim
+    partial~ f32 partial_rows head_dim
+    workspace i32 words""", "partial_rows")
 
 
 def head_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, epsilon: float = 1e-6, *, interleaved: bool = False,
@@ -390,15 +431,10 @@ def head_norm_rotary(q, k, q_weight, k_weight, cos, sin, positions, epsilon: flo
     padding, whose rows become zeros; one behind the tables gives zeros too and is reported by
     ``workspace_status``.  Returns ``(q_out, k_out)``; an output may be its input."""
     device = _cuda_device(q)
-    shape, k_shape, table = _rotary_shapes(q, k, cos)
-    dtype, columns = q.dtype, shape[2:]
-    made = _invoke(
-        "b200_head_norm_rotary", device,
-        (("q", q, dtype, shape), ("k", k, dtype, k_shape), ("q_weight", q_weight, dtype, columns),
-         ("k_weight", k_weight, dtype, columns), ("cos", cos, torch.float32, table), ("sin", sin, torch.float32, table),
-         ("positions", positions, torch.int32, shape[:1]), ("q_out", ... if q_out is None else q_out, dtype, shape),
-         ("k_out", ... if k_out is None else k_out, dtype, k_shape), _status(device)), float(epsilon), _CODES[dtype], bool(interleaved))
-    return _outputs(made, q_out, k_out)
+    made = _ROTARY(device, (q, k, q_weight, k_weight, cos, sin, positions, ... if q_out is None else q_out,
+                            ... if k_out is None else k_out, _status(device)),
+                   (), float(epsilon), _CODES[_float_type("q", q)], bool(interleaved))
+    return made if len(made) == 2 else _outputs(made, q_out, k_out)
 
 
 def head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions, epsilon: float = 1e-6, *,
@@ -407,38 +443,68 @@ def head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin
     dk_weight)``, the weights' in f32.  Rows of padding get zeros and add nothing.  ``dq`` may be
     ``grad_q`` or ``q``, and ``dk`` likewise."""
     device = _cuda_device(q)
-    shape, k_shape, table = _rotary_shapes(q, k, cos)
-    dtype, columns = q.dtype, shape[2:]
-    rows = _scratch_size("b200_head_norm_rotary_scratch", device, shape[0], shape[1], k_shape[1], shape[2])
-    made = _invoke(
-        "b200_head_norm_rotary_backward", device,
-        (("grad_q", grad_q, dtype, shape), ("grad_k", grad_k, dtype, k_shape), ("q", q, dtype, shape), ("k", k, dtype, k_shape),
-         ("q_weight", q_weight, dtype, columns), ("k_weight", k_weight, dtype, columns), ("cos", cos, torch.float32, table),
-         ("sin", sin, torch.float32, table), ("positions", positions, torch.int32, shape[:1]),
-         ("dq", ... if dq is None else dq, dtype, shape), ("dk", ... if dk is None else dk, dtype, k_shape),
-         ("dq_weight", ..., torch.float32, columns), ("dk_weight", ..., torch.float32, columns), ("partial", ..., torch.float32, (rows, shape[2]), True),
-         _status(device)), float(epsilon), _CODES[dtype], bool(interleaved))
-    return _outputs(made, dq, dk, None, None)
+    if q.dim() != 3 or not isinstance(k, torch.Tensor) or k.dim() != 3:
+        raise ValueError("q and k are (tokens, heads, head_dim) tensors")
+    tokens, heads, head_dim = q.shape
+    rows = _scratch_size("b200_head_norm_rotary_scratch", device, tokens, heads, k.shape[1], head_dim)
+    made = _ROTARY_BACKWARD(device, (grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions, ... if dq is None else dq,
+                                     ... if dk is None else dk, ..., ..., ..., _status(device)),
+                            (rows,), float(epsilon), _CODES[_float_type("q", q)], bool(interleaved))
+    return made if len(made) == 4 else _outputs(made, dq, dk, None, None)
 
 
-_NO_SCALES = (("k_scale", None, 3), ("v_scale", None, 3))
-_CACHE_TYPES = (torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn)
+_CACHE_VIEWS = """
+    k_cache cache pages kv_heads page_size head_dim
+    v_cache cache pages kv_heads page_size head_dim"""
+_SCALE_VIEWS = """
+    k_scale? f32 pages kv_heads page_size
+    v_scale? f32 pages kv_heads page_size"""
 
 
-def _cache_views(k_cache, v_cache, k_scale, v_scale) -> tuple:
-    """Shape of a paged cache, its views and its scales' views."""
-    shape = _shape("k_cache", k_cache, 4, "(pages, heads, page_size, head_dim)")
-    dtype = k_cache.dtype
-    if dtype not in _CACHE_TYPES:
-        raise TypeError(f"k_cache must be float16, bfloat16, int8 or float8_e4m3fn, got {dtype}")
-    views = (("k_cache", k_cache, dtype, shape), ("v_cache", v_cache, dtype, shape))
-    if dtype is torch.float16 or dtype is torch.bfloat16:
+def _by_cache_type(plan: _Plan) -> dict:
+    return {dtype: plan.typed(cache=dtype) for dtype in (torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn)}
+
+
+_WRITE = _by_cache_type(_Plan("b200_cache_write", """
+    k x tokens kv_heads head_dim
+    v x tokens kv_heads head_dim
+    slots i64 tokens""" + _CACHE_VIEWS + _SCALE_VIEWS + """
+    workspace i32 words"""))
+
+_READ = _by_cache_type(_Plan("b200_cache_read", _CACHE_VIEWS + """
+    slots i64 tokens""" + _SCALE_VIEWS + """
+    k_out= rows tokens kv_heads head_dim
+    v_out= rows tokens kv_heads head_dim
+    workspace i32 words"""))
+_READ = {(store, rows): plan.typed(rows=rows) for store, plan in _READ.items() for rows in (torch.float16, torch.bfloat16)
+         if store.itemsize == 1 or store is rows}
+
+_ATTENTION = _by_cache_type(_Plan("b200_paged_attention", """
+    q x batch heads head_dim""" + _CACHE_VIEWS + _SCALE_VIEWS + """
+    block_table i32 batch columns
+    lengths i32 batch
+    out= x batch heads head_dim
+    lse? f32 batch heads
+    partial~ f32 scratch
+    workspace i32 words""", "scratch"))
+
+
+def _cache_type(k_cache, k_scale, v_scale, rows: torch.dtype | None) -> torch.dtype:
+    """The type of a cache that goes with its scales and, in 16 bits, with the rows' type."""
+    if not isinstance(k_cache, torch.Tensor):
+        raise TypeError("k_cache must be a torch.Tensor")
+    store = k_cache.dtype
+    if store not in _WRITE:
+        raise TypeError(f"k_cache must be float16, bfloat16, int8 or float8_e4m3fn, got {store}")
+    if store.itemsize == 1:
+        if k_scale is None or v_scale is None:
+            raise ValueError("an 8-bit cache needs k_scale and v_scale")
+    else:
         if k_scale is not None or v_scale is not None:
             raise ValueError("a 16-bit cache has no scales")
-        return shape, views, _NO_SCALES
-    if k_scale is None or v_scale is None:
-        raise ValueError("an 8-bit cache needs k_scale and v_scale")
-    return shape, views, (("k_scale", k_scale, torch.float32, shape[:3]), ("v_scale", v_scale, torch.float32, shape[:3]))
+        if rows is not None and rows is not store:
+            raise TypeError(f"k_cache must have dtype {rows}, torch.int8 or torch.float8_e4m3fn, got {store}")
+    return store
 
 
 def cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
@@ -451,14 +517,9 @@ def cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     skipped; so are slots behind the cache, which ``workspace_status`` reports.  The slots of one call that are not
     negative must differ.  Returns ``(k_cache, v_cache)``."""
     device = _cuda_device(k)
-    dtype = _float_type("k", k, (torch.float16, torch.bfloat16))
-    cache, views, scales = _cache_views(k_cache, v_cache, k_scale, v_scale)
-    if k_cache.dtype is not dtype and k_cache.element_size() == 2:
-        raise TypeError(f"k_cache must have dtype {dtype}, torch.int8 or torch.float8_e4m3fn, got {k_cache.dtype}")
-    shape = (_shape("k", k, 3, "(tokens, heads, head_dim)")[0], cache[1], cache[3])
-    _invoke("b200_cache_write", device,
-            (("k", k, dtype, shape), ("v", v, dtype, shape), ("slots", slots, torch.int64, shape[:1]), *views, *scales,
-             _status(device)), None, _CODES[dtype], _CODES[k_cache.dtype])
+    rows = _float_type("k", k, (torch.float16, torch.bfloat16))
+    store = _cache_type(k_cache, k_scale, v_scale, rows)
+    _WRITE[store](device, (k, v, slots, k_cache, v_cache, k_scale, v_scale, _status(device)), (), None, _CODES[rows], _CODES[store])
     return k_cache, v_cache
 
 
@@ -467,20 +528,17 @@ def cache_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, *, dtype=Non
     head_dim): of a 16-bit cache as they are, of an 8-bit one as code * scale in ``dtype`` (f16 or bf16, the
     default).  Negative slots give zeros, and so do slots behind the cache, which ``workspace_status`` reports."""
     device = _cuda_device(k_cache)
-    cache, views, scales = _cache_views(k_cache, v_cache, k_scale, v_scale)
-    wide = k_cache.element_size() == 2
+    store = _cache_type(k_cache, k_scale, v_scale, None)
     if dtype is None:
-        dtype = k_cache.dtype if wide else torch.bfloat16 if k_out is None else k_out.dtype
-    if dtype not in (torch.float16, torch.bfloat16):
-        raise TypeError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
-    if wide and dtype != k_cache.dtype:
-        raise TypeError(f"a {k_cache.dtype} cache gives its rows as they are, not as {dtype}")
-    shape = (_shape("slots", slots, 1, "(tokens,)")[0], cache[1], cache[3])
-    made = _invoke(
-        "b200_cache_read", device,
-        (*views, ("slots", slots, torch.int64, shape[:1]), *scales, ("k_out", ... if k_out is None else k_out, dtype, shape),
-         ("v_out", ... if v_out is None else v_out, dtype, shape), _status(device)), None, _CODES[dtype], _CODES[k_cache.dtype])
-    return _outputs(made, k_out, v_out)
+        dtype = store if store.itemsize == 2 else torch.bfloat16 if k_out is None else k_out.dtype
+    plan = _READ.get((store, dtype))
+    if plan is None:
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
+        raise TypeError(f"a {store} cache gives its rows as they are, not as {dtype}")
+    made = plan(device, (k_cache, v_cache, slots, k_scale, v_scale, ... if k_out is None else k_out, ... if v_out is None else v_out,
+                         _status(device)), (), None, _CODES[dtype], _CODES[store])
+    return made if len(made) == 2 else _outputs(made, k_out, v_out)
 
 
 def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, k_scale=None, v_scale=None, out=None,
@@ -493,26 +551,23 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, 
     past the table is cut there, and ``workspace_status`` reports both.  Returns ``out``, or ``(out, lse)``
     with the natural logarithm of the sums (f32)."""
     device = _cuda_device(q)
-    dtype = _float_type("q", q, (torch.float16, torch.bfloat16))
-    shape = _shape("q", q, 3, "(batch, heads, head_dim)")
-    cache, views, scales = _cache_views(k_cache, v_cache, k_scale, v_scale)
-    if k_cache.dtype is not dtype and k_cache.element_size() == 2:
-        raise TypeError(f"k_cache must have dtype {dtype}, torch.int8 or torch.float8_e4m3fn, got {k_cache.dtype}")
-    batch, heads, columns = shape
-    if columns != cache[3]:
-        raise ValueError(f"q has head_dim {columns}, the cache {cache[3]}")
-    if cache[1] < 1 or heads < 1 or heads % cache[1]:
-        raise ValueError(f"{heads} query heads are not a multiple of the cache's {cache[1]}")
-    table = (batch, _shape("block_table", block_table, 2, "(batch, columns)")[1])
-    store = _CODES[k_cache.dtype]
-    words = _scratch_size("b200_paged_attention_scratch", device, batch, heads, cache[1], columns, table[1] * cache[2], store)
-    made = _invoke(
-        "b200_paged_attention", device,
-        (("q", q, dtype, shape), *views, *scales, ("block_table", block_table, torch.int32, table),
-         ("lengths", lengths, torch.int32, shape[:1]), ("out", ... if out is None else out, dtype, shape),
-         ("lse", ..., torch.float32, shape[:2]) if return_lse else ("lse", None, 2),
-         ("partial", ..., torch.float32, (words,), True), _status(device)), float(scale), _CODES[dtype], store)
-    return _outputs(made, out, None) if return_lse else out if out is not None else made[0]
+    rows = _float_type("q", q, (torch.float16, torch.bfloat16))
+    store = _cache_type(k_cache, k_scale, v_scale, rows)
+    if q.dim() != 3 or k_cache.dim() != 4 or not isinstance(block_table, torch.Tensor) or block_table.dim() != 2:
+        raise ValueError("q is a (batch, heads, head_dim) tensor, k_cache (pages, heads, page_size, head_dim), "
+                         "block_table (batch, columns)")
+    batch, heads, head_dim = q.shape
+    _, kv_heads, page_size, _ = k_cache.shape
+    if kv_heads < 1 or heads < 1 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of the cache's {kv_heads}")
+    words = _scratch_size("b200_paged_attention_scratch", device, batch, heads, kv_heads, head_dim,
+                          block_table.shape[1] * page_size, _CODES[store])
+    made = _ATTENTION[store](device, (q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, ... if out is None else out,
+                                      ... if return_lse else None, ..., _status(device)),
+                             (words,), float(scale), _CODES[rows], _CODES[store])
+    if not return_lse:
+        return made[0] if out is None else out
+    return made if out is None else (out, made[0])
 
 
 def gather_probe(table: torch.Tensor, gathers: int, *, variant: int = 1, hints: bool = True) -> None:

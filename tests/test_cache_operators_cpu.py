@@ -211,25 +211,33 @@ def test_ops_check_before_any_call():
     cache = torch.zeros(2, 2, 16, 64, dtype=torch.int8)
     with pytest.raises(ValueError, match="executes on cuda"):
         ops.cache_write(k, k, torch.zeros(3, dtype=torch.int64), cache, cache)
-    for wrong, message in (((cache, cache, None, None), "needs k_scale"), ((cache.half(), cache.half(), w, w), "has no scales"),
-                           ((cache.float(), cache.float(), None, None), "k_cache must be"), ((cache[0], cache[0], None, None), "k_cache is a")):
+    for wrong, message in (((cache, None, None, torch.half), "needs k_scale"), ((cache.half(), w, w, torch.half), "has no scales"),
+                           ((cache.half(), None, None, torch.bfloat16), "k_cache must have dtype torch.bfloat16"),
+                           ((cache.float(), None, None, None), "k_cache must be float16"), (([], None, None, None), "k_cache must be a torch.Tensor")):
         with pytest.raises((TypeError, ValueError), match=message):
-            ops._cache_views(*wrong)
+            ops._cache_type(*wrong)
 
 
 def test_a_view_that_is_not_what_it_should_be_is_named():
-    """The native module finds it before any call, ops says what is wrong with it."""
-    t = torch.zeros(3, 4)
-    good = ("first", None, 2)
-    for bad, error, message in ((("x", t.half(), torch.float32, (3, 4)), TypeError, "x must have dtype torch.float32"),
-                                (("x", t, torch.float32, (4, 3)), ValueError, r"x must have shape \(4, 3\), got \(3, 4\)"),
-                                (("x", t, torch.float32, (3, 4, 1)), ValueError, "x must have shape"),
-                                (("x", [1.0], torch.float32, (1,)), TypeError, "x must be a torch.Tensor"),
-                                (("x", None, torch.float32, (1,)), TypeError, "x must be a torch.Tensor"),
-                                (("x", t, torch.float32, (3, 4)), ValueError, "executes on cuda")):
+    """The native module finds it before any call, ops says what is wrong with it.  (On this machine every tensor is on the
+    wrong device, so the module stops at the first view and the checks here are those of the message.)"""
+    plan = ops._Plan("b200_cache_write", """
+        first? f32 rows
+        x x rows columns
+        y f32 columns
+        z= x rows""", "rows")
+    t, column = torch.zeros(3, 4), torch.zeros(4)
+    for bad, tensors, error, message in (
+            (1, (None, t.long()[:2], column, ...), ValueError, r"x must have shape \(3, 4\), got \(2, 4\)"),
+            (1, (None, [1.0], column, ...), TypeError, "x must be a torch.Tensor"), (1, (None, None, column, ...), TypeError, "x must be a torch.Tensor"),
+            (1, (None, column, column, ...), ValueError, r"x is a \(rows, columns\) tensor, got \(4,\)"),
+            (1, (None, t, column, ...), ValueError, "executes on cuda"), (0, (t, t, column, ...), ValueError, r"first is a \(rows,\) tensor")):
         with pytest.raises(error, match=message):
-            ops._invoke("b200_cache_write", 0, (good, bad), None, 1, 1)
-    for wrong in ((1, 0, [good], None, 1, 1), (1, 0, (good,), None, 1), (1, 0, ("x",), None, 1, 1), (1, 0, (good,), "x", 1, 1)):
+            plan._refuse(bad, 0, tensors, (3,))
+        with pytest.raises(error):
+            plan(0, tensors, (3,), None, 1, 1)
+    for wrong in ((1, 0, [], (), (), None, 1, 1), (1, 0, (), (), None, 1), (1, 0, plan.views, (), (), None, 1, 1),
+                  (1, 0, (), (), ("x",), None, 1, 1), (1, 0, (), (), (), "x", 1, 1)):
         with pytest.raises(TypeError):
             _native.binding().invoke(*wrong)
 

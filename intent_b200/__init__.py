@@ -12,6 +12,9 @@ doors reach them:
 
 Both run the same compile step (``b200-compile``), the same binder
 (``intent_b200.runtime``) and the same kernels; there is no other execution path.
+``intent_b200.ops`` calls the entries directly, and has the operators around a paged
+key-value cache, which the reference does not define: per-head norm with rotation,
+writing and reading the cache, attention of a new token over it.
 ``python -m intent_b200 describe|doctor`` reports the interface and the environment.
 """
 from __future__ import annotations

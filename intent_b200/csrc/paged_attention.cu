@@ -27,6 +27,10 @@
 // and only the result is rounded.  Up to four query heads stand in the columns twice: the first four carry
 // the weights' first halves and the other four the second ones, in one product instead of two.
 //
+// Measured (device time; floors at the 6447 GB/s of a copy): one sequence of 131072 keys, 32 query and 8 key heads
+// of 128 in bf16: 88.6 us (83.3), of which 85 stream at 6.3 TB/s and 4 join; 64 sequences of 100 to 4096 keys: 88.9
+// (82.9); 64 of 1000 to 8192 in e4m3: 103 (94.1); 1024 keys of one sequence: 8.2 us, all latency.
+//
 // 8-bit rows.  Codes become f16 exactly on their way into the products.  The query is scaled by a
 // power of two per row to fit f16; a key's scale multiplies its score.  A value's scale is folded into
 // the weight as exp2(s_j + log2 v_scale_j - M) with M the running maximum of that sum, so the weights

@@ -106,7 +106,8 @@ def build_binding(*, force: bool = False) -> Path:
         libraries = Path(torch.__file__).resolve().parent / "lib"
         _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{path}" for path in includes),
-              str(source), "-o", str(BINDING), f"-L{libraries}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch", "-ltorch_python"])
+              str(source), "-o", str(BINDING), f"-L{libraries}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
+              "-ltorch_python"])
     return BINDING
 
 

@@ -2,7 +2,7 @@
 // (include/intent_b200.h): types, shapes and devices are checked, outputs and scratch allocated, the slots
 // packed and the entry called on torch's current stream, without a Python object a view.  A small call of ten
 // views took 34 us of host time with ctypes and takes 8 this way; many of these kernels run for less.
-#include <ATen/Functions.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -88,10 +88,9 @@ PyObject *invoke(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
           shape[j] = known[PyLong_AsLong(PyTuple_GET_ITEM(symbols, j)) & (kMostSymbols - 1)];
           if (shape[j] < 0) return PyLong_FromSsize_t(-1 - i);
         }
-        fresh = at::empty(at::IntArrayRef(shape, rank),
-                          at::TensorOptions()
-                              .dtype(dtype == Py_None ? call_type : reinterpret_cast<THPDtype *>(dtype)->scalar_type)
-                              .device(at::kCUDA, static_cast<c10::DeviceIndex>(device)));
+        fresh = at::detail::empty_cuda(at::IntArrayRef(shape, rank),
+                                       dtype == Py_None ? call_type : reinterpret_cast<THPDtype *>(dtype)->scalar_type,
+                                       at::Device(at::kCUDA, static_cast<c10::DeviceIndex>(device)), std::nullopt);
         (PyLong_AsLong(PyTuple_GET_ITEM(view, 3)) == kScratch ? scratch : made).push_back(fresh);
       }
       const at::Tensor &tensor = fresh.defined() ? fresh : THPVariable_Unpack(object);

@@ -158,13 +158,13 @@ inline int check_units(const char *what, int64_t tokens, int64_t slices) {
 // such a kernel begins with await_stream() and touches no memory before that, so the stream's order holds; it
 // saves the 2 us that a kernel of a few microseconds otherwise waits for its predecessor's last block.
 template <typename... Parameters, typename... Arguments>
-cudaError_t launch_early(void (*kernel)(Parameters...), unsigned blocks, unsigned threads, size_t smem, cudaStream_t stream,
+cudaError_t launch_early(void (*kernel)(Parameters...), dim3 blocks, unsigned threads, size_t smem, cudaStream_t stream,
                          Arguments... arguments) {
   cudaLaunchAttribute early{};
   early.id = cudaLaunchAttributeProgrammaticStreamSerialization;
   early.val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t config{};
-  config.gridDim = dim3(blocks);
+  config.gridDim = blocks;
   config.blockDim = dim3(threads);
   config.dynamicSmemBytes = smem;
   config.stream = stream;

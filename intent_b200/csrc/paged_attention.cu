@@ -781,8 +781,8 @@ paged_attention_join_kernel(const Problem p) {
   constexpr int kLanes = D / 4, kMost = kJoinThreads / kLanes, kAtOnce = kJoinAtOnce;
   __shared__ float4 part_sums[kMost][kLanes];
   __shared__ float4 part_states[kMost];
-  const int rows = min(p.group, ROWS), lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
-  const int parts = blockDim.x / (kLanes * rows), part = slot / rows, row = slot - part * rows;
+  const int rows = min(p.group, 4), lane = threadIdx.x % kLanes, slot = threadIdx.x / kLanes;
+  const int parts = blockDim.x / (kLanes * rows), part = slot / rows, row = blockIdx.y * 4 + slot - part * rows;
   const int block = blockIdx.x + p.abreast, run = block / p.abreast;   // blocks of the first run have no border
   const Border *border = reinterpret_cast<const Border *>(p.partial + (int64_t)p.runs * p.abreast * 2 * ROWS * partial_floats(D)) + block;
   // What follows is short on purpose: every block meets it cold, and instructions that come from L2 cost more
@@ -827,7 +827,7 @@ paged_attention_join_kernel(const Problem p) {
   }
   const int kv_head = cut.head / p.row_tiles, in_group = (cut.head - kv_head * p.row_tiles) * ROWS + row;
   const int head = kv_head * p.group + in_group;
-  if (part != 0 || in_group >= p.group) return;
+  if (part != 0 || row >= ROWS || in_group >= p.group) return;
   const float base = finite_or_zero(state.top), unit = __fdividef(exp2_fast(finite_or_zero(state.weight_top) - base), state.denominator);
   T *out = static_cast<T *>(p.out) + cut.b * p.out_batch + head * p.out_head + 4 * lane;
   *reinterpret_cast<uint2 *>(out) = make_uint2(pack<T>(state.sum.x * unit, state.sum.y * unit), pack<T>(state.sum.z * unit, state.sum.w * unit));
@@ -876,11 +876,12 @@ template <typename T, int STORE, int D, int ROWS> int launch(const Problem &p, c
   B200_CUDA_TRY(opt_in_dynamic_smem(kernel, bytes));
   B200_CUDA_TRY(heads::launch_early(kernel, p.runs * p.abreast, kBlock, bytes, stream, p));
   if (p.runs == 1) return B200_OK;   // no border
-  // threads for all the pieces that a head has if all are alike, eight to a thread, as far as a block goes
-  const int lanes = (p.group < ROWS ? p.group : ROWS) * D / 4;
+  // four rows a block; threads for all the pieces that a head has if all are alike, eight to a thread, as far
+  // as a block goes
+  const int rows = p.group < ROWS ? p.group : ROWS, lanes = (rows < 4 ? rows : 4) * D / 4;
   const int64_t heads = (int64_t)p.batch * (p.kv_heads * p.row_tiles / p.abreast), want = (p.runs / heads + 2 + kJoinAtOnce - 1) / kJoinAtOnce;
   const int parts = (int)(want < kJoinThreads / lanes ? want : kJoinThreads / lanes);
-  B200_CUDA_TRY(heads::launch_early(paged_attention_join_kernel<T, D, ROWS>, (p.runs - 1) * p.abreast, lanes * parts, 0, stream, p));
+  B200_CUDA_TRY(heads::launch_early(paged_attention_join_kernel<T, D, ROWS>, dim3((p.runs - 1) * p.abreast, (rows + 3) / 4), lanes * parts, 0, stream, p));
   return B200_OK;
 }
 template <typename T, int STORE, int D> int by_rows(const Problem &p, cudaStream_t stream) {

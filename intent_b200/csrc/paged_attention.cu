@@ -9,13 +9,14 @@
 //
 // Work.  The unit is a step: WARPS * KEYS key positions of one (sequence, key head, tile of query heads).  All
 // steps of the call, sequence after sequence, are cut into as many equal runs as there are resident
-// blocks (of several heads abreast, see heads_abreast); a block finds its run by a scan of the lengths and crosses from one sequence to the next
-// without draining its copies.  A ragged batch therefore loads all SMs alike, a single long
+// blocks (of several heads abreast, see heads_abreast); a block finds its run by a scan of the lengths and crosses
+// from one sequence to the next without draining its copies.  A ragged batch therefore loads all SMs alike, a single long
 // sequence is spread over all of them, and a short one is not cut without need.  A piece
 // that is a whole (sequence, head) is finished in place; others leave their unnormalised sums and the
 // maxima they are relative to in `partial`, which a second kernel joins in the order of the blocks
 // (no atomics: results do not vary).  Only the borders between runs cut heads, so that kernel has a
-// block for each border and row, which the run's own note tells what it cuts.
+// block for each border and four rows, which the run's own note tells what it cuts.  Where no sequence can be
+// long, each (sequence, head) is a run, and nothing is joined (see whole_heads).
 //
 // Inside a block every warp is on its own: it copies KEYS rows of K and V with cp.async into its own
 // ring in shared memory (16 bytes a lane, rows past the end zero-filled, so that nothing that an
@@ -29,7 +30,8 @@
 //
 // Measured (device time; floors at the 6447 GB/s of a copy): one sequence of 131072 keys, 32 query and 8 key heads
 // of 128 in bf16: 88.6 us (83.3), of which 85 stream at 6.3 TB/s and 4 join; 64 sequences of 100 to 4096 keys: 88.9
-// (82.9); 64 of 1000 to 8192 in e4m3: 103 (94.1); 1024 keys of one sequence: 8.2 us, all latency.
+// (82.9); 64 of 1000 to 8192 in e4m3: 103 (94.1); 1024 keys of one sequence: 8.2 us, all latency; 8 of up to 300, 32 heads
+// of 64, whole: 7.1.
 //
 // 8-bit rows.  Codes become f16 exactly on their way into the products.  The query is scaled by a
 // power of two per row to fit f16; a key's scale multiplies its score.  A value's scale is folded into
@@ -71,6 +73,7 @@ struct Problem {
   float *partial;
   int batch, kv_heads, group, row_tiles, page_size, pages;
   int runs, abreast;                             // blocks = runs * abreast
+  int whole;                                     // a run is one (sequence, head tile)
   uint32_t page_magic, page_shift, runs_magic;   // for divisions by page_size and by runs
   double inverse_runs;
   int64_t most_keys;                             // slots that a row of the table names
@@ -256,26 +259,6 @@ paged_attention_kernel(const Problem p) {
   // ---- this block's run of steps, which it goes through for one of every `abreast` heads
   const int head_tiles = p.kv_heads * p.row_tiles / p.abreast;
   const int run = blockIdx.x / p.abreast, lane_head = blockIdx.x - run * p.abreast;
-  int64_t total = 0, before = 0, steps_here = 0;
-  for (int base = 0; base < p.batch; base += kBlock) {
-    const int b = base + threadIdx.x;
-    const int given = b < p.batch ? p.lengths[b * p.lengths_step] : 0;
-    const int length = given <= 0 ? 0 : (int)min((int64_t)given, p.most_keys);
-    if (blockIdx.x == 0 && given > p.most_keys) heads::report_index(p.status, b);
-    steps_here = (length + S::kStep - 1) / S::kStep;
-    total += block_scan<kBlock>(steps_here, before, scan_scratch);
-  }
-  total *= head_tiles;
-  // runs of each or each + 1 steps; none is empty, which the join relies on
-  int64_t each = 1;
-  int rest = 0;
-  if (total >= p.runs) {
-    each = (int64_t)((double)total * p.inverse_runs);
-    rest = (int)(total - each * p.runs);
-    if (rest < 0) { --each; rest += p.runs; }
-    if (rest >= p.runs) { ++each; rest -= p.runs; }
-  }
-  Border *border = reinterpret_cast<Border *>(p.partial + (int64_t)gridDim.x * 2 * ROWS * partial_floats(D)) + blockIdx.x;
   // sequences that have not begun
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
     if (p.lengths[b * p.lengths_step] > 0 && p.most_keys > 0) continue;
@@ -285,38 +268,69 @@ paged_attention_kernel(const Problem p) {
     for (int head = threadIdx.x; p.lse && head < p.kv_heads * p.group; head += kBlock)
       p.lse[b * p.lse_batch + head * p.lse_head] = -INFINITY;
   }
-  if (run >= min((int64_t)p.runs, total)) {
-    if (threadIdx.x == 0) border->step = 0;
-    return;
-  }
-  const int64_t begin = run_begin(p, each, rest, run), end = run_begin(p, each, rest, run + 1);
-  int64_t carried = 0;
-  for (int base = 0; base < p.batch; base += kBlock) {
-    const int b = base + threadIdx.x;
-    int64_t sum = total;
-    if (p.batch > kBlock) {   // else the scan above stands
-      steps_here = b < p.batch ? (length_of(p, b) + S::kStep - 1) / S::kStep : 0;
-      sum = block_scan<kBlock>(steps_here, before, scan_scratch) * head_tiles;
-    }
-    const int64_t first = carried + before * head_tiles;
-    if (begin >= first && begin < first + steps_here * head_tiles) {
-      start_b = b;
-      start_rest = begin - first;
-    }
-    carried += sum;
-    if (carried > begin) break;
-  }
-  __syncthreads();
   Place load;             // where the next copies are from
-  load.b = start_b;
-  load.length = length_of(p, load.b);
-  load.steps = (load.length + S::kStep - 1) / S::kStep;
-  load.head = start_rest >> 32 ? (int)(start_rest / load.steps) : (int)((uint32_t)start_rest / (uint32_t)load.steps);
-  load.step = (int)(start_rest - (int64_t)load.head * load.steps);
-  load.head = load.head * p.abreast + lane_head;
-  load.left = end - begin;
+  if (p.whole) {
+    load.b = blockIdx.x / head_tiles;
+    load.head = blockIdx.x - load.b * head_tiles;
+    const int given = p.lengths[load.b * p.lengths_step];
+    if (given > p.most_keys && load.head == 0 && threadIdx.x == 0) heads::report_index(p.status, load.b);
+    load.length = length_of(p, load.b);
+    if (load.length == 0) return;
+    load.left = load.steps = (load.length + S::kStep - 1) / S::kStep;
+    load.step = 0;
+  } else {
+    int64_t total = 0, before = 0, steps_here = 0;
+    for (int base = 0; base < p.batch; base += kBlock) {
+      const int b = base + threadIdx.x;
+      const int given = b < p.batch ? p.lengths[b * p.lengths_step] : 0;
+      const int length = given <= 0 ? 0 : (int)min((int64_t)given, p.most_keys);
+      if (blockIdx.x == 0 && given > p.most_keys) heads::report_index(p.status, b);
+      steps_here = (length + S::kStep - 1) / S::kStep;
+      total += block_scan<kBlock>(steps_here, before, scan_scratch);
+    }
+    total *= head_tiles;
+    // runs of each or each + 1 steps; none is empty, which the join relies on
+    int64_t each = 1;
+    int rest = 0;
+    if (total >= p.runs) {
+      each = (int64_t)((double)total * p.inverse_runs);
+      rest = (int)(total - each * p.runs);
+      if (rest < 0) { --each; rest += p.runs; }
+      if (rest >= p.runs) { ++each; rest -= p.runs; }
+    }
+    Border *border = reinterpret_cast<Border *>(p.partial + (int64_t)gridDim.x * 2 * ROWS * partial_floats(D)) + blockIdx.x;
+    if (run >= min((int64_t)p.runs, total)) {
+      if (threadIdx.x == 0) border->step = 0;
+      return;
+    }
+    const int64_t begin = run_begin(p, each, rest, run), end = run_begin(p, each, rest, run + 1);
+    int64_t carried = 0;
+    for (int base = 0; base < p.batch; base += kBlock) {
+      const int b = base + threadIdx.x;
+      int64_t sum = total;
+      if (p.batch > kBlock) {   // else the scan above stands
+        steps_here = b < p.batch ? (length_of(p, b) + S::kStep - 1) / S::kStep : 0;
+        sum = block_scan<kBlock>(steps_here, before, scan_scratch) * head_tiles;
+      }
+      const int64_t first = carried + before * head_tiles;
+      if (begin >= first && begin < first + steps_here * head_tiles) {
+        start_b = b;
+        start_rest = begin - first;
+      }
+      carried += sum;
+      if (carried > begin) break;
+    }
+    __syncthreads();
+    load.b = start_b;
+    load.length = length_of(p, load.b);
+    load.steps = (load.length + S::kStep - 1) / S::kStep;
+    load.head = start_rest >> 32 ? (int)(start_rest / load.steps) : (int)((uint32_t)start_rest / (uint32_t)load.steps);
+    load.step = (int)(start_rest - (int64_t)load.head * load.steps);
+    load.head = load.head * p.abreast + lane_head;
+    load.left = end - begin;
+    if (threadIdx.x == 0) *border = Border{each, rest, load.b, load.head, load.step, load.steps, 0};
+  }
   Place use = load;       // what the next products take
-  if (threadIdx.x == 0) *border = Border{each, rest, load.b, load.head, load.step, load.steps, 0};
 
   // ---- copies: lane r looks row r of the tile up; a row's 16-byte pieces go to neighbouring lanes
   unsigned char *ring = dynamic_smem + warp * S::kStages * S::kStageBytes;
@@ -745,8 +759,8 @@ paged_attention_kernel(const Problem p) {
 
 // Block y joins the pieces of the head that border y cuts, if it is the first one that does: the runs that
 // hold the head's steps are contiguous, its first piece lies in its run's slot 1 and the others in slot 0.
-// Heads that no border cuts are done.  D / 4 threads take a row, four columns each; more of them take more
-// pieces of it, eight at a time, with a running maximum of their own.
+// Heads that no border cuts are done.  D / 4 threads take a row, four columns each, and a block up to four rows;
+// more threads take more pieces of them, eight at a time, with a running maximum of their own.
 struct State {
   float4 sum;
   float denominator, top, weight_top;
@@ -851,23 +865,37 @@ int heads_abreast(int64_t head_tiles, int64_t resident) {
   return 1;
 }
 
-// As many runs as blocks are resident, or as there can be steps.
+// Whether every (sequence, head tile) gets a block of its own, if the longest sequence that the table has room for is
+// short.  It saves the scan of the lengths, the pieces and the join; against it stands that one block goes through
+// a head's steps alone.  Device time, split / whole, 8 key heads of 128 with 4 query heads on each in bf16:
+// 8 sequences of 128 positions 7.5 / 5.1 us, of 256 8.2 / 7.2, of 512 11.1 / 11.1, of 1024 13.4 / 21.4; one of 256 6.9 / 6.9,
+// of 512 7.4 / 10.8; 64 of up to 512 20.8 / 18.0, of 1024 30.5 / 28.9.  In int8: 8 of 256 8.6 / 6.8, of 512 9.7 / 9.5; one of
+// 512 7.8 / 8.9; 64 of up to 512 19.0 / 17.1.  Heads of 64: one sequence of 256 6.4 / 5.8, of 512 6.6 / 8.7; 32 of up to
+// 512 11.1 / 10.0, of 1024 14.9 / 17.6.  It loses where 16 query heads share codes and there are many: 256 sequences of
+// up to 512 in int8 81 / 85.
+bool whole_heads(int64_t heads, int64_t most_keys, int64_t resident) {
+  return heads < (1 << 30) && most_keys <= (2 * heads < resident ? 256 : 512);
+}
+
+// As many runs as blocks are resident, or as there can be steps; or a run for each (sequence, head tile).
 struct Split {
   int64_t runs, abreast;
+  bool whole;
 };
 Split split_of(int64_t batch, int64_t kv_heads, int64_t group, int64_t most_keys, int store) {
   const int64_t rows = rows_of(group), tiles = kv_heads * ((group + rows - 1) / rows), step = step_of(store);
   const int64_t each = (most_keys + step - 1) / step;
   const int64_t resident = (int64_t)(rows <= 8 ? Shape<cache::kNative, 128, 8>::kBlocksPerSm : Shape<cache::kNative, 128, 16>::kBlocksPerSm) * sm_count();
-  if (batch == 0 || tiles == 0 || each == 0) return {1, 1};
+  if (batch == 0 || tiles == 0 || each == 0) return {1, 1, false};
+  if (whole_heads(batch * tiles, most_keys, resident)) return {batch * tiles, 1, true};
   const int64_t abreast = heads_abreast(tiles, resident), most = resident / abreast, groups = tiles / abreast;
-  if (batch >= most || groups >= most || each >= most || batch * groups >= most) return {most, abreast};
-  return {batch * groups * each < most ? batch * groups * each : most, abreast};
+  if (batch >= most || groups >= most || each >= most || batch * groups >= most) return {most, abreast, false};
+  return {batch * groups * each < most ? batch * groups * each : most, abreast, false};
 }
 
-// Words of scratch: two unfinished pieces and a border a block.
+// Words of scratch: two unfinished pieces and a border a block, if heads are cut.
 int64_t scratch_words(const Split &split, int64_t group, int64_t columns) {
-  return split.runs * split.abreast * (2 * rows_of(group) * partial_floats((int)columns) + (int64_t)(sizeof(Border) / 4));
+  return split.whole ? 0 : split.runs * split.abreast * (2 * rows_of(group) * partial_floats((int)columns) + (int64_t)(sizeof(Border) / 4));
 }
 
 template <typename T, int STORE, int D, int ROWS> int launch(const Problem &p, cudaStream_t stream) {
@@ -875,7 +903,7 @@ template <typename T, int STORE, int D, int ROWS> int launch(const Problem &p, c
   const size_t bytes = Shape<STORE, D, ROWS>::kSmemBytes;
   B200_CUDA_TRY(opt_in_dynamic_smem(kernel, bytes));
   B200_CUDA_TRY(heads::launch_early(kernel, p.runs * p.abreast, kBlock, bytes, stream, p));
-  if (p.runs == 1) return B200_OK;   // no border
+  if (p.runs == 1 || p.whole) return B200_OK;   // no border
   // four rows a block; threads for all the pieces that a head has if all are alike, eight to a thread, as far
   // as a block goes
   const int rows = p.group < ROWS ? p.group : ROWS, lanes = (rows < 4 ? rows : 4) * D / 4;
@@ -953,9 +981,9 @@ extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float s
   const int64_t most_keys = table.d1 * k.d2;
   const int64_t group = q.d1 / k.d1;
   const Split split = split_of(q.d0, k.d1, group, most_keys, store);
-  if (!q.data || !out.data || !lengths.data || (table.d1 && !table.data) || !partial.data)
+  if (!q.data || !out.data || !lengths.data || (table.d1 && !table.data) || (!split.whole && !partial.data))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
-  if (partial.d0 < scratch_words(split, group, q.d2) || partial.s0 != 1 || !aligned16(partial.data))
+  if (!split.whole && (partial.d0 < scratch_words(split, group, q.d2) || partial.s0 != 1 || !aligned16(partial.data)))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the scratch is too short, not contiguous or not 16-byte aligned", what);
   if (!heads::vector_rows(q, 2) || !heads::vector_rows(out, 2))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT,
@@ -982,7 +1010,7 @@ extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float s
   p.batch = (int)q.d0; p.kv_heads = (int)k.d1; p.group = (int)group;
   p.row_tiles = (int)((group + rows_of(group) - 1) / rows_of(group));
   p.page_size = (int)k.d2; p.pages = (int)k.d0;
-  p.runs = (int)split.runs; p.abreast = (int)split.abreast;
+  p.runs = (int)split.runs; p.abreast = (int)split.abreast; p.whole = split.whole;
   p.inverse_runs = 1.0 / (double)split.runs;
   p.runs_magic = (uint32_t)(((int64_t(1) << 32) + split.runs - 1) / split.runs - (split.runs == 1));
   p.most_keys = most_keys;

@@ -297,8 +297,9 @@ _GIVEN, _OUTPUT, _SCRATCH, _OPTIONAL = range(4)
 
 class _Plan:
     """The views of an entry that takes them as one array of slots, in its order.  ``views``: a line for each,
-    "name dtype axis axis ...", where dtype x is the call's own, and axes of one name have one extent.  A name that ends in ``=``
-    is an output, in ``~`` scratch, in ``?`` a view that may be missing.  ``given``: the axes whose extents a call passes."""
+    "name dtype axis axis ...", where dtype x is the call's own, and axes of one name have one extent.  A name that
+    ends in ``=`` is an output, in ``~`` scratch, in ``?`` a view that may be missing.  ``given``: the axes whose
+    extents a call passes."""
 
     def __init__(self, entry: str, views: str, given: str = ""):
         self.entry, self.address = entry, None
@@ -321,8 +322,9 @@ class _Plan:
         return plan
 
     def __call__(self, device: int, tensors: tuple, extents: tuple, number, code: int, other: int) -> tuple:
-        """Calls the entry on the current stream and returns the tensors that were made for it: those given as ``...``.
-        They, and the scratch, are contiguous allocations of the call's own in the stream's order, so calls may overlap."""
+        """Calls the entry on the current stream and returns the tensors that were made for it: those given as
+        ``...``.  They, and the scratch, are contiguous allocations of the call's own in the stream's order, so
+        calls may overlap."""
         if self.address is None:
             self.invoke, self.address = _native.binding().invoke, _native.address(self.entry)
         made = self.invoke(self.address, device, self.views, tensors, extents, number, code, other)
@@ -447,8 +449,8 @@ def head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin
         raise ValueError("q and k are (tokens, heads, head_dim) tensors")
     tokens, heads, head_dim = q.shape
     rows = _scratch_size("b200_head_norm_rotary_scratch", device, tokens, heads, k.shape[1], head_dim)
-    made = _ROTARY_BACKWARD(device, (grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions, ... if dq is None else dq,
-                                     ... if dk is None else dk, ..., ..., ..., _status(device)),
+    made = _ROTARY_BACKWARD(device, (grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions,
+                                     ... if dq is None else dq, ... if dk is None else dk, ..., ..., ..., _status(device)),
                             (rows,), float(epsilon), _CODES[_float_type("q", q)], bool(interleaved))
     return made if len(made) == 4 else _outputs(made, dq, dk, None, None)
 
@@ -462,7 +464,8 @@ _SCALE_VIEWS = """
 
 
 def _by_cache_type(plan: _Plan) -> dict:
-    return {dtype: plan.typed(cache=dtype) for dtype in (torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn)}
+    return {dtype: plan.typed(cache=dtype)
+            for dtype in (torch.float16, torch.bfloat16, torch.int8, torch.float8_e4m3fn)}
 
 
 _WRITE = _by_cache_type(_Plan("b200_cache_write", """
@@ -476,8 +479,8 @@ _READ = _by_cache_type(_Plan("b200_cache_read", _CACHE_VIEWS + """
     k_out= rows tokens kv_heads head_dim
     v_out= rows tokens kv_heads head_dim
     workspace i32 words"""))
-_READ = {(store, rows): plan.typed(rows=rows) for store, plan in _READ.items() for rows in (torch.float16, torch.bfloat16)
-         if store.itemsize == 1 or store is rows}
+_READ = {(store, rows): plan.typed(rows=rows) for store, plan in _READ.items()
+         for rows in (torch.float16, torch.bfloat16) if store.itemsize == 1 or store is rows}
 
 _ATTENTION = _by_cache_type(_Plan("b200_paged_attention", """
     q x batch heads head_dim""" + _CACHE_VIEWS + _SCALE_VIEWS + """
@@ -519,7 +522,8 @@ def cache_write(k, v, slots, k_cache, v_cache, k_scale=None, v_scale=None):
     device = _cuda_device(k)
     rows = _float_type("k", k, (torch.float16, torch.bfloat16))
     store = _cache_type(k_cache, k_scale, v_scale, rows)
-    _WRITE[store](device, (k, v, slots, k_cache, v_cache, k_scale, v_scale, _status(device)), (), None, _CODES[rows], _CODES[store])
+    _WRITE[store](device, (k, v, slots, k_cache, v_cache, k_scale, v_scale, _status(device)), (), None,
+                  _CODES[rows], _CODES[store])
     return k_cache, v_cache
 
 
@@ -536,8 +540,8 @@ def cache_read(k_cache, v_cache, slots, k_scale=None, v_scale=None, *, dtype=Non
         if dtype not in (torch.float16, torch.bfloat16):
             raise TypeError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
         raise TypeError(f"a {store} cache gives its rows as they are, not as {dtype}")
-    made = plan(device, (k_cache, v_cache, slots, k_scale, v_scale, ... if k_out is None else k_out, ... if v_out is None else v_out,
-                         _status(device)), (), None, _CODES[dtype], _CODES[store])
+    made = plan(device, (k_cache, v_cache, slots, k_scale, v_scale, ... if k_out is None else k_out,
+                         ... if v_out is None else v_out, _status(device)), (), None, _CODES[dtype], _CODES[store])
     return made if len(made) == 2 else _outputs(made, k_out, v_out)
 
 
@@ -548,7 +552,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, 
     names in order; both int32.  heads is a multiple of the cache's heads, neighbouring query heads share a key
     head; head_dim is 64 or 128.  A sequence of length 0 gets zeros (and lse -infinity).  What lies behind a
     sequence, in its last page or in the table, is never used.  A page outside the cache is left out, a length
-    past the table is cut there, and ``workspace_status`` reports both.  Returns ``out``, or ``(out, lse)``
+    past the table is cut there, and ``workspace_status`` reports both; a sequence that has lost all its positions
+    gets NaN.  Returns ``out``, or ``(out, lse)``
     with the natural logarithm of the sums (f32)."""
     device = _cuda_device(q)
     rows = _float_type("q", q, (torch.float16, torch.bfloat16))
@@ -562,8 +567,8 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, 
         raise ValueError(f"{heads} query heads are not a multiple of the cache's {kv_heads}")
     words = _scratch_size("b200_paged_attention_scratch", device, batch, heads, kv_heads, head_dim,
                           block_table.shape[1] * page_size, _CODES[store])
-    made = _ATTENTION[store](device, (q, k_cache, v_cache, k_scale, v_scale, block_table, lengths, ... if out is None else out,
-                                      ... if return_lse else None, ..., _status(device)),
+    made = _ATTENTION[store](device, (q, k_cache, v_cache, k_scale, v_scale, block_table, lengths,
+                                      ... if out is None else out, ... if return_lse else None, ..., _status(device)),
                              (words,), float(scale), _CODES[rows], _CODES[store])
     if not return_lse:
         return made[0] if out is None else out

@@ -160,10 +160,10 @@ def test_cache_halves_of_one_allocation_are_taken_apart():
 
 def attend(**change):
     words = ctypes.c_int64()
-    assert _native.entry("b200_paged_attention_scratch")(2, 8, 2, 64, 48, 2, ctypes.byref(words)) == 0
+    assert _native.entry("b200_paged_attention_scratch")(2, 8, 2, 64, 4800, 2, ctypes.byref(words)) == 0
     none3, none2 = [None] + [0] * 6, [None] + [0] * 4
     p = {"q": view(2, 8, 64, address=FAR[0]), "kc": view(9, 2, 16, 64, address=FAR[1]), "vc": view(9, 2, 16, 64, address=FAR[2]),
-         "ks": none3, "vs": none3, "table": view(2, 3), "lengths": view(2), "out": view(2, 8, 64, address=FAR[3]), "lse": none2,
+         "ks": none3, "vs": none3, "table": view(2, 300), "lengths": view(2), "out": view(2, 8, 64, address=FAR[3]), "lse": none2,
          "scale": 0.125, "partial": view(words.value, address=FAR[4]), "space": SPACE, "dtype": 2, "store": 2} | change
     return call("b200_paged_attention", *p.values(), None)
 
@@ -171,7 +171,7 @@ def attend(**change):
 @pytest.mark.parametrize("change, status", [
     ({"dtype": 0}, 1), ({"store": 1}, 1), ({"store": 3}, 1), ({"q": view(2, 7, 64, address=FAR[0])}, 1),
     ({"q": view(2, 8, 32, address=FAR[0])}, 1), ({"out": view(2, 4, 64, address=FAR[3])}, 1), ({"out": view(2, 8, 64, address=FAR[0])}, 1),
-    ({"out": view(2, 8, 64, address=FAR[3], strides=[0, 64, 1])}, 1), ({"table": view(3, 3)}, 1), ({"lengths": view(1)}, 1),
+    ({"out": view(2, 8, 64, address=FAR[3], strides=[0, 64, 1])}, 1), ({"table": view(3, 300)}, 1), ({"lengths": view(1)}, 1),
     ({"lengths": view(2, address=0)}, 1), ({"lse": view(2, 4, address=FAR[5])}, 1), ({"scale": float("inf")}, 1),
     ({"partial": view(16, address=FAR[4])}, 1), ({"partial": view(1 << 20, address=0)}, 1), ({"partial": view(1 << 22, address=FAR[4] + 4)}, 1),
     ({"space": view(3)}, 1), ({"q": view(2, 8, 64, address=FAR[0] + 2)}, 2),
@@ -201,6 +201,8 @@ def test_scratch_entries_check_their_extents():
     size = _native.entry("b200_paged_attention_scratch")
     assert size(2, 8, 3, 64, 10, 2, ctypes.byref(words)) == 1 and size(2, 8, 0, 64, 10, 2, ctypes.byref(words)) == 1
     assert size(1 << 40, 8, 2, 64, 1 << 30, 2, ctypes.byref(words)) == 0 and 0 < words.value < 1 << 24
+    assert size(1 << 40, 8, 2, 64, 10, 2, ctypes.byref(words)) == 0 and 0 < words.value < 1 << 24
+    assert size(2, 8, 2, 64, 10, 2, ctypes.byref(words)) == 0 and words.value == 0     # nothing is cut
     assert _native.entry("b200_head_norm_rotary_scratch")(-1, 8, 2, 64, ctypes.byref(words)) == 1
 
 

@@ -327,6 +327,13 @@ def check_attention(case):
         case["q"], case["k_cache"], case["v_cache"], case["k_scale"], case["v_scale"], case["block_table"], case["lengths"], case["scale"])
     plain.close(out, expected, slack)
     plain.close(lse, expected_lse, lse_slack)
+    page, table = case["k_cache"].shape[2], case["block_table"]
+    if int(case["lengths"].max()) <= table.shape[1] * page:
+        # with room for long sequences behind it, which nothing reads, a table's work is split another way
+        room = torch.full((table.shape[0], 4096 // page + 1), 2 ** 30, dtype=torch.int32, device=DEV)
+        other, other_lse = attend(case | {"block_table": torch.cat([table, room], 1)})
+        plain.close(other, expected, slack)
+        plain.close(other_lse, expected_lse, lse_slack)
     return out, lse
 
 
@@ -343,6 +350,21 @@ ATTEND = [  # lengths, kv_heads, group, page, layout
 @pytest.mark.parametrize("lengths, kv_heads, group, page, layout", ATTEND)
 def test_paged_attention(lengths, kv_heads, group, page, layout, columns, store, dtype):
     check_attention(attention_case(lengths, kv_heads, group, columns, page, dtype, store or dtype, layout, seed=len(lengths) + group))
+    no_status()
+
+
+@pytest.mark.parametrize("store", [F16, I8])
+@pytest.mark.parametrize("columns", [64, 128])
+@pytest.mark.parametrize("batch", [2, 70])
+def test_paged_attention_where_tables_begin_to_be_cut(batch, columns, store):
+    """Tables of as many positions as a block takes by itself, and of one page more, with few and many sequences."""
+    for room in (256, 512):
+        for positions in (room, room + 16):
+            lengths = [positions, 1] + [(i * 131) % positions for i in range(batch - 2)]
+            case = attention_case(lengths, 4, 3, columns, 16, F16, store, "tokens", seed=batch + positions, slack_columns=0)
+            check_attention(case)
+            results = [attend(case) for _ in range(3)]
+            assert all(torch.equal(results[0][0], out) and torch.equal(results[0][1], lse) for out, lse in results)
     no_status()
 
 
@@ -401,6 +423,11 @@ def test_bad_pages_and_lengths_are_left_out_and_reported():
         status_names(1)
     case["block_table"][2, :6] = -1                      # nothing of a sequence is there: no sum at all
     out, lse = attend(case)
+    with pytest.raises(ValueError):
+        ops.workspace_status(DEV)
+    assert out[2].isnan().all() and (lse[2] == -float("inf")).all() and out[0].isfinite().all()
+    room = torch.full((3, 300), -1, dtype=torch.int32, device=DEV)
+    out, lse = attend(case | {"block_table": torch.cat([case["block_table"], room], 1)})
     with pytest.raises(ValueError):
         ops.workspace_status(DEV)
     assert out[2].isnan().all() and (lse[2] == -float("inf")).all() and out[0].isfinite().all()

@@ -450,7 +450,8 @@ def head_norm_rotary_backward(grad_q, grad_k, q, k, q_weight, k_weight, cos, sin
     tokens, heads, head_dim = q.shape
     rows = _scratch_size("b200_head_norm_rotary_scratch", device, tokens, heads, k.shape[1], head_dim)
     made = _ROTARY_BACKWARD(device, (grad_q, grad_k, q, k, q_weight, k_weight, cos, sin, positions,
-                                     ... if dq is None else dq, ... if dk is None else dk, ..., ..., ..., _status(device)),
+                                     ... if dq is None else dq, ... if dk is None else dk, ..., ..., ...,
+                                     _status(device)),
                             (rows,), float(epsilon), _CODES[_float_type("q", q)], bool(interleaved))
     return made if len(made) == 4 else _outputs(made, dq, dk, None, None)
 

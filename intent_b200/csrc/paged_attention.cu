@@ -240,6 +240,67 @@ struct Place {            // where in the sequence of steps a warp is
   }
 };
 
+// Infinities among the values.  A weight is positive however far below the others it lies, so an infinite value gives
+// that infinity; two of both signs give NaN, and so does one under a score of -infinity (0 times it).  The products
+// cannot be trusted with them: a weight enters as two numbers that may be 0 or of both signs.  They turn out NaN then,
+// and a thread that finds one in its four columns goes through the piece's rows again: what comes back is the sum of
+// what is not finite there, 0 if nothing is.  An infinite score needs an infinity (or NaN) in its key or query, and one of
+// +infinity makes the denominator NaN, so such a row under an infinite value leaves NaN in any case.
+__device__ __forceinline__ bool any_special(const void *row, int vectors, uint32_t exponent) {   // exponent: of both halves of a word
+  bool found = false;
+  for (int i = 0; i < vectors; ++i) {
+    const uint4 x = static_cast<const uint4 *>(row)[i];
+    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      found |= (words[j] & exponent & 0xffffu) == (exponent & 0xffffu) || (words[j] & exponent & 0xffff0000u) == (exponent & 0xffff0000u);
+  }
+  return found;
+}
+template <typename T, int D>
+__device__ __forceinline__ float4 special_values(const Problem &p, int b, int kv_head, int head, int column, int begin, int end) {
+  constexpr int kAtOnce = 4;
+  const uint32_t exponent = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+  const bool spoilt = any_special(static_cast<const T *>(p.q) + b * p.q_batch + head * p.q_head, D * 2 / 16, exponent);
+  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll 1
+  for (int key0 = begin; key0 < end; key0 += kAtOnce) {
+    int entry[kAtOnce], offset[kAtOnce];
+    uint2 raw[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int key = min(key0 + i, end - 1), at = key / p.page_size;
+      offset[i] = key - at * p.page_size;
+      entry[i] = p.table[b * p.table_row + at * p.table_column];
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      raw[i] = make_uint2(0, 0);
+      if (key0 + i < end && (uint32_t)entry[i] < (uint32_t)p.pages)
+        raw[i] = *reinterpret_cast<const uint2 *>(p.v + entry[i] * p.v_page + kv_head * p.v_head + offset[i] * p.v_slot + column * 2);
+    }
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const float value[4] = {unpack<T>(raw[i].x, 0), unpack<T>(raw[i].x, 1), unpack<T>(raw[i].y, 0), unpack<T>(raw[i].y, 1)};
+      bool any = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) any |= !(fabsf(value[j]) < INFINITY);
+      if (!any) continue;
+      const bool no_weight = spoilt || any_special(p.k + entry[i] * p.k_page + kv_head * p.k_head + offset[i] * p.k_slot, D * 2 / 16, exponent);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (!(fabsf(value[j]) < INFINITY)) sum[j] += no_weight ? NAN : value[j];
+    }
+  }
+  return make_float4(sum[0], sum[1], sum[2], sum[3]);
+}
+__device__ __forceinline__ bool any_nan(const float4 &x) { return isnan(x.x) || isnan(x.y) || isnan(x.z) || isnan(x.w); }
+// sums, with what is not finite in the place of NaN.
+__device__ __forceinline__ float4 replaced(const float4 &sum, const float4 &special) {
+  return make_float4(special.x != 0.0f ? special.x : sum.x, special.y != 0.0f ? special.y : sum.y, special.z != 0.0f ? special.z : sum.z,
+                     special.w != 0.0f ? special.w : sum.w);
+}
+
 template <typename T, int STORE, int D, int ROWS>
 __global__ void __launch_bounds__(kBlock, (Shape<STORE, D, ROWS>::kBlocksPerSm))
 paged_attention_kernel(const Problem p) {
@@ -711,6 +772,10 @@ paged_attention_kernel(const Problem p) {
           sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
         }
       }
+      if constexpr (!kCodes)
+        if (any_nan(sum) && units[row] < INFINITY)   // the denominator is a number above 0
+          sum = replaced(sum, special_values<T, D>(p, at.b, kv_head, head0 + row, column, piece_first * S::kStep,
+                                                   min((at.step + 1) * S::kStep, at.length)));
       if (whole) {
         const float unit = units[row];
         *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at.b * p.out_batch + (head0 + row) * p.out_head + column) =
@@ -842,6 +907,17 @@ paged_attention_join_kernel(const Problem p) {
   const int kv_head = cut.head / p.row_tiles, in_group = (cut.head - kv_head * p.row_tiles) * ROWS + row;
   const int head = kv_head * p.group + in_group;
   if (part != 0 || row >= ROWS || in_group >= p.group) return;
+  if (any_nan(state.sum) && state.denominator > 0.0f) {
+    // a piece's infinity times a weight that is 0 in f32: what counts is what the pieces hold that is not finite
+    float4 special = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
+#pragma unroll 1
+    for (int i = 0; i < pieces; ++i) {
+      const float4 x = reinterpret_cast<const float4 *>(origin + i * pitch + (i == 0 ? ROWS * partial_floats(D) : 0))[lane];
+      special = make_float4(special.x + (isfinite(x.x) ? 0.0f : x.x), special.y + (isfinite(x.y) ? 0.0f : x.y),
+                            special.z + (isfinite(x.z) ? 0.0f : x.z), special.w + (isfinite(x.w) ? 0.0f : x.w));
+    }
+    state.sum = replaced(state.sum, special);
+  }
   const float base = finite_or_zero(state.top), unit = __fdividef(exp2_fast(finite_or_zero(state.weight_top) - base), state.denominator);
   T *out = static_cast<T *>(p.out) + cut.b * p.out_batch + head * p.out_head + 4 * lane;
   *reinterpret_cast<uint2 *>(out) = make_uint2(pack<T>(state.sum.x * unit, state.sum.y * unit), pack<T>(state.sum.z * unit, state.sum.w * unit));

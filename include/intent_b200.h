@@ -356,8 +356,9 @@ int b200_cache_read(const int64_t *slots, int64_t count, int32_t dtype, int32_t 
  * greater than the table's columns * page_size counts as that, and both are recorded in the
  * workspace; a sequence that has positions, but all of them absent, gets NaN and -infinity.  An infinite
  * value of a 16-bit cache gives that infinity, however small its weight, two of both signs NaN, and so does
- * one under a score of -infinity.  D is 64 or 128; f32 arithmetic, the softmax weights enter the products with 16 bits or
- * more (see the kernel), one rounding at the end; sums are joined in a fixed order, so results do not vary.
+ * one under a score of -infinity.  D is 64 or 128; f32 arithmetic.  The softmax weights enter the products with 16 bits
+ * (bf16 caches), or with 22 but no finer than 2^-43 of the largest (f16 and 8-bit caches; there that is the largest product
+ * of a weight and its row's scale); one rounding at the end; sums are joined in a fixed order, so results do not vary.
  * partial: 16-byte aligned scratch, f32 words as b200_paged_attention_scratch says for this device
  * (keys = table columns * page_size); it may be 0 words, and null then.  Calls that may overlap need scratch of their own each.
  * No counterpart in the reference.

@@ -24,9 +24,12 @@
 // product columns of V) are the 16 rows and query heads the 8 columns, so the group sizes of real
 // models fill the products without padding; tcgen05's smallest tiles would pad them 2 to 16 times and
 // take the weights through shared memory, to speed up what is not the time.  The weights enter the
-// second product as the sum of two halves of 16 bits, so that they count with 22 (f16) or 16 (bf16) bits
-// and only the result is rounded.  Up to four query heads stand in the columns twice: the first four carry
-// the weights' first halves and the other four the second ones, in one product instead of two.
+// second product as the sum of two halves of 16 bits, so that they count with 16 bits (bf16) or with 22, and with
+// 2^-43 of the largest where those are finer (f16: the products of f16 rows and of codes, see kLift); the result is
+// rounded once.  Up to four query heads stand in the columns twice: the first four carry
+// the weights' first halves and the other four the second ones, in one product instead of two.  Second halves are
+// scaled in f16; more heads add them apart for that, which costs 8-bit rows of 8 and 16 query heads 2 to 6 % (32 sequences of
+// 4096 keys, 16 heads on each of 8 key heads in e4m3: 75 to 79 us) and 16-bit ones nothing.
 //
 // Measured (device time; floors at the 6447 GB/s of a copy): one sequence of 131072 keys, 32 query and 8 key heads
 // of 128 in bf16: 88.6 us (83.3), of which 85 stream at 6.3 TB/s and 4 join; 64 sequences of 100 to 4096 keys: 88.9
@@ -77,7 +80,7 @@ struct Problem {
   uint32_t page_magic, page_shift, runs_magic;   // for divisions by page_size and by runs
   double inverse_runs;
   int64_t most_keys;                             // slots that a row of the table names
-  float scale_log2e;
+  float scale_log2e, lift;
   int *status;
 };
 
@@ -97,6 +100,13 @@ template <int STORE, int D, int ROWS> struct Shape {
   static constexpr int kSmemBytes = kRingBytes + kWarps * kColumns * 16 + ROWS * 4;
   static_assert(kColumns * D * 4 <= kStageBytes, "a warp's sums fit the stage that it has just used");
 };
+// Weights of the products, relative to the running maximum, are 2^lift times what they stand for, and their second halves
+// kRest times: f16 has room up to 2^15 above (the maximum lags by up to 2^8) and none below 2^-24.  Second halves then
+// keep what is above 2^-36, and a weight is off by at most 2^-43 of the largest, or 2^-23 of itself.  Without,
+// the ends of a softmax were lost behind a key that holds nearly all of it: by 23 % if they lie 2^26 below.
+template <typename M> constexpr bool kHalf = std::is_same<M, __half>::value;
+template <typename M> constexpr float kLift = kHalf<M> ? 7.0f : 0.0f;
+template <typename M> constexpr float kRest = kHalf<M> ? 2048.0f : 1.0f;
 constexpr int partial_floats(int columns) { return columns + 4; }   // sums, m, l, M, unused
 
 // What a run begins with, for the kernel that joins: (sequence, head tile) and how many of its steps lie
@@ -648,8 +658,8 @@ paged_attention_kernel(const Problem p) {
     uint32_t high[kTiles][kHeads][2], rest[kTiles][kHeads][2];   // head g, keys 16 t + 2 c, + 1 and + 8, + 9
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
-      const float base[2] = {finite_or_zero(m[h][0]), finite_or_zero(m[h][1])};
-      const float weight_base[2] = {finite_or_zero(weight_max[h][0]), finite_or_zero(weight_max[h][1])};
+      const float base[2] = {finite_or_zero(m[h][0]) - kLift<M>, finite_or_zero(m[h][1]) - kLift<M>};
+      const float weight_base[2] = {finite_or_zero(weight_max[h][0]) - kLift<M>, finite_or_zero(weight_max[h][1]) - kLift<M>};
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -662,12 +672,22 @@ paged_attention_kernel(const Problem p) {
             // log2 of a masked key's zero scale is -infinity: its weight is 0
             if constexpr (kCodes) w[j] = exp2_fast(s[t][h][2 * k + j] + log_scale[t][k] - weight_base[j]);
           }
-          const uint32_t pair = pack<M>(w[0], w[1]), left = pack<M>(w[0] - unpack<M>(pair, 0), w[1] - unpack<M>(pair, 1));
+          const uint32_t pair = pack<M>(w[0], w[1]), left = pack<M>((w[0] - unpack<M>(pair, 0)) * kRest<M>, (w[1] - unpack<M>(pair, 1)) * kRest<M>);
           high[t][h][k] = transposed(kTwice && c >= 2 ? left : pair);
           if constexpr (!kTwice) rest[t][h][k] = transposed(left);
         }
     }
     // sums += values (transposed) . weights
+    auto add_rest = [](float (&to)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, const uint32_t (&b)[2]) {
+      if constexpr (kRest<M> == 1.0f) {
+        multiply<M>(to, a0, a1, a2, a3, b[0], b[1]);
+      } else {
+        float apart[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+        multiply<M>(apart, a0, a1, a2, a3, b[0], b[1]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) to[j] = fmaf(apart[j], 1.0f / kRest<M>, to[j]);
+      }
+    };
 #pragma unroll
     for (int t = 0; t < kTiles; ++t) {
 #pragma unroll
@@ -680,7 +700,7 @@ paged_attention_kernel(const Problem p) {
           for (int h = 0; h < kHeads; ++h) multiply<M>(sums[i][h], r[0], r[1], r[2], r[3], high[t][h][0], high[t][h][1]);
           if constexpr (!kTwice) {
 #pragma unroll
-            for (int h = 0; h < kHeads; ++h) multiply<M>(sums[i][h], r[0], r[1], r[2], r[3], rest[t][h][0], rest[t][h][1]);
+            for (int h = 0; h < kHeads; ++h) add_rest(sums[i][h], r[0], r[1], r[2], r[3], rest[t][h]);
           }
         } else {                      // a 16-bit unit holds two neighbouring columns: even ones are rows 0 .. 7, odd ones 8 .. 15
           uint32_t v[2][4];
@@ -698,8 +718,7 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
             for (int h = 0; h < kHeads; ++h)
 #pragma unroll
-              for (int j = 0; j < 2; ++j)
-                multiply<M>(sums[2 * i + j][h], v[j][0], v[j][1], v[j][2], v[j][3], rest[t][h][0], rest[t][h][1]);
+              for (int j = 0; j < 2; ++j) add_rest(sums[2 * i + j][h], v[j][0], v[j][1], v[j][2], v[j][3], rest[t][h]);
           }
         }
       }
@@ -729,7 +748,8 @@ paged_attention_kernel(const Problem p) {
         float weight_top = weight_max[h][j];
 #pragma unroll
         for (int w = 1; w < kWarps; ++w) weight_top = fmaxf(weight_top, stats[(warp ^ w) * S::kColumns + row].z);
-        const float shrink = exp2_fast(weight_max[h][j] - finite_or_zero(weight_top));
+        float shrink = exp2_fast(weight_max[h][j] - finite_or_zero(weight_top));
+        if (kTwice && c >= 2) shrink *= 1.0f / kRest<M>;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
 #pragma unroll
@@ -754,7 +774,7 @@ paged_attention_kernel(const Problem p) {
       for (int w = 0; w < kWarps; ++w) denominator += state[w].y * exp2_fast(state[w].x - base);
       units[row] = __fdiv_rn(kCodes ? exp2_fast(finite_or_zero(weight_top) - base) : 1.0f, denominator);
       if (whole) {
-        if (p.lse) p.lse[at.b * p.lse_batch + (head0 + row) * p.lse_head] = (base + log2f(denominator)) * kLn2;
+        if (p.lse) p.lse[at.b * p.lse_batch + (head0 + row) * p.lse_head] = (base - kLift<M> + log2f(denominator)) * kLn2;
       } else {
         *reinterpret_cast<float4 *>(to + row * partial_floats(D) + D) = make_float4(top, denominator, weight_top, 0.0f);
       }
@@ -921,7 +941,7 @@ paged_attention_join_kernel(const Problem p) {
   const float base = finite_or_zero(state.top), unit = __fdividef(exp2_fast(finite_or_zero(state.weight_top) - base), state.denominator);
   T *out = static_cast<T *>(p.out) + cut.b * p.out_batch + head * p.out_head + 4 * lane;
   *reinterpret_cast<uint2 *>(out) = make_uint2(pack<T>(state.sum.x * unit, state.sum.y * unit), pack<T>(state.sum.z * unit, state.sum.w * unit));
-  if (lane == 0 && p.lse) p.lse[cut.b * p.lse_batch + head * p.lse_head] = (base + __log2f(state.denominator)) * kLn2;
+  if (lane == 0 && p.lse) p.lse[cut.b * p.lse_batch + head * p.lse_head] = (base - p.lift + __log2f(state.denominator)) * kLn2;
 }
 
 // --------------------------------------------------------------------- host
@@ -1094,6 +1114,7 @@ extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float s
   while ((int64_t(1) << p.page_shift) < k.d2) ++p.page_shift;
   if (k.d2) p.page_magic = (uint32_t)(((int64_t(1) << 32) * ((int64_t(1) << p.page_shift) - k.d2)) / k.d2 + 1);
   p.scale_log2e = scale * kLog2e;
+  p.lift = store == B200_BF16 ? kLift<__nv_bfloat16> : kLift<__half>;
   p.status = static_cast<int *>(const_cast<void *>(workspace.data));
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   return dtype == B200_F16 ? by_store<__half>(p, store, (int)q.d2, s) : by_store<__nv_bfloat16>(p, store, (int)q.d2, s);

@@ -76,3 +76,43 @@ def test_an_infinite_value_gives_that_infinity(length, room, group, dtype):
         out, lse = attend(q, case, 0.125)
         assert out[0, group:, 20].isnan().all() and lse.isfinite().all() and (out[0, :group, 3] == inf).all()
         assert out[0, group:, :20].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype, store", [(F16, F16), (BF16, BF16), (F16, I8), (BF16, E4M3)])
+@pytest.mark.parametrize("group", [1, 4, 7, 16])
+@pytest.mark.parametrize("length, room", [(450, 0), (4096, 0), (4096, 8000)])
+def test_small_weights_behind_a_sink_count(length, room, group, dtype, store):
+    """One key takes nearly all of the softmax and its value is zero but for one column, so the others are what all the other
+    keys hold, each 24 to 32 powers of two below it.  A weight enters as two halves, the second 2^-11 of the first's steps: in f16 (the products of f16
+    rows and of codes) that keeps what is above 2^-36, with the largest weight at 2^7 or more, so each is off
+    by at most 2^-43 of the largest (times its row's scale over the largest product's), beside 2^-16 of itself."""
+    scale = 1 / 16
+    for below in (24.0, 26.0, 32.0):
+        k, v = torch.zeros(length, 1, 128, device=DEV), randn(length, 1, 128, seed=3) + 0.5
+        k[:, 0, 0] = -(below + 1.0 * (torch.rand(length, generator=torch.Generator().manual_seed(int(below))).to(DEV) - 0.5)) * math.log(2.0)
+        k[1, 0, 0], v[1] = 0.0, 0.0
+        v[1, 0, 0] = 1.0
+        q = torch.zeros(1, group, 128, device=DEV)
+        q[..., 0] = 1 / scale
+        q = q.to(dtype)
+        case = one_sequence(k, v, group, dtype, store, room=room)
+        out, lse = attend(q, case, scale)
+        rows = []
+        for cache, size in ((case["k_cache"], case["k_scale"]), (case["v_cache"], case["v_scale"])):
+            wide = plain.values(cache, size)[case["block_table"][0, :-(-length // 16)].long()]
+            rows.append(wide.permute(1, 0, 2, 3).reshape(-1, 128)[:length])
+        scores = rows[0] @ q[0, 0].double() * scale
+        weights = torch.softmax(scores, 0)
+        sizes = torch.ones(length, dtype=torch.float64, device=DEV)
+        if case["v_scale"] is not None:
+            sizes = case["v_scale"][case["block_table"][0, :-(-length // 16)].long()].double().reshape(-1)[:length]
+        expected = (weights[:, None] * rows[1]).sum(0)
+        # a score of magnitude 33 is rounded once from its product and once when scaled (2^-24 each, of 33 log2 e), and the
+        # difference to the base once more; exp2 and log2 add 2^-20
+        delta = 4 * 48 * plain.F32 + 2.0 ** -20
+        size = (weights[:, None] * rows[1].abs()).sum(0)
+        slack = (2 * delta + 2.0 ** -16 + (length / 64 + 64) * plain.F32) * size
+        if store != BF16:
+            slack = slack + 2.0 ** -43 * (weights * sizes).amax() * (rows[1].abs() / sizes[:, None]).sum(0)
+        plain.close(out, expected.expand(1, group, 128), slack)
+        plain.close(lse, torch.logsumexp(scores, 0).expand(1, group), delta + (length / 64 + 64) * plain.F32)

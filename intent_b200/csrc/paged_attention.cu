@@ -104,8 +104,10 @@ template <int STORE, int D, int ROWS> struct Shape {
 // kRest times: f16 has room up to 2^15 above (the maximum lags by up to 2^8) and none below 2^-24.  Second halves then
 // keep what is above 2^-36, and a weight is off by at most 2^-43 of the largest, or 2^-23 of itself.  Without,
 // the ends of a softmax were lost behind a key that holds nearly all of it: by 23 % if they lie 2^26 below.
+// bf16 has no end there but one above: its largest numbers times a weight of more than 1 are infinite, so its weights stand
+// lower by the 2^8 that the maximum may lag.
 template <typename M> constexpr bool kHalf = std::is_same<M, __half>::value;
-template <typename M> constexpr float kLift = kHalf<M> ? 7.0f : 0.0f;
+template <typename M> constexpr float kLift = kHalf<M> ? 7.0f : -8.0f;
 template <typename M> constexpr float kRest = kHalf<M> ? 2048.0f : 1.0f;
 constexpr int partial_floats(int columns) { return columns + 4; }   // sums, m, l, M, unused
 
@@ -615,7 +617,7 @@ paged_attention_kernel(const Problem p) {
             for (int h = 0; h < kHeads; ++h) s[t][h][2 * k] = s[t][h][2 * k + 1] = -INFINITY;
     }
     // The bases m and weight_max move only when a score passes them by more than 8 (log2 units): until then
-    // weights reach 2^8, well inside every type here.
+    // weights reach 2^8 times what they stand for at the most, which kLift leaves room for.
     bool grown = false;
 #pragma unroll
     for (int h = 0; h < kHeads; ++h)

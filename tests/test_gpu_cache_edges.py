@@ -116,3 +116,20 @@ def test_small_weights_behind_a_sink_count(length, room, group, dtype, store):
             slack = slack + 2.0 ** -43 * (weights * sizes).amax() * (rows[1].abs() / sizes[:, None]).sum(0)
         plain.close(out, expected.expand(1, group, 128), slack)
         plain.close(lse, torch.logsumexp(scores, 0).expand(1, group), delta + (length / 64 + 64) * plain.F32)
+
+
+@pytest.mark.parametrize("group", [1, 7, 16])
+@pytest.mark.parametrize("length, room", [(200, 0), (3000, 0)])
+def test_values_near_the_end_of_bf16(length, room, group):
+    """The largest numbers of bf16, under scores that rise slowly: a weight is at most 1, whatever the base was when it came."""
+    k, v = torch.zeros(length, 1, 64, device=DEV), torch.zeros(length, 1, 64, device=DEV)
+    k[:, 0, 0] = torch.linspace(0, 5, length, device=DEV)             # 7.2 in units of log2: the base does not follow
+    v[length - 2, 0, :32], v[length - 1, 0, 32:], v[0, 0, 5] = -3.3e38, 3.3e38, 3e38
+    q = torch.zeros(1, group, 64, device=DEV, dtype=BF16)
+    q[..., 0] = 1
+    case = one_sequence(k, v, group, BF16, BF16, room=room)
+    out, lse = attend(q, case, 1.0)
+    expected, slack, expected_lse, lse_slack = plain.attention(q, case["k_cache"], case["v_cache"], None, None, case["block_table"],
+                                                               case["lengths"], 1.0)
+    plain.close(out, expected, slack)
+    plain.close(lse, expected_lse, lse_slack)

@@ -354,7 +354,8 @@ int b200_cache_read(const int64_t *slots, int64_t count, int32_t dtype, int32_t 
  * past a sequence's length is read into a result, whatever it holds; entries of block_table past it may have any
  * value.  An entry within it that is no page counts its positions as absent, a length
  * greater than the table's columns * page_size counts as that, and both are recorded in the
- * workspace; a sequence that has positions, but all of them absent, gets NaN and -infinity.  An infinite
+ * workspace; a sequence that has positions, but all of them absent (if the table has no columns, too), gets NaN and
+ * -infinity.  An infinite
  * value of a 16-bit cache gives that infinity, however small its weight, two of both signs NaN, and so does
  * one under a score of -infinity.  D is 64 or 128; f32 arithmetic.  The softmax weights enter the products with 16 bits
  * (bf16 caches), or with 22 but no finer than 2^-43 of the largest (f16 and 8-bit caches; there that is the largest product

@@ -332,12 +332,13 @@ paged_attention_kernel(const Problem p) {
   // ---- this block's run of steps, which it goes through for one of every `abreast` heads
   const int head_tiles = p.kv_heads * p.row_tiles / p.abreast;
   const int run = blockIdx.x / p.abreast, lane_head = blockIdx.x - run * p.abreast;
-  // sequences that have not begun
+  // sequences that have not begun, and those of a table that names no slot: all that they hold is absent
   for (int b = blockIdx.x; b < p.batch; b += gridDim.x) {
-    if (p.lengths[b * p.lengths_step] > 0 && p.most_keys > 0) continue;
+    const bool begun = p.lengths[b * p.lengths_step] > 0;
+    if (begun && p.most_keys > 0) continue;
     T *out = static_cast<T *>(p.out) + b * p.out_batch;
     for (int index = threadIdx.x; index < p.kv_heads * p.group * D; index += kBlock)
-      out[(index / D) * p.out_head + index % D] = Element<T>::narrow(0.0f);
+      out[(index / D) * p.out_head + index % D] = Element<T>::narrow(begun ? NAN : 0.0f);
     for (int head = threadIdx.x; p.lse && head < p.kv_heads * p.group; head += kBlock)
       p.lse[b * p.lse_batch + head * p.lse_head] = -INFINITY;
   }

@@ -133,3 +133,13 @@ def test_values_near_the_end_of_bf16(length, room, group):
                                                                case["lengths"], 1.0)
     plain.close(out, expected, slack)
     plain.close(lse, expected_lse, lse_slack)
+
+
+def test_a_table_without_columns_has_lost_what_a_sequence_holds():
+    q = randn(3, 4, 64, dtype=F16)
+    case = one_sequence(randn(20, 2, 64), randn(20, 2, 64), 2, F16, F16)
+    out, lse = ops.paged_attention(q, case["k_cache"], case["v_cache"], case["block_table"].expand(3, -1)[:, :0], int32([0, 5, -3]), 0.125,
+                                   return_lse=True)
+    with pytest.raises(ValueError, match=r"\(row 1\)"):
+        ops.workspace_status(DEV)
+    assert not out[0].any() and not out[2].any() and out[1].isnan().all() and (lse == -float("inf")).all()

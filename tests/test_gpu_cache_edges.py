@@ -143,3 +143,31 @@ def test_a_table_without_columns_has_lost_what_a_sequence_holds():
     with pytest.raises(ValueError, match=r"\(row 1\)"):
         ops.workspace_status(DEV)
     assert not out[0].any() and not out[2].any() and out[1].isnan().all() and (lse == -float("inf")).all()
+
+
+# ------------------------------------------------------------------------ norm and rotation
+def rotary_inputs(tokens, heads, kv_heads, columns, pairs, dtype, seed=0):
+    both = randn(tokens, heads + kv_heads + 1, columns, dtype=dtype, seed=seed)
+    w = (1 + 0.3 * randn(2, columns, seed=seed + 1)).to(dtype)
+    angle = torch.rand(64, pairs, device=DEV, dtype=torch.float64, generator=torch.Generator(device=DEV).manual_seed(seed)) * 7
+    positions = torch.arange(tokens, device=DEV, dtype=torch.int32) * 7 % 64
+    return both[:, :heads], both[:, heads:heads + kv_heads], w[0], w[1], angle.cos().float(), angle.sin().float(), positions
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_padding_gets_zero_gradients_under_any_weight(dtype):
+    q, k, qw, kw, cos, sin, positions = rotary_inputs(40, 4, 2, 64, 16, dtype, seed=3)
+    clean = ops.head_norm_rotary_backward(q, k, q, k, qw, kw, cos, sin, positions)
+    positions[::3] = -1
+    positions[31] = 64
+    qw[5], qw[40], kw[20] = float("inf"), float("nan"), -float("inf")
+    grads = ops.head_norm_rotary_backward(q, k, q, k, qw, kw, cos, sin, positions)
+    with pytest.raises(ValueError, match=r"\(row 31\)"):
+        ops.workspace_status(DEV)
+    absent = (positions < 0) | (positions > 63)
+    assert not grads[0][absent].any() and not grads[1][absent].any()
+    assert grads[0][~absent].isnan().all() and clean[0].isfinite().all()
+    # the weights' gradients do not depend on the weights
+    for i, (g, x, w) in enumerate(((q, q, qw), (k, k, kw))):
+        _, _, dw, dw_slack = plain.norm_rotary_backward(g, x, torch.ones_like(w), cos, sin, positions, 1e-6, False)
+        plain.close(grads[2 + i], dw, dw_slack)

@@ -4,6 +4,7 @@
 // views took 34 us of host time with ctypes and takes 6.4 this way; many of these kernels run for less.
 #include <ATen/cuda/EmptyTensor.h>
 #include <torch/csrc/Dtype.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include <c10/cuda/CUDAGuard.h>
@@ -35,7 +36,7 @@ PyObject *invoke(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     PyErr_SetString(PyExc_TypeError, "invoke(entry, device, plan, tensors, extents, number, code, other)");
     return nullptr;
   }
-  try {
+  HANDLE_TH_ERRORS   // an allocation that fails becomes torch.OutOfMemoryError, as it does of torch's own
     void *entry = PyLong_AsVoidPtr(arguments[0]);
     const long device = PyLong_AsLong(arguments[1]);
     PyObject *plan = arguments[2], *tensors = arguments[3], *extents = arguments[4];
@@ -111,10 +112,7 @@ PyObject *invoke(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
     PyObject *result = PyTuple_New(static_cast<Py_ssize_t>(made.size()));
     for (size_t i = 0; result && i < made.size(); ++i) PyTuple_SET_ITEM(result, static_cast<Py_ssize_t>(i), THPVariable_Wrap(made[i]));
     return result;
-  } catch (const std::exception &error) {
-    if (!PyErr_Occurred()) PyErr_SetString(PyExc_RuntimeError, error.what());
-    return nullptr;
-  }
+  END_HANDLE_TH_ERRORS
 }
 
 PyMethodDef methods[] = {

@@ -171,3 +171,14 @@ def test_padding_gets_zero_gradients_under_any_weight(dtype):
     for i, (g, x, w) in enumerate(((q, q, qw), (k, k, kw))):
         _, _, dw, dw_slack = plain.norm_rotary_backward(g, x, torch.ones_like(w), cos, sin, positions, 1e-6, False)
         plain.close(grads[2 + i], dw, dw_slack)
+
+
+# ----------------------------------------------------------------------------------- the call
+def test_an_output_that_does_not_fit_raises_torchs_error():
+    """275 GB of rows: what catches torch.OutOfMemoryError to make room catches this."""
+    cache = torch.zeros(1, 64, 1, 128, dtype=F16, device=DEV)
+    slots = torch.zeros(1, dtype=torch.int64, device=DEV).expand(1 << 24)
+    with pytest.raises(torch.OutOfMemoryError):
+        ops.cache_read(cache, cache, slots)
+    back = ops.cache_read(cache, cache, slots[:3])
+    assert back[0].shape == (3, 64, 128) and not back[0].any()

@@ -395,11 +395,10 @@ head_norm_rotary_backward_kernel(Operand q, Operand k, Rotation r, int unit_rows
         for (int i = 0; i < 8; ++i)
           g.own[i] = mul(fma(x.own[i], Two{projection, projection}, g.own[i]), Two{rstd, rstd});
         Eight<T> a, b;
+        g.narrow(a, b);
         if (position < 0) {   // 0 times a weight may be NaN
           a.clear();
           b.clear();
-        } else {
-          g.narrow(a, b);
         }
         a.store(target + row * o.out_head + first);
         b.store(target + row * o.out_head + second);

@@ -49,7 +49,7 @@ extern "C" {
 #define B200_E4M3 4
 
 /* Number of int32 words every workspace view must hold (zero-initialised by
-   the caller once; word 0 is a sticky device-side status, see b200_workspace_status). */
+   the caller once; words 0 and 4 are sticky device-side reports, see b200_workspace_status). */
 #define B200_WORKSPACE_WORDS 64
 
 int b200_abi_version(void);
@@ -442,12 +442,12 @@ int b200_gather_probe(const void *table, int64_t table_rows, int64_t gathers, in
 int b200_selftest_bounded_wait(void *workspace, int64_t ws_d0, int64_t ws_s0, int64_t limit_cycles, void *stream);
 
 /*
- * Reads word 0 of a workspace after synchronising `stream`: B200_OK,
- * B200_ERR_DEVICE_TIMEOUT when a bounded wait inside a kernel gave up, or
+ * Reads the reports of a workspace after synchronising `stream`: B200_OK,
+ * B200_ERR_DEVICE_TIMEOUT when a bounded wait inside a kernel gave up (word 0), or
  * B200_ERR_INVALID_ARGUMENT when a kernel met a position, slot, page or length outside
- * its table or cache and left it out.
- * `detail` (may be null) receives word 1, which names the wait that ran out, or the
- * token or sequence.
+ * its table or cache and left it out (word 4); of both, the wait is what is returned.
+ * `detail` (may be null) receives the word after it, which names the wait that ran out, or the
+ * token or sequence.  The words stay as they are: the caller clears the workspace.
  */
 int b200_workspace_status(const void *workspace, int32_t *detail, void *stream);
 

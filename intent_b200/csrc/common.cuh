@@ -10,6 +10,9 @@
 
 namespace b200 {
 
+// Words of a workspace that report an index outside its table or cache (words 0 and 1: tc.cuh, word 2: spmm.cu).
+constexpr int kBadIndex = 4;
+
 // ---- host side: status + last-error text --------------------------------
 int fail(int status, const char *format, ...);
 int cuda_fail(cudaError_t error, const char *what);

@@ -180,10 +180,10 @@ __device__ __forceinline__ void await_stream() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
-// Word 0 of the workspace becomes 3 and word 1 the position of a bad index (b200_workspace_status
-// reports it); the first one found stays.
+// Word kBadIndex of the workspace becomes 1 and the next one the position of a bad index (b200_workspace_status
+// reports it); the first one found stays.  Words 0 and 1 belong to waits that give up, which a bad index must not hide.
 __device__ __forceinline__ void report_index(int *status, int position) {
-  if (atomicCAS(status, 0, 3) == 0) status[1] = position;
+  if (atomicCAS(status + kBadIndex, 0, 1) == 0) status[kBadIndex + 1] = position;
 }
 
 // Two f32 at a time (one instruction each on this part).

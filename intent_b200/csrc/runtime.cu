@@ -92,17 +92,19 @@ extern "C" int b200_device_check(int device) {
 
 extern "C" int b200_workspace_status(const void *workspace, int32_t *detail, void *stream) {
   if (!workspace) return fail(B200_ERR_INVALID_ARGUMENT, "workspace_status: null workspace");
-  int32_t words[2] = {0, 0};
+  int32_t words[kBadIndex + 2] = {};
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   B200_CUDA_TRY(cudaMemcpyAsync(words, workspace, sizeof words, cudaMemcpyDeviceToHost, s));
   B200_CUDA_TRY(cudaStreamSynchronize(s));
   if (detail) *detail = words[1];
   if (words[0] == 2)   // only the checked build (-DB200_CHECKED) writes this
     return fail(B200_ERR_INVALID_ARGUMENT, "checked build: an index or offset was outside its array (row %d)", words[1]);
-  if (words[0] == 3)   // head_norm_rotary, cache_write / cache_read, paged_attention
-    return fail(B200_ERR_INVALID_ARGUMENT, "a position, slot, page or length was outside its table or cache (row %d)", words[1]);
   if (words[0] != 0)
     return fail(B200_ERR_DEVICE_TIMEOUT, "a bounded device-side wait gave up (site %d)", words[1]);
+  if (words[kBadIndex] != 0) {   // head_norm_rotary, cache_write / cache_read, paged_attention
+    if (detail) *detail = words[kBadIndex + 1];
+    return fail(B200_ERR_INVALID_ARGUMENT, "a position, slot, page or length was outside its table or cache (row %d)", words[kBadIndex + 1]);
+  }
   return B200_OK;
 }
 

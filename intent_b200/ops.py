@@ -78,7 +78,8 @@ def workspace(device: torch.device) -> torch.Tensor:
 
 
 def workspace_status(device: torch.device) -> None:
-    """Synchronise and raise if a bounded device-side wait gave up."""
+    """Synchronise and raise if a bounded device-side wait gave up (``NativeCallError``), or else if a position, slot,
+    page or length was outside its table or cache (``ValueError``).  What was raised is cleared."""
     ws = workspace(device)
     detail = ctypes.c_int32(0)
     with torch.cuda.device(ws.device):

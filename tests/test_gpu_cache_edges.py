@@ -182,3 +182,28 @@ def test_an_output_that_does_not_fit_raises_torchs_error():
         ops.cache_read(cache, cache, slots)
     back = ops.cache_read(cache, cache, slots[:3])
     assert back[0].shape == (3, 64, 128) and not back[0].any()
+
+
+def test_a_bad_index_does_not_hide_a_wait_that_gave_up():
+    cache = torch.zeros(1, 1, 16, 64, dtype=F16, device=DEV)
+    rows, far = randn(2, 1, 64, dtype=F16), torch.tensor([1, 99], device=DEV)
+
+    def bad_slot():
+        ops.cache_write(rows, rows, far, cache, cache.clone())
+
+    def wait_that_gives_up():
+        space = ops.workspace(DEV)
+        status = _native.entry("b200_selftest_bounded_wait")(space.data_ptr(), space.numel(), 1, 100_000, torch.cuda.current_stream().cuda_stream)
+        _native.check("b200_selftest_bounded_wait", status)
+
+    for first, second in ((bad_slot, wait_that_gives_up), (wait_that_gives_up, bad_slot)):
+        first()
+        second()
+        with pytest.raises(_native.NativeCallError) as error:
+            ops.workspace_status(DEV)
+        assert error.value.status == _native.ERR_DEVICE_TIMEOUT
+        ops.workspace_status(DEV)
+    bad_slot()
+    with pytest.raises(ValueError, match=r"\(row 1\)"):
+        ops.workspace_status(DEV)
+    ops.workspace_status(DEV)

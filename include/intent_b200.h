@@ -300,7 +300,7 @@ int b200_flash_attention(const void *q, int64_t q_d0, int64_t q_d1, int64_t q_d2
  * position behind the tables, which is also recorded in the workspace (b200_workspace_status).
  * D a multiple of 16 in [16, 256], pairs a multiple of 8; unit inner strides, 16-byte aligned bases,
  * outer strides of whole 16-byte steps.  An output may be its own input view, and otherwise overlaps
- * no operand.  q and k may be slices of one tensor, and so may the outputs.
+ * no operand; views that interleave with equal longest steps do not overlap.  q and k may be slices of one tensor, and so may the outputs.
  * slots: q 3, k 3, q_weight 1, k_weight 1, cosine 2, sine 2, positions 1, q_out 3, k_out 3, workspace 1.
  */
 int b200_head_norm_rotary(const int64_t *slots, int64_t count, float epsilon, int32_t dtype, int32_t interleaved, void *stream);
@@ -330,7 +330,8 @@ int b200_head_norm_rotary_backward(const int64_t *slots, int64_t count, float ep
  *   scale NaN and codes 0.
  * A negative slot marks padding, whose row is not written; nor is the row of a slot behind the cache,
  * which is recorded in the workspace.  The slots of one call that are not negative must differ: what a
- * slot holds that is named twice is unspecified.  D a multiple of 16 in [16, 256]; unit inner strides,
+ * slot holds that is named twice is unspecified.  Nothing that is written overlaps another operand (codes may lie
+ * beside their scales in one allocation, page for page or row for row).  D a multiple of 16 in [16, 256]; unit inner strides,
  * 16-byte aligned bases, outer strides of whole 16-byte steps.  Key and value cache may be parts of
  * one allocation.  No counterpart in the reference.
  * slots: k 3, v 3, slots 1, k_cache 4, v_cache 4, k_scale 3, v_scale 3, workspace 1.

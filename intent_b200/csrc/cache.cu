@@ -246,7 +246,21 @@ int check(const char *what, const Arguments &a, bool write) {
     for (int j = 0; j < 4; ++j)
       if (heads::overlap(row_spans[i], cache_spans[j]))
         return fail(B200_ERR_INVALID_ARGUMENT, "%s: the rows and the cache overlap", what);
-  return B200_OK;
+  using heads::footprint;
+  const heads::Footprint space = footprint(a.workspace, 4), slots = footprint(a.slots, 8);
+  const heads::Footprint rows[] = {footprint(a.k, 2), footprint(a.v, 2)}, codes[] = {footprint(a.cache.k, wide), footprint(a.cache.v, wide)};
+  const heads::Footprint scales[] = {scaled ? footprint(a.cache.k_scale, 4) : heads::Footprint(),
+                                     scaled ? footprint(a.cache.v_scale, 4) : heads::Footprint()};
+  status = heads::check_written(what, &space, 1, &slots, 1);
+  for (int i = 0; i < 2 && status == B200_OK; ++i) {
+    const heads::Footprint around[] = {slots, space};
+    status = heads::check_written(what, write ? &codes[i] : &rows[i], 1, around, 2);
+    if (status == B200_OK && write) status = heads::check_written(what, &scales[i], 1, around, 2);
+    if (status == B200_OK && write) status = heads::check_written(what, &scales[i], 1, codes, 2);
+    if (status == B200_OK) status = heads::check_written(what, &space, 1, write ? rows : codes, 2);
+    if (status == B200_OK && !write) status = heads::check_written(what, &space, 1, scales, 2);
+  }
+  return status;
 }
 
 void pack(const Arguments &a, Rows &rows, Pages &pages, Extents &x) {

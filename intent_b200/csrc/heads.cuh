@@ -137,6 +137,71 @@ inline bool apart(const View3 &a, const View3 &b, int size) {
   return apart(View4{a.data, a.d0, a.d1, a.d2, 1, a.s0, a.s1, a.s2, 1}, View4{b.data, b.d0, b.d1, b.d2, 1, b.s0, b.s1, b.s2, 1}, size);
 }
 
+// Where a view's elements lie: its lowest address, and the axes that move, the longest steps first (bytes).
+struct Footprint {
+  int64_t base = 0, element = 0;   // element 0: nothing
+  int axes = 0;
+  int64_t extents[4], steps[4];
+  Footprint() = default;
+  Footprint(const void *data, int size, int count, const int64_t *counts, const int64_t *strides)
+      : base((int64_t)reinterpret_cast<uintptr_t>(data)), element(size) {
+    for (int i = 0; i < count; ++i) {
+      if (counts[i] == 0) element = 0;
+      if (counts[i] <= 1 || strides[i] == 0) continue;
+      if (strides[i] < 0) base += (counts[i] - 1) * strides[i] * size;
+      const int64_t step = llabs(strides[i]) * size;
+      int at = axes++;
+      for (; at > 0 && steps[at - 1] < step; --at) {
+        extents[at] = extents[at - 1];
+        steps[at] = steps[at - 1];
+      }
+      extents[at] = counts[i];
+      steps[at] = step;
+    }
+  }
+  int64_t length(int axis) const {   // of what the axes from `axis` on reach
+    int64_t bytes = element;
+    for (int i = axis; i < axes; ++i) bytes += (extents[i] - 1) * steps[i];
+    return bytes;
+  }
+};
+inline Footprint footprint(const View1 &v, int size) { return Footprint(v.data, size, 1, &v.d0, &v.s0); }
+inline Footprint footprint(const View2 &v, int size) {
+  const int64_t extents[] = {v.d0, v.d1}, strides[] = {v.s0, v.s1};
+  return Footprint(v.data, size, 2, extents, strides);
+}
+inline Footprint footprint(const View3 &v, int size) {
+  const int64_t extents[] = {v.d0, v.d1, v.d2}, strides[] = {v.s0, v.s1, v.s2};
+  return Footprint(v.data, size, 3, extents, strides);
+}
+inline Footprint footprint(const View4 &v, int size) {
+  const int64_t extents[] = {v.d0, v.d1, v.d2, v.d3}, strides[] = {v.s0, v.s1, v.s2, v.s3};
+  return Footprint(v.data, size, 4, extents, strides);
+}
+
+// Whether two views share no byte, by a sufficient test: one ends before the other begins, or their longest steps are
+// alike and what lies inside a step is apart, seen from this step and from the next (a cache's pages with their scales
+// behind the codes).  b's part begins `gap` bytes behind a's.
+inline bool disjoint(const Footprint &a, const Footprint &b, int axis, int64_t gap) {
+  if (!a.element || !b.element || gap >= a.length(axis) || gap + b.length(axis) <= 0) return true;
+  if (axis >= a.axes || axis >= b.axes || a.steps[axis] != b.steps[axis]) return false;
+  const int64_t step = a.steps[axis], inside = ((gap % step) + step) % step;
+  if (a.length(axis + 1) > step || b.length(axis + 1) > step) return false;
+  return disjoint(a, b, axis + 1, inside) && disjoint(a, b, axis + 1, inside - step);
+}
+inline bool disjoint(const Footprint &a, const Footprint &b) { return disjoint(a, b, 0, b.base - a.base); }
+
+// What a call writes meets neither what it reads nor anything else that it writes.
+inline int check_written(const char *what, const Footprint *written, int count, const Footprint *read, int reads) {
+  for (int i = 0; i < count; ++i) {
+    for (int j = 0; j < reads; ++j)
+      if (!disjoint(written[i], read[j])) return fail(B200_ERR_INVALID_ARGUMENT, "%s: an output overlaps an operand", what);
+    for (int j = 0; j < i; ++j)
+      if (!disjoint(written[i], written[j])) return fail(B200_ERR_INVALID_ARGUMENT, "%s: two outputs (or scratch) overlap", what);
+  }
+  return B200_OK;
+}
+
 // Lanes that share a row when each holds 16 of its columns: a power of two, so that a warp holds
 // whole rows and the sum over a row is a butterfly of shuffles.
 inline int row_lanes(int64_t columns) {

@@ -1092,6 +1092,18 @@ extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float s
   if (!heads::distinct(out) || heads::overlap(to, heads::span(q, 2)) || heads::overlap(to, heads::span(k, size)) ||
       heads::overlap(to, heads::span(v, size)))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the output overlaps itself or an input", what);
+  using heads::footprint;
+  const bool codes = size == 1;
+  const heads::Footprint written[] = {footprint(out, 2), lse.data ? footprint(lse, 4) : heads::Footprint(),
+                                      split.whole ? heads::Footprint() : footprint(partial, 4), footprint(workspace, 4)};
+  const heads::Footprint read[] = {footprint(q, 2), footprint(k, size), footprint(v, size),
+                                   codes ? footprint(held.k_scale, 4) : heads::Footprint(),
+                                   codes ? footprint(held.v_scale, 4) : heads::Footprint(), footprint(table, 4), footprint(lengths, 4)};
+  const int64_t lse_extents[] = {lse.d0, lse.d1}, lse_strides[] = {lse.s0, lse.s1};
+  if (lse.data && !heads::distinct(2, lse_extents, lse_strides))
+    return fail(B200_ERR_INVALID_ARGUMENT, "%s: the elements of lse overlap one another", what);
+  const int met = heads::check_written(what, written, 4, read, 7);
+  if (met != B200_OK) return met;
 
   Problem p{};
   p.q = q.data; p.q_batch = q.s0; p.q_head = q.s1;

@@ -521,6 +521,25 @@ bool meet(const View3 &a, const View3 &b, int size) {
   return heads::overlap(heads::span(a, size), heads::span(b, size)) && !side_by_side(a, b, size);
 }
 
+// What is written beside rows (the weights' gradients, the scratch and the workspace; `others`), and the outputs' rows against
+// what is read beside rows.
+int check_beside(const char *what, const Arguments &a, const View3 *const *rows, int count, int size, const heads::Footprint *others,
+                 int other_count) {
+  using heads::footprint;
+  const heads::Footprint read[] = {footprint(a.q_weight, size), footprint(a.k_weight, size), footprint(a.cosine, 4), footprint(a.sine, 4),
+                                   footprint(a.positions, 4)};
+  const heads::Footprint space = footprint(a.workspace, 4);
+  for (int i = 0; i < count; ++i) {
+    const heads::Footprint row = footprint(*rows[i], size);
+    int status = heads::check_written(what, others, other_count, &row, 1);
+    if (status == B200_OK) status = heads::check_written(what, &space, 1, &row, 1);
+    if (status == B200_OK && i >= count - 2) status = heads::check_written(what, &row, 1, read, 5);
+    if (status != B200_OK) return status;
+  }
+  const int status = heads::check_written(what, others, other_count, &space, 1);
+  return status != B200_OK ? status : heads::check_written(what, others, other_count, read, 5);
+}
+
 // Outputs: rows[count - 2] of q and rows[count - 1] of k; before them inputs of q and k in turn.  A row is
 // written after it has been read, so an output may BE an input of its own rows, but it meets no other one,
 // nor the other output, nor itself.
@@ -694,6 +713,7 @@ extern "C" int b200_head_norm_rotary(const int64_t *slots, int64_t count, float 
   if (a.q.d0 == 0 || a.q.d1 + a.k.d1 == 0) return B200_OK;
   const int size = heads::element_size(dtype);
   status = check_outputs(what, rows, 4, size);
+  if (status == B200_OK) status = check_beside(what, a, rows, 4, size, nullptr, 0);
   if (status != B200_OK) return status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
@@ -746,6 +766,8 @@ extern "C" int b200_head_norm_rotary_backward(const int64_t *slots, int64_t coun
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the scratch is contiguous", what);
   const int size = heads::element_size(dtype);
   status = check_outputs(what, rows, 6, size);
+  const heads::Footprint others[] = {heads::footprint(to_q_weight, 4), heads::footprint(to_k_weight, 4), heads::footprint(partial, 4)};
+  if (status == B200_OK) status = check_beside(what, a, rows, 6, size, others, 3);
   if (status != B200_OK) return status;
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   float *scratch = static_cast<float *>(const_cast<void *>(partial.data));

@@ -222,6 +222,7 @@ int check(const char *what, const Arguments &a, bool write) {
   if (a.k.d0 >= (int64_t(1) << 31)) return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: 2^31 rows or more", what);
   if (!a.workspace.data || a.workspace.d0 < B200_WORKSPACE_WORDS || a.workspace.s0 != 1)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the workspace needs %d contiguous int32 words", what, B200_WORKSPACE_WORDS);
+  if (!heads::aligned4(a.workspace.data)) return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the workspace is 4-byte aligned", what);
   if (!a.k.d0 || !a.k.d1) return B200_OK;
   status = heads::check_units(what, a.k.d0, a.k.d1);
   if (status != B200_OK) return status;

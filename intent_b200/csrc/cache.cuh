@@ -149,7 +149,7 @@ inline int check(const char *what, const Cache &c, int32_t dtype, int32_t store,
     if (!sane(*s)) return fail(B200_ERR_INVALID_ARGUMENT, "%s: negative or huge extent or stride", what);
     if (s->d0 != c.k.d0 || s->d1 != c.k.d1 || s->d2 != c.k.d2 || (any && !s->data))
       return fail(B200_ERR_INVALID_ARGUMENT, "%s: an 8-bit cache needs scales of shape (pages, heads, page_size)", what);
-    if (reinterpret_cast<uintptr_t>(s->data) & 3) return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: scales are 4-byte aligned", what);
+    if (!aligned4(s->data)) return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: scales are 4-byte aligned", what);
   }
   return B200_OK;
 }

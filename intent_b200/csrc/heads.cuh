@@ -55,6 +55,9 @@ inline bool sane(int64_t extent, int64_t stride) {
 inline bool sane(const View3 &v) { return sane(v.d0, v.s0) && sane(v.d1, v.s1) && sane(v.d2, v.s2); }
 inline bool sane(const View4 &v) { return sane(v.d0, v.s0) && sane(v.d1, v.s1) && sane(v.d2, v.s2) && sane(v.d3, v.s3); }
 
+// Words that kernels load and store one by one: a misaligned one would fault.
+inline bool aligned4(const void *p) { return (reinterpret_cast<uintptr_t>(p) & 3) == 0; }
+
 // Rows move as 128-bit vectors: unit innermost stride, 16-byte aligned base and outer strides.
 inline bool vector_rows(const View3 &v, int size) {
   const int64_t step = 16 / size;

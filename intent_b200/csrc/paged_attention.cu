@@ -1084,6 +1084,8 @@ extern "C" int b200_paged_attention(const int64_t *slots, int64_t count, float s
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (!split.whole && (partial.d0 < scratch_words(split, group, q.d2) || partial.s0 != 1 || !aligned16(partial.data)))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the scratch is too short, not contiguous or not 16-byte aligned", what);
+  if (!heads::aligned4(table.data) || !heads::aligned4(lengths.data) || !heads::aligned4(lse.data) || !heads::aligned4(workspace.data))
+    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: block table, lengths, lse and workspace are 4-byte aligned", what);
   if (!heads::vector_rows(q, 2) || !heads::vector_rows(out, 2))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT,
                 "%s: rows need a unit inner stride, a 16-byte aligned base and outer strides of whole 16-byte steps", what);

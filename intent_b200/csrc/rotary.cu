@@ -499,6 +499,8 @@ int check(const char *what, const Arguments &a, const View3 *const *rows, int ro
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   if (a.q_weight.s0 != 1 || a.k_weight.s0 != 1 || !aligned16(a.q_weight.data) || !aligned16(a.k_weight.data))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: weights need a unit stride and a 16-byte aligned base", what);
+  if (!heads::aligned4(a.positions.data) || !heads::aligned4(a.workspace.data))
+    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: positions and workspace are 4-byte aligned", what);
   if (a.cosine.s1 != 1 || a.sine.s1 != 1 || !aligned16(a.cosine.data) || !aligned16(a.sine.data) ||
       (a.cosine.d0 > 1 && (a.cosine.s0 % 4 || a.sine.s0 % 4)))
     return fail(B200_ERR_UNSUPPORTED_LAYOUT,
@@ -757,13 +759,13 @@ extern "C" int b200_head_norm_rotary_backward(const int64_t *slots, int64_t coun
   if (status != B200_OK) return status;
   if (!to_q_weight.data || !to_k_weight.data || to_q_weight.d0 != a.q.d2 || to_k_weight.d0 != a.q.d2)
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: a weight's gradient does not have head_dim entries", what);
-  if (to_q_weight.s0 != 1 || to_k_weight.s0 != 1)
-    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the weights' gradients need a unit stride", what);
+  if (to_q_weight.s0 != 1 || to_k_weight.s0 != 1 || !heads::aligned4(to_q_weight.data) || !heads::aligned4(to_k_weight.data))
+    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the weights' gradients need a unit stride and 4-byte alignment", what);
   const BackwardShape shape = backward_shape(a.q.d0, a.q.d1, a.k.d1, a.q.d2);
   if (partial.d0 < shape.blocks || partial.d1 != a.q.d2 || (shape.blocks && !partial.data))
     return fail(B200_ERR_INVALID_ARGUMENT, "%s: the scratch needs (%d, head_dim) f32", what, shape.blocks);
-  if (partial.s1 != 1 || (shape.blocks > 1 && partial.s0 != partial.d1))
-    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the scratch is contiguous", what);
+  if (!heads::aligned4(partial.data) || partial.s1 != 1 || (shape.blocks > 1 && partial.s0 != partial.d1))
+    return fail(B200_ERR_UNSUPPORTED_LAYOUT, "%s: the scratch is contiguous and 4-byte aligned", what);
   const int size = heads::element_size(dtype);
   status = check_outputs(what, rows, 6, size);
   const heads::Footprint others[] = {heads::footprint(to_q_weight, 4), heads::footprint(to_k_weight, 4), heads::footprint(partial, 4)};

@@ -47,10 +47,10 @@ class Slots {
 
 inline int element_size(int dtype) { return dtype == B200_F32 ? 4 : dtype == B200_F16 || dtype == B200_BF16 ? 2 : 1; }
 
-// Every stride times extent stays far from the end of 64 bits, whatever the caller passes.
+// Strides times extents, added up over four axes and in bytes, stay below 2^61, whatever the caller passes.
 inline bool sane(int64_t extent, int64_t stride) {
   return extent >= 0 && extent < (int64_t(1) << 40) && stride > -(int64_t(1) << 40) && stride < (int64_t(1) << 40) &&
-         (extent <= 1 || llabs(stride) <= (int64_t(1) << 60) / extent);
+         (extent <= 1 || llabs(stride) <= (int64_t(1) << 57) / extent);
 }
 inline bool sane(const View3 &v) { return sane(v.d0, v.s0) && sane(v.d1, v.s1) && sane(v.d2, v.s2); }
 inline bool sane(const View4 &v) { return sane(v.d0, v.s0) && sane(v.d1, v.s1) && sane(v.d2, v.s2) && sane(v.d3, v.s3); }
@@ -279,11 +279,6 @@ __device__ __forceinline__ Two fma(Two x, Two y, Two z) {
   return two(r);
 }
 __device__ __forceinline__ Two swap(Two x) { return {x.b, x.a}; }
-__device__ __forceinline__ Two add(Two x, Two y) {
-  uint64_t r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(bits(x)), "l"(bits(y)));
-  return two(r);
-}
 
 // Eight consecutive columns, as raw 128-bit vectors and as f32.
 template <typename T> struct Eight {

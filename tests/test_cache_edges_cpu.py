@@ -98,3 +98,12 @@ def test_scales_that_attention_writes_over_are_refused():
 def test_words_that_are_not_aligned_are_refused(call, change):
     """A kernel that loads one of them would fault."""
     assert call(**change) == 2
+
+
+def test_views_whose_reach_passes_64_bits_are_refused():
+    """Each axis is in range, but all of them together reach 2^63 bytes, where the comparison of places would wrap."""
+    huge = 1 << 30
+    cache = view(huge, 1, huge, 64, address=FAR[2], strides=[0, 0, 64, 1])
+    scales = view(huge, 1, huge, address=FAR[4], strides=[huge, 0, huge])
+    rows = [view(6, 1, 64, address=x) for x in FAR[:2]]
+    assert write("b200_cache_read", k=rows[0], v=rows[1], kc=cache, vc=cache, ks=scales, vs=scales) == 1

@@ -7,6 +7,8 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
 
+#include <c10/cuda/CUDAException.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -115,7 +117,40 @@ PyObject *invoke(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
+// zeroed(device, words) -> int32 zeros that are there when it returns and belong to no graph, also if the
+// current stream is being captured: they are made on a stream of their own, and waited for.
+PyObject *zeroed(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
+  HANDLE_TH_ERRORS
+  const long device = count == 2 ? PyLong_AsLong(arguments[0]) : -1;
+  const long long words = count == 2 ? PyLong_AsLongLong(arguments[1]) : -1;
+  if (PyErr_Occurred()) return nullptr;
+  if (device < 0 || words < 0) {
+    PyErr_SetString(PyExc_TypeError, "zeroed(device, words)");
+    return nullptr;
+  }
+  const c10::DeviceIndex index = static_cast<c10::DeviceIndex>(device);
+  const c10::cuda::CUDAGuard guard(index);
+  // memory may be allocated and another stream waited for while a graph is being captured
+  const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  c10::cuda::CUDAStream stream = c10::cuda::getStreamFromPool(false, index);
+  cudaStreamCaptureStatus status = cudaStreamCaptureStatusNone;
+  for (int i = 0; i < 64; ++i) {   // the pool's streams go round, and the one being captured may be among them
+    C10_CUDA_CHECK(cudaStreamIsCapturing(stream.stream(), &status));
+    if (status == cudaStreamCaptureStatusNone) break;
+    stream = c10::cuda::getStreamFromPool(false, index);
+  }
+  const c10::cuda::CUDAStreamGuard on(stream);
+  const int64_t shape[1] = {words};
+  at::Tensor space = at::detail::empty_cuda(at::IntArrayRef(shape, 1), at::kInt, at::Device(at::kCUDA, index), std::nullopt);
+  C10_CUDA_CHECK(cudaMemsetAsync(space.data_ptr(), 0, static_cast<size_t>(words) * 4, stream.stream()));
+  C10_CUDA_CHECK(cudaStreamSynchronize(stream.stream()));
+  return THPVariable_Wrap(space);
+  END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"zeroed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(zeroed)), METH_FASTCALL,
+     "zeroed(device, words) -> int32 zeros outside any graph"},
     {"invoke", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(invoke)), METH_FASTCALL,
      "invoke(entry, device, plan, tensors, extents, number, code, other) -> the tensors made, or a status"},
     {nullptr, nullptr, 0, nullptr}};

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 from functools import lru_cache
+from threading import Lock
 
 import torch
 
@@ -65,16 +66,34 @@ def _call(name: str, device: torch.device, *arguments) -> None:
 
 
 _workspaces: dict[torch.device, torch.Tensor] = {}
+_workspaces_lock = Lock()
 
 
 def workspace(device: torch.device) -> torch.Tensor:
-    """The zero-initialised int32 status/workspace view the tensor-core entries take."""
+    """The zero-initialised int32 status/workspace view that entries report to, one per device and shared by all
+    streams.  Its zeros are there before anything else sees it, and it belongs to no graph: replays of one would
+    clear its reports."""
     device = torch.device(device)
     if device.type == "cuda" and device.index is None:
         device = torch.device("cuda", torch.cuda.current_device())
-    if device not in _workspaces:
-        _workspaces.setdefault(device, torch.zeros(_native.WORKSPACE_WORDS, dtype=torch.int32, device=device))
-    return _workspaces[device]
+    space = _workspaces.get(device)
+    if space is None:
+        with _workspaces_lock:
+            space = _workspaces.get(device)
+            if space is None:
+                space = _workspaces[device] = _zeroed(device)
+    return space
+
+
+def _zeroed(device: torch.device) -> torch.Tensor:
+    if device.type != "cuda":
+        return torch.zeros(_native.WORKSPACE_WORDS, dtype=torch.int32, device=device)
+    with torch.cuda.device(device):
+        if torch.cuda.is_current_stream_capturing():
+            return _native.binding().zeroed(device.index, _native.WORKSPACE_WORDS)
+        space = torch.zeros(_native.WORKSPACE_WORDS, dtype=torch.int32, device=device)
+        torch.cuda.current_stream(device).synchronize()
+        return space
 
 
 def workspace_status(device: torch.device) -> None:
@@ -373,18 +392,10 @@ _status_spaces: dict[int, torch.Tensor] = {}
 
 
 def _status(device: int) -> torch.Tensor:
-    """``workspace(device)``, where an entry records a bad index.  It is made once per device and shared by all
-    streams, so the first call may not fall into a graph capture, whose replays would clear it, and its
-    zeros have to be there before any other stream writes to it."""
+    """``workspace(device)``, where an entry records a bad index, by the device's number (a lookup takes a tenth of the time)."""
     space = _status_spaces.get(device)
     if space is None:
-        where = torch.device("cuda", device)
-        with torch.cuda.device(where):
-            if torch.cuda.is_current_stream_capturing():
-                raise RuntimeError("call this operator once outside a graph capture before capturing it")
-            space = workspace(where)
-            torch.cuda.current_stream(where).synchronize()
-        _status_spaces[device] = space
+        space = _status_spaces[device] = workspace(torch.device("cuda", device))
     return space
 
 

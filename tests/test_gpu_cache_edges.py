@@ -207,3 +207,45 @@ def test_a_bad_index_does_not_hide_a_wait_that_gave_up():
     with pytest.raises(ValueError, match=r"\(row 1\)"):
         ops.workspace_status(DEV)
     ops.workspace_status(DEV)
+
+
+@pytest.mark.parametrize("first", ["c = ops.gemm(a, b)", "ops.cache_write(rows, rows, good, cache, other); c = ops.gemm(a, b)"])
+def test_a_first_call_inside_a_capture_leaves_later_reports_alone(first):
+    """In a process of its own: the first call on the device is a captured one, so its status words must neither come
+    from the graph's memory nor be cleared by its replays."""
+    program = textwrap.dedent("""
+        import torch
+        from intent_b200 import ops
+        a = torch.randn(256, 256, device="cuda:0").bfloat16()
+        b = a.t()
+        cache = torch.zeros(1, 1, 16, 64, device="cuda:0").half()
+        rows, other = torch.ones(2, 1, 64, device="cuda:0").half(), cache.clone()
+        good, bad = torch.tensor([1, 5], device="cuda:0"), torch.tensor([1, 99], device="cuda:0")
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            FIRST
+            out = ops.softmax(c)
+        ops.workspace_status("cuda:0")                      # nothing has run: nothing to report
+        ops.cache_write(rows, rows, bad, cache, other)
+        for _ in range(3):
+            graph.replay()
+        torch.cuda.synchronize()
+        try:
+            ops.workspace_status("cuda:0")
+        except ValueError as error:
+            assert "row 1" in str(error), error
+        else:
+            raise SystemExit("the replays cleared the report")
+        ops.workspace_status("cuda:0")
+        want = a.double() @ b.double()
+        assert (c.double() - want).abs().max() <= 2.0 ** -8 * want.abs().max()
+        cache.zero_()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert int((cache[0, 0, :, 0] == 1).sum()) == (2 if "cache_write" in 'FIRST' else 0)
+        del graph
+        print("held")
+    """).replace("FIRST", first)
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=600, cwd=Path(__file__).resolve().parents[1])
+    assert done.returncode == 0 and "held" in done.stdout, done.stdout + done.stderr

@@ -111,6 +111,19 @@ BINDING_PATH = LIBRARY_PATH.with_name("binding.so")
 _binding = None
 
 
+def binding_built_for() -> str:
+    """What ``binding.so`` depends on beside its source: torch's C++ interface and Python's."""
+    import sysconfig
+
+    import torch
+    return f"torch {torch.__version__} {int(torch._C._GLIBCXX_USE_CXX11_ABI)} python {sysconfig.get_config_var('SOABI')}"
+
+
+def binding_is_current(module: Path) -> bool:
+    """Whether the module names this torch and this Python; found without loading it, which another torch may not survive."""
+    return f"built for {binding_built_for()};".encode() in module.read_bytes()
+
+
 def binding():
     """The module that calls entries which take their views as one array (``csrc/binding.cpp``)."""
     global _binding
@@ -118,6 +131,9 @@ def binding():
         if _binding is None:
             if not BINDING_PATH.exists():
                 raise NativeLibraryMissing(f"{BINDING_PATH} is missing: build it with `python -m intent_b200.build`.")
+            if not binding_is_current(BINDING_PATH):   # it reads torch's objects by their layout
+                raise NativeLibraryMissing(f"{BINDING_PATH} was not built for {binding_built_for()}: "
+                                           "build it again with `python -m intent_b200.build`.")
             loader = ExtensionFileLoader("binding", str(BINDING_PATH))
             _binding = module_from_spec(spec_from_file_location("binding", str(BINDING_PATH), loader=loader))
             loader.exec_module(_binding)

@@ -19,6 +19,8 @@ import sys
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
+from . import _native
+
 PACKAGE = Path(__file__).resolve().parent
 ROOT = PACKAGE.parent
 CSRC = PACKAGE / "csrc"
@@ -93,10 +95,11 @@ BINDING = PACKAGE / "lib" / "binding.so"
 
 
 def build_binding(*, force: bool = False) -> Path:
-    """The module that packs torch tensors for the entries that take their views as one array."""
+    """The module that packs torch tensors for the entries that take their views as one array.  It is good for the
+    torch and the Python that it was built against, which it names (``_native.binding_built_for``)."""
     source = CSRC / "binding.cpp"
     BINDING.parent.mkdir(parents=True, exist_ok=True)
-    if force or _stale(BINDING, [source]):
+    if force or _stale(BINDING, [source]) or not _native.binding_is_current(BINDING):
         import sysconfig
 
         import torch
@@ -105,7 +108,7 @@ def build_binding(*, force: bool = False) -> Path:
         includes = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(cuda / "include")]
         libraries = Path(torch.__file__).resolve().parent / "lib"
         _run([os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared",
-              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", *(f"-I{path}" for path in includes),
+              f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f'-DB200_BUILT_FOR="{_native.binding_built_for()}"', *(f"-I{path}" for path in includes),
               str(source), "-o", str(BINDING), f"-L{libraries}", "-lc10", "-lc10_cuda", "-ltorch_cpu", "-ltorch_cuda", "-ltorch",
               "-ltorch_python"])
     return BINDING

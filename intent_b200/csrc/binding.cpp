@@ -148,6 +148,9 @@ PyObject *zeroed(PyObject *, PyObject *const *arguments, Py_ssize_t count) {
   END_HANDLE_TH_ERRORS
 }
 
+// What build.py and _native.py look for in the file.
+const char built_for[] = "built for " B200_BUILT_FOR ";";
+
 PyMethodDef methods[] = {
     {"zeroed", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(zeroed)), METH_FASTCALL,
      "zeroed(device, words) -> int32 zeros outside any graph"},
@@ -158,4 +161,11 @@ PyModuleDef definition = {PyModuleDef_HEAD_INIT, "binding", nullptr, -1, methods
 
 }  // namespace
 
-PyMODINIT_FUNC PyInit_binding(void) { return PyModule_Create(&definition); }
+PyMODINIT_FUNC PyInit_binding(void) {
+  PyObject *module = PyModule_Create(&definition);
+  if (module && PyModule_AddStringConstant(module, "built_for", built_for) < 0) {
+    Py_DECREF(module);
+    return nullptr;
+  }
+  return module;
+}

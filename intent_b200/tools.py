@@ -84,7 +84,18 @@ def doctor(device: int | None = 0, *, compiler=None) -> dict:
         if missing:
             raise ImportError(f"{_native.LIBRARY_PATH} lacks {missing}")
         return {"path": str(_native.LIBRARY_PATH), "abi_version": int(handle.b200_abi_version()),
-                "entries": len(_native.SIGNATURES), "binding": _native.binding().__file__}
+                "entries": len(_native.SIGNATURES)}
+
+    def native_binding():
+        return _native.binding().__file__
+
+    def binding_beside(library):
+        """In the library's entry while it is there, and an entry of its own when it is not: the library may well be."""
+        try:
+            if library is not None:
+                library["binding"] = native_binding()
+        except Exception:
+            check("native binding", "compiler_resources", native_binding)
 
     def python_module(name):
         module = importlib.import_module(name)
@@ -100,7 +111,7 @@ def doctor(device: int | None = 0, *, compiler=None) -> dict:
                 "capabilities": compilation.device_capabilities(device)}
 
     check("b200 compile step", "compiler", compiler_information)
-    check("native library", "compiler_resources", native_library)
+    binding_beside(check("native library", "compiler_resources", native_library))
     check("torch", "python_package", lambda: python_module("torch"))
     if device is None:
         result["scope"] = "Compiler and library only; the runtime device was not checked"

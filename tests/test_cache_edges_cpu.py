@@ -107,3 +107,42 @@ def test_views_whose_reach_passes_64_bits_are_refused():
     scales = view(huge, 1, huge, address=FAR[4], strides=[huge, 0, huge])
     rows = [view(6, 1, 64, address=x) for x in FAR[:2]]
     assert write("b200_cache_read", k=rows[0], v=rows[1], kc=cache, vc=cache, ks=scales, vs=scales) == 1
+
+
+# ------------------------------------------------------------------------- the native module
+def test_the_module_is_rebuilt_for_another_torch(monkeypatch, tmp_path):
+    """Its source is older than it, but it was built against other headers."""
+    from intent_b200 import build
+    module, commands = tmp_path / "binding.so", []
+
+    def compile(command):
+        commands.append(command)
+        module.write_bytes(f"... built for {_native.binding_built_for()};".encode())
+        return ""
+    monkeypatch.setattr(build, "BINDING", module)
+    monkeypatch.setattr(build, "_run", compile)
+    for expected in (1, 1):
+        build.build_binding()
+        assert len(commands) == expected
+    real = _native.binding_built_for()
+    monkeypatch.setattr(_native, "binding_built_for", lambda: real.replace("torch ", "torch 9"))
+    for expected in (2, 2):
+        build.build_binding()
+        assert len(commands) == expected
+
+
+def test_a_module_built_for_another_torch_is_not_loaded(monkeypatch, tmp_path):
+    from intent_b200 import tools
+    module = tmp_path / "binding.so"
+    monkeypatch.setattr(_native, "BINDING_PATH", module)
+    monkeypatch.setattr(_native, "_binding", None)
+    for content in ("", "built for torch 1.0 0 python cpython-27;"):
+        module.write_text(content)
+        with pytest.raises(_native.NativeLibraryMissing, match="build it again"):
+            _native.binding()
+    # the library is there all the same, and doctor says which of the two is not
+    report = {entry["name"]: entry for entry in tools.doctor(None)["checks"]}
+    assert report["native library"]["status"] == "available" and report["native binding"]["status"] == "unavailable"
+    monkeypatch.undo()
+    report = {entry["name"]: entry for entry in tools.doctor(None)["checks"]}
+    assert "native binding" not in report and report["native library"]["detail"]["binding"] == str(_native.BINDING_PATH)

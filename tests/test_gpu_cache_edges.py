@@ -249,3 +249,47 @@ def test_a_first_call_inside_a_capture_leaves_later_reports_alone(first):
     """).replace("FIRST", first)
     done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=600, cwd=Path(__file__).resolve().parents[1])
     assert done.returncode == 0 and "held" in done.stdout, done.stdout + done.stderr
+
+
+def unit_rows(tokens, heads, kv_heads, columns):
+    """Heads of a token that one group of lanes takes, by the rule beside the kernel (rotary.cu, rows_of_unit)."""
+    lanes = 1
+    while lanes * 16 < columns:
+        lanes *= 2
+    groups = 2 * torch.cuda.get_device_properties(0).multi_processor_count * 256 // lanes
+    for rows in range(8, 1, -1):
+        units = -(-heads // rows) + -(-kv_heads // rows)
+        if tokens * units >= groups and units * rows * 7 <= (heads + kv_heads) * 8:
+            return rows
+    return 1
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("tokens, heads, kv_heads, columns, pairs, rows", [
+    (6500, 5, 3, 64, 32, 3),           # 5 = 3 + 2: a unit that is not full
+    (9600, 7, 7, 64, 16, 8), (2400, 32, 8, 128, 64, 8), (2500, 31, 8, 128, 32, 8), (3300, 13, 2, 256, 128, 2), (19000, 15, 2, 48, 24, 3)])
+def test_units_of_several_heads(tokens, heads, kv_heads, columns, pairs, rows, interleaved, dtype):
+    """Calls large enough that a group of lanes takes several heads of a token, and not always as many; padding, rows of zeros
+    and an epsilon of 0, so that a row that is not there would show."""
+    assert unit_rows(tokens, heads, kv_heads, columns) == rows
+    q, k, qw, kw, cos, sin, positions = rotary_inputs(tokens, heads, kv_heads, columns, pairs, dtype, seed=tokens)
+    q, k = q.clone(), k.clone()
+    positions[::7] = -1
+    q[::7], k[::7] = 0, float("nan")
+    live = (positions >= 0)[:, None, None]
+    out = ops.head_norm_rotary(q, k, qw, kw, cos, sin, positions, 0.0, interleaved=interleaved)
+    gq, gk = randn(*q.shape, dtype=dtype, seed=71), randn(*k.shape, dtype=dtype, seed=72)
+    grads = ops.head_norm_rotary_backward(gq, gk, q, k, qw, kw, cos, sin, positions, 0.0, interleaved=interleaved)
+    ops.workspace_status(DEV)
+    for i, (x, w, g) in enumerate(((q, qw, gq), (k, kw, gk))):
+        x = torch.where(live, x, 1.0)
+        plain.close(out[i], *plain.norm_rotary(x, w, cos, sin, positions, 0.0, interleaved))
+        dx, dx_slack, dw, dw_slack = plain.norm_rotary_backward(g, x, w, cos, sin, positions, 0.0, interleaved)
+        plain.close(grads[i], dx, dx_slack)
+        # no lane adds more than 256 rows here either
+        plain.close(grads[2 + i], dw, dw_slack)
+    in_place = ops.head_norm_rotary_backward(gq, gk, q, k, qw, kw, cos, sin, positions, 0.0, interleaved=interleaved, dq=gq, dk=gk)
+    assert all(torch.equal(a, b) for a, b in zip(in_place, grads))
+    in_place = ops.head_norm_rotary(q, k, qw, kw, cos, sin, positions, 0.0, interleaved=interleaved, q_out=q, k_out=k)
+    assert all(torch.equal(a, b) for a, b in zip(in_place, out))

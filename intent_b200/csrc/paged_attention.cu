@@ -28,8 +28,8 @@
 // 2^-43 of the largest where those are finer (f16: the products of f16 rows and of codes, see kLift); the result is
 // rounded once.  Up to four query heads stand in the columns twice: the first four carry
 // the weights' first halves and the other four the second ones, in one product instead of two.  Second halves are
-// scaled in f16; more heads add them apart for that, which costs 8-bit rows of 8 and 16 query heads 2 to 6 % (32 sequences of
-// 4096 keys, 16 heads on each of 8 key heads in e4m3: 75 to 79 us) and 16-bit ones nothing.
+// scaled in f16; more heads add them apart for that, which costs 8-bit rows of 8 and 16 query heads 2 to 8 % (32 sequences of
+// 4096 keys, 16 heads on each of 8 key heads in e4m3: 73 to 79 us) and 16-bit ones nothing.
 //
 // Measured (device time; floors at the 6447 GB/s of a copy): one sequence of 131072 keys, 32 query and 8 key heads
 // of 128 in bf16: 88.6 us (83.3), of which 85 stream at 6.3 TB/s and 4 join; 64 sequences of 100 to 4096 keys: 88.9
@@ -38,9 +38,10 @@
 //
 // 8-bit rows.  Codes become f16 exactly on their way into the products.  The query is scaled by a
 // power of two per row to fit f16; a key's scale multiplies its score.  A value's scale is folded into
-// the weight as exp2(s_j + log2 v_scale_j - M) with M the running maximum of that sum, so the weights
-// that enter the product are at most 1 and the largest of them is, however the scales differ; the
-// denominator keeps its own maximum and f32 weights.
+// the weight as exp2((s_j - m) + log2 v_scale_j - w), where m is the running maximum of the scores and w that of the
+// rest, so the weights that enter the product are at most 1 and the largest of them is, however the scales differ; the
+// denominator keeps f32 weights relative to m.  Scores enter differences only: a score of 2^20 has no room for what
+// is added to it.
 #include <type_traits>
 
 #include "cache.cuh"
@@ -109,7 +110,7 @@ template <int STORE, int D, int ROWS> struct Shape {
 template <typename M> constexpr bool kHalf = std::is_same<M, __half>::value;
 template <typename M> constexpr float kLift = kHalf<M> ? 7.0f : -8.0f;
 template <typename M> constexpr float kRest = kHalf<M> ? 2048.0f : 1.0f;
-constexpr int partial_floats(int columns) { return columns + 4; }   // sums, m, l, M, unused
+constexpr int partial_floats(int columns) { return columns + 4; }   // sums, m, l, w, unused
 
 // What a run begins with, for the kernel that joins: (sequence, head tile) and how many of its steps lie
 // before the run; and what a run holds.
@@ -409,7 +410,7 @@ paged_attention_kernel(const Problem p) {
   // ---- copies: lane r looks row r of the tile up; a row's 16-byte pieces go to neighbouring lanes
   unsigned char *ring = dynamic_smem + warp * S::kStages * S::kStageBytes;
   const uint32_t ring_address = shared_address(ring);
-  float4 *stats = reinterpret_cast<float4 *>(dynamic_smem + S::kRingBytes);   // m, l, weight_max of the warps' rows
+  float4 *stats = reinterpret_cast<float4 *>(dynamic_smem + S::kRingBytes);   // m, l, above of the warps' rows
   float *units = reinterpret_cast<float *>(stats + kWarps * S::kColumns);
   int entry = -1, offset = 0;
   bool inside = false;
@@ -545,7 +546,7 @@ paged_attention_kernel(const Problem p) {
   };
 
   // ---- running state of a piece; sums: columns (of V) x heads
-  float sums[D / 16][kHeads][4], m[kHeads][2], l[kHeads][2], weight_max[kHeads][2];
+  float sums[D / 16][kHeads][4], m[kHeads][2], l[kHeads][2], above[kHeads][2];   // above: w, 0 without codes
   int piece_first = use.step;
   auto reset = [&]() {
 #pragma unroll
@@ -555,7 +556,7 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
         for (int j = 0; j < 4; ++j) sums[i][h][j] = 0.0f;
 #pragma unroll
-      for (int j = 0; j < 2; ++j) { m[h][j] = weight_max[h][j] = -INFINITY; l[h][j] = 0.0f; }
+      for (int j = 0; j < 2; ++j) { m[h][j] = -INFINITY; above[h][j] = kCodes ? -INFINITY : 0.0f; l[h][j] = 0.0f; }
     }
     piece_first = use.step;
   };
@@ -617,7 +618,7 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
             for (int h = 0; h < kHeads; ++h) s[t][h][2 * k] = s[t][h][2 * k + 1] = -INFINITY;
     }
-    // The bases m and weight_max move only when a score passes them by more than 8 (log2 units): until then
+    // The bases m and above move only when a score passes them by more than 8 (log2 units): until then
     // weights reach 2^8 times what they stand for at the most, which kLift leaves room for.
     bool grown = false;
 #pragma unroll
@@ -626,8 +627,9 @@ paged_attention_kernel(const Problem p) {
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int t = 0; t < kTiles; ++t) {
-          grown |= fmaxf(s[t][h][j], s[t][h][2 + j]) > m[h][j] + 8.0f;
-          if constexpr (kCodes) grown |= fmaxf(s[t][h][j] + log_scale[t][0], s[t][h][2 + j] + log_scale[t][1]) > weight_max[h][j] + 8.0f;
+          const float d[2] = {s[t][h][j] - m[h][j], s[t][h][2 + j] - m[h][j]};
+          grown |= fmaxf(d[0], d[1]) > 8.0f;
+          if constexpr (kCodes) grown |= fmaxf(d[0] + log_scale[t][0], d[1] + log_scale[t][1]) > above[h][j] + 8.0f;
         }
     if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
@@ -635,22 +637,27 @@ paged_attention_kernel(const Problem p) {
         float shrink[2];
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          float top = m[h][j], weight_top = weight_max[h][j];
+          float top = m[h][j];
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t) {
-            top = fmaxf(top, fmaxf(s[t][h][j], s[t][h][2 + j]));
-            if constexpr (kCodes) weight_top = fmaxf(weight_top, fmaxf(s[t][h][j] + log_scale[t][0], s[t][h][2 + j] + log_scale[t][1]));
-          }
+          for (int t = 0; t < kTiles; ++t) top = fmaxf(top, fmaxf(s[t][h][j], s[t][h][2 + j]));
 #pragma unroll
-          for (int other = 4; other < 32; other <<= 1) {
-            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, other));
-            if constexpr (kCodes) weight_top = fmaxf(weight_top, __shfl_xor_sync(0xffffffffu, weight_top, other));
-          }
-          if constexpr (!kCodes) weight_top = top;
-          l[h][j] *= exp2_fast(m[h][j] - finite_or_zero(top));
-          shrink[j] = exp2_fast(weight_max[h][j] - finite_or_zero(weight_top));
+          for (int other = 4; other < 32; other <<= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, other));
+          const float base = finite_or_zero(top), moved = m[h][j] - base;
+          l[h][j] *= exp2_fast(moved);
           m[h][j] = top;
-          weight_max[h][j] = weight_top;
+          if constexpr (kCodes) {
+            const float old = above[h][j] + moved;
+            float w = old;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t)
+              w = fmaxf(w, fmaxf(s[t][h][j] - base + log_scale[t][0], s[t][h][2 + j] - base + log_scale[t][1]));
+#pragma unroll
+            for (int other = 4; other < 32; other <<= 1) w = fmaxf(w, __shfl_xor_sync(0xffffffffu, w, other));
+            shrink[j] = exp2_fast(old - finite_or_zero(w));
+            above[h][j] = w;
+          } else {
+            shrink[j] = exp2_fast(moved);
+          }
         }
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
@@ -661,8 +668,8 @@ paged_attention_kernel(const Problem p) {
     uint32_t high[kTiles][kHeads][2], rest[kTiles][kHeads][2];   // head g, keys 16 t + 2 c, + 1 and + 8, + 9
 #pragma unroll
     for (int h = 0; h < kHeads; ++h) {
-      const float base[2] = {finite_or_zero(m[h][0]) - kLift<M>, finite_or_zero(m[h][1]) - kLift<M>};
-      const float weight_base[2] = {finite_or_zero(weight_max[h][0]) - kLift<M>, finite_or_zero(weight_max[h][1]) - kLift<M>};
+      const float base[2] = {finite_or_zero(m[h][0]), finite_or_zero(m[h][1])};
+      const float lift[2] = {kLift<M> - finite_or_zero(above[h][0]), kLift<M> - finite_or_zero(above[h][1])};
 #pragma unroll
       for (int t = 0; t < kTiles; ++t)
 #pragma unroll
@@ -670,10 +677,11 @@ paged_attention_kernel(const Problem p) {
           float w[2];
 #pragma unroll
           for (int j = 0; j < 2; ++j) {
-            w[j] = exp2_fast(s[t][h][2 * k + j] - base[j]);
+            const float d = s[t][h][2 * k + j] - base[j];
+            w[j] = exp2_fast(d + kLift<M>);
             l[h][j] += w[j];
             // log2 of a masked key's zero scale is -infinity: its weight is 0
-            if constexpr (kCodes) w[j] = exp2_fast(s[t][h][2 * k + j] + log_scale[t][k] - weight_base[j]);
+            if constexpr (kCodes) w[j] = exp2_fast(d + (log_scale[t][k] + lift[j]));
           }
           const uint32_t pair = pack<M>(w[0], w[1]), left = pack<M>((w[0] - unpack<M>(pair, 0)) * kRest<M>, (w[1] - unpack<M>(pair, 1)) * kRest<M>);
           high[t][h][k] = transposed(kTwice && c >= 2 ? left : pair);
@@ -737,7 +745,7 @@ paged_attention_kernel(const Problem p) {
       for (int j = 0; j < 2; ++j) {
 #pragma unroll
         for (int other = 4; other < 32; other <<= 1) l[h][j] += __shfl_xor_sync(0xffffffffu, l[h][j], other);
-        if (g == 0) stats[warp * S::kColumns + h * 8 + 2 * c + j] = make_float4(m[h][j], l[h][j], weight_max[h][j], 0.0f);
+        if (g == 0) stats[warp * S::kColumns + h * 8 + 2 * c + j] = make_float4(m[h][j], l[h][j], above[h][j], 0.0f);
       }
     __syncthreads();
     float *mine = reinterpret_cast<float *>(ring + stage * S::kStageBytes);
@@ -748,10 +756,14 @@ paged_attention_kernel(const Problem p) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         const int row = h * 8 + 2 * c + j;
-        float weight_top = weight_max[h][j];
+        float top = -INFINITY, weight_top = -INFINITY;
 #pragma unroll
-        for (int w = 1; w < kWarps; ++w) weight_top = fmaxf(weight_top, stats[(warp ^ w) * S::kColumns + row].z);
-        float shrink = exp2_fast(weight_max[h][j] - finite_or_zero(weight_top));
+        for (int w = 0; w < kWarps; ++w) top = fmaxf(top, stats[w * S::kColumns + row].x);
+        const float base = finite_or_zero(top);
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+          weight_top = fmaxf(weight_top, stats[w * S::kColumns + row].z + (stats[w * S::kColumns + row].x - base));
+        float shrink = exp2_fast(above[h][j] + (m[h][j] - base) - finite_or_zero(weight_top));
         if (kTwice && c >= 2) shrink *= 1.0f / kRest<M>;
 #pragma unroll
         for (int i = 0; i < D / 16; ++i)
@@ -770,12 +782,14 @@ paged_attention_kernel(const Problem p) {
       for (int w = 0; w < kWarps; ++w) {
         state[w] = stats[w * S::kColumns + row];
         top = fmaxf(top, state[w].x);
-        weight_top = fmaxf(weight_top, state[w].z);
       }
       const float base = finite_or_zero(top);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) denominator += state[w].y * exp2_fast(state[w].x - base);
-      units[row] = __fdiv_rn(kCodes ? exp2_fast(finite_or_zero(weight_top) - base) : 1.0f, denominator);
+      for (int w = 0; w < kWarps; ++w) {
+        weight_top = fmaxf(weight_top, state[w].z + (state[w].x - base));
+        denominator += state[w].y * exp2_fast(state[w].x - base);
+      }
+      units[row] = __fdiv_rn(kCodes ? exp2_fast(finite_or_zero(weight_top)) : 1.0f, denominator);
       if (whole) {
         if (p.lse) p.lse[at.b * p.lse_batch + (head0 + row) * p.lse_head] = (base - kLift<M> + log2f(denominator)) * kLn2;
       } else {
@@ -854,19 +868,19 @@ struct State {
   float denominator, top, weight_top;
 };
 template <int COUNT> __device__ __forceinline__ void add(State &state, const float4 (&x)[COUNT], const float4 (&other)[COUNT]) {
-  float top = state.top, weight_top = state.weight_top;
+  float top = state.top;
 #pragma unroll
-  for (int j = 0; j < COUNT; ++j) {
-    top = fmaxf(top, other[j].x);
-    weight_top = fmaxf(weight_top, other[j].z);
-  }
-  const float base = finite_or_zero(top), weight_base = finite_or_zero(weight_top);
-  const float mine = exp2_fast(state.weight_top - weight_base);
+  for (int j = 0; j < COUNT; ++j) top = fmaxf(top, other[j].x);
+  const float base = finite_or_zero(top), old = state.weight_top + (state.top - base);
+  float weight_top = old;
+#pragma unroll
+  for (int j = 0; j < COUNT; ++j) weight_top = fmaxf(weight_top, other[j].z + (other[j].x - base));
+  const float weight_base = finite_or_zero(weight_top), mine = exp2_fast(old - weight_base);
   state.denominator *= exp2_fast(state.top - base);
   state.sum = make_float4(state.sum.x * mine, state.sum.y * mine, state.sum.z * mine, state.sum.w * mine);
 #pragma unroll
   for (int j = 0; j < COUNT; ++j) {
-    const float shrink = exp2_fast(other[j].z - weight_base);
+    const float shrink = exp2_fast(other[j].z + (other[j].x - base) - weight_base);
     state.denominator += other[j].y * exp2_fast(other[j].x - base);
     state.sum.x += x[j].x * shrink;
     state.sum.y += x[j].y * shrink;
@@ -941,7 +955,7 @@ paged_attention_join_kernel(const Problem p) {
     }
     state.sum = replaced(state.sum, special);
   }
-  const float base = finite_or_zero(state.top), unit = __fdividef(exp2_fast(finite_or_zero(state.weight_top) - base), state.denominator);
+  const float base = finite_or_zero(state.top), unit = __fdividef(exp2_fast(finite_or_zero(state.weight_top)), state.denominator);
   T *out = static_cast<T *>(p.out) + cut.b * p.out_batch + head * p.out_head + 4 * lane;
   *reinterpret_cast<uint2 *>(out) = make_uint2(pack<T>(state.sum.x * unit, state.sum.y * unit), pack<T>(state.sum.z * unit, state.sum.w * unit));
   if (lane == 0 && p.lse) p.lse[cut.b * p.lse_batch + head * p.lse_head] = (base - p.lift + __log2f(state.denominator)) * kLn2;

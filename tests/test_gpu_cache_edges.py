@@ -293,3 +293,20 @@ def test_units_of_several_heads(tokens, heads, kv_heads, columns, pairs, rows, i
     assert all(torch.equal(a, b) for a, b in zip(in_place, grads))
     in_place = ops.head_norm_rotary(q, k, qw, kw, cos, sin, positions, 0.0, interleaved=interleaved, q_out=q, k_out=k)
     assert all(torch.equal(a, b) for a, b in zip(in_place, out))
+
+
+@pytest.mark.parametrize("dtype, store", [(F16, F16), (BF16, BF16), (F16, I8), (BF16, E4M3)])
+@pytest.mark.parametrize("group", [4, 7, 16])
+@pytest.mark.parametrize("size", [1.0, 2.0 ** 14, 2.0 ** 15.4])
+def test_equal_values_come_back_whatever_the_scores(size, group, dtype, store):
+    """Scores of up to 2^34, of which f32 holds no fraction: weights add up to 1 all the same, so the result is the value.  A
+    weight is off by 2^-16 of itself at most, its sums by 2^-24 for each of their terms."""
+    for length, room in ((300, 0), (3000, 0)):
+        k = size * (1 + torch.rand(length, 1, 64, generator=torch.Generator().manual_seed(length)).to(DEV))
+        q = (size * (1 + torch.rand(1, group, 64, generator=torch.Generator().manual_seed(group)).to(DEV))).clamp(max=60000).to(dtype)
+        for sign in (1.0, -1.0):
+            case = one_sequence(sign * k.clamp(max=60000), torch.ones(length, 1, 64, device=DEV), group, dtype, store, room=room)
+            out, lse = attend(q, case, 0.5)
+            value = plain.values(case["v_cache"], case["v_scale"])[case["block_table"][0, 0].long(), 0, 0, 0]
+            plain.close(out, value.expand(1, group, 64), 2.0 ** -15 + (length + 64) * plain.F32)
+            assert lse.isfinite().all()

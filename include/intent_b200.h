@@ -352,22 +352,27 @@ int b200_cache_read(const int64_t *slots, int64_t count, int32_t dtype, int32_t 
  * b200_cache_write fills.  heads is a multiple of the cache's heads; query head h reads key head
  * h / (heads / kv_heads).   s = scale * q . k,  out = softmax(s) . v,  lse = log(sum(e^s)) (f32, natural
  * logarithm; lse may be null).  A sequence of length 0 (or less) gets zeros and -infinity.  Nothing
- * past a sequence's length is read into a result, whatever it holds; entries of block_table past it may have any
- * value.  An entry within it that is no page counts its positions as absent, a length
+ * past a sequence's length is read into a result, whatever it holds; entries of block_table past it may
+ * have any value.  An entry within it that is no page counts its positions as absent, a length
  * greater than the table's columns * page_size counts as that, and both are recorded in the
- * workspace; a sequence that has positions, but all of them absent (if the table has no columns, too), gets NaN and
- * -infinity.  An infinite
- * value of a 16-bit cache gives that infinity, however small its weight, two of both signs NaN, and so does
- * one under a score of -infinity.  D is 64 or 128; f32 arithmetic.  The softmax weights enter the products with 16 bits
- * (bf16 caches), or with 22 but no finer than 2^-43 of the largest (f16 and 8-bit caches; there that is the largest product
- * of a weight and its row's scale); one rounding at the end; sums are joined in a fixed order, so results do not vary.
+ * workspace; a sequence that has positions, but all of them absent (if the table has no columns, too),
+ * gets NaN and -infinity.  An infinite value of a 16-bit cache gives that infinity, however small its
+ * weight, two of both signs NaN, and so does one under a score of -infinity; a call with an infinity or a
+ * NaN among its values takes up to ten times as long.  Scales of an 8-bit cache are numbers >= 0 or NaN.
+ * D is 64 or 128; f32 arithmetic.  The softmax weights enter the products with 16 bits (bf16 caches), or
+ * with 22 but no finer than 2^-43 of the largest (f16 and 8-bit caches; there that is the largest
+ * product of a weight and its row's scale); exponentials are off by 2^-22 of themselves, logarithms (of
+ * a value's scale, of the sums) by two units of their last place; one rounding at the end; sums are joined
+ * in a fixed order, so results do not vary.
  * partial: 16-byte aligned scratch, f32 words as b200_paged_attention_scratch says for this device
- * (keys = table columns * page_size); it may be 0 words, and null then.  Calls that may overlap need scratch of their own each.
+ * (keys = table columns * page_size); it may be 0 words, and null then.  Calls that may overlap need
+ * scratch of their own each.
  * No counterpart in the reference.
- * slots: q 3, k_cache 4, v_cache 4, k_scale 3, v_scale 3, block_table 2, lengths 1, out 3, lse 2, partial 1, workspace 1.
+ * slots: q 3, k_cache 4, v_cache 4, k_scale 3, v_scale 3, block_table 2, lengths 1, out 3, lse 2, partial 1,
+ * workspace 1.
  */
 int b200_paged_attention_scratch(int64_t batch, int64_t heads, int64_t kv_heads, int64_t head_dim, int64_t keys,
-                                            int32_t store, int64_t *words);
+                                 int32_t store, int64_t *words);
 int b200_paged_attention(const int64_t *slots, int64_t count, float scale, int32_t dtype, int32_t store, void *stream);
 
 /*

@@ -8,7 +8,7 @@
 //
 // Measured for 32768 tokens of 8 heads of 128 columns (bf16 rows, pages of 16 in any order; floors at the
 // 6447 GB/s of a copy): 16 bits written in 41.8 us and read in 44 (41.7); int8 written in 38.5 us, read
-// in 35.4 (31.6); e4m3 written in 34.1, read in 38.5 (31.6).  int8 is written at 84% of the copy's rate, held
+// in 35.4 (31.6); e4m3 written in 34.1, read in 38.5 (31.6).  int8 is written at 82% of the copy's rate, held
 // up by the exact quotients; reading writes two bytes for each that it reads.
 #include "cache.cuh"
 

@@ -32,8 +32,8 @@
 // 4096 keys, 16 heads on each of 8 key heads in e4m3: 73 to 79 us) and 16-bit ones nothing.
 //
 // Measured (device time; floors at the 6447 GB/s of a copy): one sequence of 131072 keys, 32 query and 8 key heads
-// of 128 in bf16: 88.6 us (83.3), of which 85 stream at 6.3 TB/s and 4 join; 64 sequences of 100 to 4096 keys: 88.9
-// (82.9); 64 of 1000 to 8192 in e4m3: 103 (94.1); 1024 keys of one sequence: 8.2 us, all latency; 8 of up to 300, 32 heads
+// of 128 in bf16: 88.8 us (83.3), of which 85 stream at 6.3 TB/s and 4 join; 64 sequences of 100 to 4096 keys: 88.9
+// (82.9); 64 of 1000 to 8192 in e4m3: 103 (94.1); 1024 keys of one sequence: 8.5 us, all latency; 8 of up to 300, 32 heads
 // of 64, whole: 7.1.
 //
 // 8-bit rows.  Codes become f16 exactly on their way into the products.  The query is scaled by a
@@ -120,6 +120,8 @@ struct Border {
 };
 static_assert(sizeof(Border) == 32, "two vectors");
 
+// Good to 2^-22 of the result: a score of 4 in f32 is no better.  The logarithm of a value's scale (__log2f) is off by two
+// units of its last place, 2^-20 for scales of 2^-8, and a weight by as much of itself.
 __device__ __forceinline__ float exp2_fast(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -258,7 +260,8 @@ struct Place {            // where in the sequence of steps a warp is
 // cannot be trusted with them: a weight enters as two numbers that may be 0 or of both signs.  They turn out NaN then,
 // and a thread that finds one in its four columns goes through the piece's rows again: what comes back is the sum of
 // what is not finite there, 0 if nothing is.  An infinite score needs an infinity (or NaN) in its key or query, and one of
-// +infinity makes the denominator NaN, so such a row under an infinite value leaves NaN in any case.
+// +infinity makes the denominator NaN, so such a row under an infinite value leaves NaN in any case.  A block that
+// holds one waits for that: 64 sequences of up to 4096 keys take 780 us instead of 85, and calls without any nothing more.
 __device__ __forceinline__ bool any_special(const void *row, int vectors, uint32_t exponent) {   // exponent: of both halves of a word
   bool found = false;
   for (int i = 0; i < vectors; ++i) {
@@ -955,6 +958,7 @@ paged_attention_join_kernel(const Problem p) {
     }
     state.sum = replaced(state.sum, special);
   }
+  // __fdividef and __log2f: 2 units of the last place, in a few instructions that every block meets cold
   const float base = finite_or_zero(state.top), unit = __fdividef(exp2_fast(finite_or_zero(state.weight_top)), state.denominator);
   T *out = static_cast<T *>(p.out) + cut.b * p.out_batch + head * p.out_head + 4 * lane;
   *reinterpret_cast<uint2 *>(out) = make_uint2(pack<T>(state.sum.x * unit, state.sum.y * unit), pack<T>(state.sum.z * unit, state.sum.w * unit));
@@ -984,8 +988,9 @@ int heads_abreast(int64_t head_tiles, int64_t resident) {
 // 8 sequences of 128 positions 7.5 / 5.1 us, of 256 8.2 / 7.2, of 512 11.1 / 11.1, of 1024 13.4 / 21.4; one of 256 6.9 / 6.9,
 // of 512 7.4 / 10.8; 64 of up to 512 20.8 / 18.0, of 1024 30.5 / 28.9.  In int8: 8 of 256 8.6 / 6.8, of 512 9.7 / 9.5; one of
 // 512 7.8 / 8.9; 64 of up to 512 19.0 / 17.1.  Heads of 64: one sequence of 256 6.4 / 5.8, of 512 6.6 / 8.7; 32 of up to
-// 512 11.1 / 10.0, of 1024 14.9 / 17.6.  It loses where 16 query heads share codes and there are many: 256 sequences of
-// up to 512 in int8 81 / 85.
+// 512 11.1 / 10.0, of 1024 14.9 / 17.6.  Of 64 to 256 sequences of up to 400 and 512, on 1 to 8 key heads of 4 to 24 query heads
+// each, in bf16, int8 and e4m3, whole ones take 2 to 32 % less time, with one exception: where 2048 heads of 16 query heads
+// share codes, seven to a resident block, equal runs even the end out and gain up to 3 % (256 of up to 512 in e4m3 83 / 86).
 bool whole_heads(int64_t heads, int64_t most_keys, int64_t resident) {
   return heads < (1 << 30) && most_keys <= (2 * heads < resident ? 256 : 512);
 }

@@ -566,7 +566,7 @@ def paged_attention(q, k_cache, v_cache, block_table, lengths, scale: float, *, 
     head; head_dim is 64 or 128.  A sequence of length 0 gets zeros (and lse -infinity).  What lies behind a
     sequence, in its last page or in the table, is never used.  A page outside the cache is left out, a length
     past the table is cut there, and ``workspace_status`` reports both; a sequence that has lost all its positions
-    gets NaN.  Returns ``out``, or ``(out, lse)``
+    gets NaN.  Infinite values give infinities; infinities and NaN among the values cost a call time.  Returns ``out``, or ``(out, lse)``
     with the natural logarithm of the sums (f32)."""
     device = _cuda_device(q)
     rows = _float_type("q", q, (torch.float16, torch.bfloat16))

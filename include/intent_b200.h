@@ -358,7 +358,7 @@ int b200_cache_read(const int64_t *slots, int64_t count, int32_t dtype, int32_t 
  * workspace; a sequence that has positions, but all of them absent (if the table has no columns, too),
  * gets NaN and -infinity.  An infinite value of a 16-bit cache gives that infinity, however small its
  * weight, two of both signs NaN, and so does one under a score of -infinity; a call with an infinity or a
- * NaN among its values takes up to ten times as long.  Scales of an 8-bit cache are numbers >= 0 or NaN.
+ * NaN among its values takes about twice as long.  Scales of an 8-bit cache are numbers >= 0 or NaN.
  * D is 64 or 128; f32 arithmetic.  The softmax weights enter the products with 16 bits (bf16 caches), or
  * with 22 but no finer than 2^-43 of the largest (f16 and 8-bit caches; there that is the largest
  * product of a weight and its row's scale); exponentials are off by 2^-22 of themselves, logarithms (of

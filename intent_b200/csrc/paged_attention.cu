@@ -258,57 +258,61 @@ struct Place {            // where in the sequence of steps a warp is
 // Infinities among the values.  A weight is positive however far below the others it lies, so an infinite value gives
 // that infinity; two of both signs give NaN, and so does one under a score of -infinity (0 times it).  The products
 // cannot be trusted with them: a weight enters as two numbers that may be 0 or of both signs.  They turn out NaN then,
-// and a thread that finds one in its four columns goes through the piece's rows again: what comes back is the sum of
-// what is not finite there, 0 if nothing is.  An infinite score needs an infinity (or NaN) in its key or query, and one of
-// +infinity makes the denominator NaN, so such a row under an infinite value leaves NaN in any case.  A block that
-// holds one waits for that: 64 sequences of up to 4096 keys take 780 us instead of 85, and calls without any nothing more.
-__device__ __forceinline__ bool any_special(const void *row, int vectors, uint32_t exponent) {   // exponent: of both halves of a word
+// and the block goes through the piece's rows again: its lanes add up what is not finite in eight columns of every 8th
+// or 16th row each, 0 if nothing is (64 sequences of up to 4096 keys with one such value 175 us instead of 86; calls without
+// any cost nothing).  An infinite score needs an infinity (or NaN) in its key or query, and one of
+// +infinity makes the denominator NaN, so such a row under an infinite value leaves NaN in any case.
+__device__ __forceinline__ bool special(uint32_t pair, uint32_t exponent) {   // exponent: all its bits, of both halves
+  return (pair & exponent & 0xffffu) == (exponent & 0xffffu) || (pair & exponent & 0xffff0000u) == (exponent & 0xffff0000u);
+}
+__device__ __forceinline__ bool special(const uint4 &x, uint32_t exponent) {
+  return special(x.x, exponent) || special(x.y, exponent) || special(x.z, exponent) || special(x.w, exponent);
+}
+template <int VECTORS> __device__ __forceinline__ bool special_row(const void *row, uint32_t exponent) {
   bool found = false;
-  for (int i = 0; i < vectors; ++i) {
-    const uint4 x = static_cast<const uint4 *>(row)[i];
-    const uint32_t words[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-      found |= (words[j] & exponent & 0xffffu) == (exponent & 0xffffu) || (words[j] & exponent & 0xffff0000u) == (exponent & 0xffff0000u);
-  }
+#pragma unroll 1
+  for (int i = 0; i < VECTORS; ++i) found |= special(static_cast<const uint4 *>(row)[i], exponent);
   return found;
 }
+template <typename T> constexpr uint32_t kExponent = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
+
+// Of keys [begin, end) of a head, as many at a time as the block has rows of lanes; `to`: the warp's, (rows of lanes, D).
 template <typename T, int D>
-__device__ __forceinline__ float4 special_values(const Problem &p, int b, int kv_head, int head, int column, int begin, int end) {
-  constexpr int kAtOnce = 4;
-  const uint32_t exponent = std::is_same<T, __half>::value ? 0x7c007c00u : 0x7f807f80u;
-  const bool spoilt = any_special(static_cast<const T *>(p.q) + b * p.q_batch + head * p.q_head, D * 2 / 16, exponent);
-  float sum[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+__device__ __forceinline__ void special_values(const Problem &p, int b, int kv_head, int begin, int end, float *to) {
+  constexpr int kVectors = D * 2 / 16, kRows = 32 / kVectors, kAtOnce = 4, kStride = kWarps * kRows;
+  const int lane = threadIdx.x & 31, vector = lane % kVectors, first = (threadIdx.x >> 5) * kRows + lane / kVectors;
+  float sum[8] = {0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll 1
-  for (int key0 = begin; key0 < end; key0 += kAtOnce) {
+  for (int64_t key0 = begin + first; key0 < end; key0 += kAtOnce * kStride) {
     int entry[kAtOnce], offset[kAtOnce];
-    uint2 raw[kAtOnce];
+    uint4 raw[kAtOnce];
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const int key = min(key0 + i, end - 1), at = key / p.page_size;
-      offset[i] = key - at * p.page_size;
-      entry[i] = p.table[b * p.table_row + at * p.table_column];
+      const int key = (int)min(key0 + i * kStride, (int64_t)end - 1), column = key / p.page_size;
+      entry[i] = key0 + i * kStride < end ? p.table[b * p.table_row + column * p.table_column] : -1;
+      offset[i] = key - column * p.page_size;
     }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      raw[i] = make_uint2(0, 0);
-      if (key0 + i < end && (uint32_t)entry[i] < (uint32_t)p.pages)
-        raw[i] = *reinterpret_cast<const uint2 *>(p.v + entry[i] * p.v_page + kv_head * p.v_head + offset[i] * p.v_slot + column * 2);
+      raw[i] = make_uint4(0, 0, 0, 0);
+      if ((uint32_t)entry[i] < (uint32_t)p.pages)
+        raw[i] = *reinterpret_cast<const uint4 *>(p.v + entry[i] * p.v_page + kv_head * p.v_head + offset[i] * p.v_slot + vector * 16);
     }
 #pragma unroll
     for (int i = 0; i < kAtOnce; ++i) {
-      const float value[4] = {unpack<T>(raw[i].x, 0), unpack<T>(raw[i].x, 1), unpack<T>(raw[i].y, 0), unpack<T>(raw[i].y, 1)};
-      bool any = false;
+      if (!special(raw[i], kExponent<T>)) continue;
+      const bool no_weight = special_row<kVectors>(p.k + entry[i] * p.k_page + kv_head * p.k_head + offset[i] * p.k_slot, kExponent<T>);
+      const uint32_t words[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
 #pragma unroll
-      for (int j = 0; j < 4; ++j) any |= !(fabsf(value[j]) < INFINITY);
-      if (!any) continue;
-      const bool no_weight = spoilt || any_special(p.k + entry[i] * p.k_page + kv_head * p.k_head + offset[i] * p.k_slot, D * 2 / 16, exponent);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-        if (!(fabsf(value[j]) < INFINITY)) sum[j] += no_weight ? NAN : value[j];
+      for (int j = 0; j < 8; ++j) {
+        const float value = unpack<T>(words[j / 2], j % 2);
+        if (!(fabsf(value) < INFINITY)) sum[j] += no_weight ? NAN : value;
+      }
     }
   }
-  return make_float4(sum[0], sum[1], sum[2], sum[3]);
+  float4 *mine = reinterpret_cast<float4 *>(to + (lane / kVectors) * D + vector * 8);
+  mine[0] = make_float4(sum[0], sum[1], sum[2], sum[3]);
+  mine[1] = make_float4(sum[4], sum[5], sum[6], sum[7]);
 }
 __device__ __forceinline__ bool any_nan(const float4 &x) { return isnan(x.x) || isnan(x.y) || isnan(x.z) || isnan(x.w); }
 // sums, with what is not finite in the place of NaN.
@@ -800,6 +804,7 @@ paged_attention_kernel(const Problem p) {
       }
     }
     __syncthreads();
+    bool found = false;
     for (int index = threadIdx.x; index < rows * (D / 4); index += kBlock) {
       const int row = index / (D / 4), column = index % (D / 4) * 4;
       float4 sum = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
@@ -812,10 +817,7 @@ paged_attention_kernel(const Problem p) {
           sum = make_float4(sum.x + x.x, sum.y + x.y, sum.z + x.z, sum.w + x.w);
         }
       }
-      if constexpr (!kCodes)
-        if (any_nan(sum) && units[row] < INFINITY)   // the denominator is a number above 0
-          sum = replaced(sum, special_values<T, D>(p, at.b, kv_head, head0 + row, column, piece_first * S::kStep,
-                                                   min((at.step + 1) * S::kStep, at.length)));
+      if constexpr (!kCodes) found |= any_nan(sum) && units[row] < INFINITY;   // the denominator is a number above 0
       if (whole) {
         const float unit = units[row];
         *reinterpret_cast<uint2 *>(static_cast<T *>(p.out) + at.b * p.out_batch + (head0 + row) * p.out_head + column) =
@@ -824,7 +826,28 @@ paged_attention_kernel(const Problem p) {
         *reinterpret_cast<float4 *>(to + row * partial_floats(D) + column) = sum;
       }
     }
-    __syncthreads();   // the stage, `stats` and `units` are free again
+    if constexpr (kCodes) {
+      __syncthreads();   // the stage, `stats` and `units` are free again
+    } else if (__syncthreads_or(found)) {
+      special_values<T, D>(p, at.b, kv_head, piece_first * S::kStep, min((at.step + 1) * S::kStep, at.length), mine);
+      __syncthreads();
+#pragma unroll 1
+      for (int index = threadIdx.x; index < rows * D; index += kBlock) {
+        const int row = index / D, column = index % D;
+        float extra = 0.0f;
+#pragma unroll
+        for (int w = 0; w < kWarps; ++w)
+#pragma unroll
+          for (int r = 0; r < 32 / S::kChunks; ++r)
+            extra += reinterpret_cast<const float *>(dynamic_smem + (w * S::kStages + stage) * S::kStageBytes)[r * D + column];
+        if (extra == 0.0f || !(units[row] < INFINITY)) continue;
+        if (special_row<D * 2 / 16>(static_cast<const T *>(p.q) + at.b * p.q_batch + (head0 + row) * p.q_head, kExponent<T>)) extra = NAN;
+        T *result = static_cast<T *>(p.out) + at.b * p.out_batch + (head0 + row) * p.out_head + column;
+        if (!whole) to[row * partial_floats(D) + column] = extra;
+        else *result = Element<T>::narrow(extra);
+      }
+      __syncthreads();
+    }
   };
 
   // ---- the run

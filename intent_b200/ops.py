@@ -88,7 +88,7 @@ def workspace(device: torch.device) -> torch.Tensor:
 def _zeroed(device: torch.device) -> torch.Tensor:
     if device.type != "cuda":
         return torch.zeros(_native.WORKSPACE_WORDS, dtype=torch.int32, device=device)
-    with torch.cuda.device(device):
+    with torch.cuda.device(device), torch.inference_mode(False):   # what is made in that mode cannot be cleared outside of it
         if torch.cuda.is_current_stream_capturing():
             return _native.binding().zeroed(device.index, _native.WORKSPACE_WORDS)
         space = torch.zeros(_native.WORKSPACE_WORDS, dtype=torch.int32, device=device)

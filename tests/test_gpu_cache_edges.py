@@ -310,3 +310,25 @@ def test_equal_values_come_back_whatever_the_scores(size, group, dtype, store):
             value = plain.values(case["v_cache"], case["v_scale"])[case["block_table"][0, 0].long(), 0, 0, 0]
             plain.close(out, value.expand(1, group, 64), 2.0 ** -15 + (length + 64) * plain.F32)
             assert lse.isfinite().all()
+
+
+def test_a_first_call_in_inference_mode_leaves_reports_readable_outside():
+    """In a process of its own: status words made in inference mode could not be cleared outside of it."""
+    program = textwrap.dedent("""
+        import torch
+        from intent_b200 import ops
+        cache = torch.zeros(1, 1, 16, 64, device="cuda:0").half()
+        rows, bad = torch.ones(2, 1, 64, device="cuda:0").half(), torch.tensor([1, 99], device="cuda:0")
+        with torch.inference_mode():
+            ops.cache_write(rows, rows, bad, cache, cache.clone())
+        for expected in (True, False):
+            try:
+                ops.workspace_status("cuda:0")
+                reported = False
+            except ValueError as error:
+                reported = "row 1" in str(error)
+            assert reported == expected
+        print("held")
+    """)
+    done = subprocess.run([sys.executable, "-c", program], capture_output=True, text=True, timeout=600, cwd=Path(__file__).resolve().parents[1])
+    assert done.returncode == 0 and "held" in done.stdout, done.stdout + done.stderr

@@ -1,7 +1,7 @@
 // The way from torch tensors to an entry that takes its views as one array of slots
 // (include/intent_b200.h): types, shapes and devices are checked, outputs and scratch allocated, the slots
 // packed and the entry called on torch's current stream, without a Python object a view.  A small call of ten
-// views took 34 us of host time with ctypes and takes 6.4 this way; many of these kernels run for less.
+// views took 34 us of host time with ctypes and takes 6.7 this way; many of these kernels run for less.
 #include <ATen/cuda/EmptyTensor.h>
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
